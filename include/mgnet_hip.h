@@ -793,6 +793,51 @@ int mgn_project_bwd(const float* points, const float* A, const float* t, const f
                     float* d_points, float* partials, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Activations and weights in 8 bits: e4m3 codes with one power-of-two scale per block of 128 (csrc/q8.hip)
+ *   block = 128 neighbouring channels of one row of an [M, C] matrix, or a 128 x 128 tile of a weight matrix; with a = the block's largest
+ *   finite magnitude, e = max(-111, smallest e with a <= 448 * 2^e), code = e4m3(x / 2^e) (nearest, ties to even), value = code * 2^e.
+ *   Magnitudes above 1.875 * 2^127 (fp16: 1.875 * 2^15) count as that number; NaN and infinities become NaN.
+ * codes  : [M][ldc] bytes, ldc = C rounded up to 16, zero behind column C;  scales : [ceil(C / 128)][lds] bytes e + 127, lds = M rounded
+ *   up to 16 (bytes behind row M are unspecified).  Both 16-byte aligned; sizes from mgn_q8_bytes.  M <= 0x7fffff00, C <= 2^20.
+ * mgn_q8_pack       : x (dtype 0 = fp32, 1 = 16-bit); row r = pixel (n, h, w) of a map with element strides sn, sh, sw and unit channel
+ *                     stride, r = (n * H + h) * W + w (a plain matrix: H = W = 1, sn = row stride).  Any alignment of the element type.
+ * mgn_q8_unpack     : the values, y [M][C] contiguous (dtype as above).
+ * mgn_q8_pack_weight: w [N][K] with element strides sr, sc -> tile scales; codes/scales of [N][K] and / or codes_t/scales_t of its
+ *                     transpose [K][N] (the same values).  A pair may be NULL.
+ * mgn_q8_matmul     : out[m][n] = act( sum_k a[m][k] b[n][k] + bias[n] ), a [M][K], b [N][K] packed, fp32 accumulation, one rounding;
+ *                     act 0 none | 1 ReLU | 2 leaky ReLU; out fp32 or 16-bit, rows ldo elements apart.
+ * mgn_q8_wgrad      : dw[n][k] = sum_m dy[m][n] x[m][k] with dy 16-bit (rows ldy elements apart, ldy % 8 == 0, 16-byte aligned; columns
+ *                     N .. ldy are ignored) and x packed; db[n] = sum_m dy[m][n] (nullable).  Fixed summation order.
+ * ---------------------------------------------------------------------------------------------- */
+int mgn_q8_bytes(long M, int C, size_t* codes, size_t* scales);
+int mgn_q8_pack(const void* x, int dtype, long M, int C, long sn, long sh, long sw, int H, int W, void* codes, void* scales, void* stream);
+int mgn_q8_unpack(const void* codes, const void* scales, long M, int C, void* y, int dtype, void* stream);
+int mgn_q8_pack_weight(const void* w, int dtype, long sr, long sc, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t, void* stream);
+int mgn_q8_matmul(const void* a, const void* a_scales, long M, const void* b, const void* b_scales, int N, int K, const float* bias, int act, float slope,
+                  void* out, int out_f32, long ldo, void* stream);
+int mgn_q8_wgrad_workspace_bytes(long M, int N, int K, size_t* bytes);
+int mgn_q8_wgrad(const void* dy, long ldy, long M, int N, const void* codes, const void* scales, int K, float* dw, float* db, void* workspace,
+                 size_t workspace_bytes, void* stream);
+/* Block tail y = relu(norm(x) + shortcut) (res_net.py:62-79) that keeps x in 8 bits for its backward pass.  All maps [M, C] channels-last,
+ * 16-bit, 16-byte aligned, C % 8 == 0, C <= 8192.
+ *   stats      : partials[rows][C][2] (rows = mgn_q8_tail_partial_rows) of (x - shift), (x - shift)^2 and shift[C] = x's first row, the
+ *                input of mgn_iabn_coeffs_from_partials
+ *   fwd        : y = relu(scale * x + offset + shortcut) (one rounding), x packed, relu_bits: one byte per 8 outputs, bit k = (y[k] > 0);
+ *                codes, scales and relu_bits all NULL: y alone (inference)
+ *   bwd_reduce : dz = g * (y > 0) (the shortcut's gradient); sums[2][C] = { sum dz, sum dz * x_hat } with x_hat = (packed x - mean) * rstd;
+ *                dwb[2][C] = { d weight, d bias } of this rank; partials as above (scratch)
+ *   bwd_apply  : dx = (|weight| + eps) * rstd * (dz - sums[0] / n - x_hat * sums[1] / n), n = total_count (all ranks) */
+int mgn_q8_tail_partial_rows(long M, int C, int* rows);
+int mgn_q8_tail_stats(const void* x, long M, int C, float* partials, float* shift, void* stream);
+int mgn_q8_tail_fwd(const void* x, const void* shortcut, const float* scale, const float* offset, long M, int C, void* y, void* codes, void* scales,
+                    void* relu_bits, void* stream);
+int mgn_q8_tail_bwd_reduce(const void* codes, const void* scales, const void* g, const void* relu_bits, const float* mean, const float* rstd,
+                           const float* weight, long M, int C, void* dz, float* partials, float* sums, float* dwb, void* stream);
+int mgn_q8_tail_sums(const float* partials, int rows, int C, const float* rstd, const float* weight, float* sums, float* dwb, void* stream);
+int mgn_q8_tail_bwd_apply(const void* codes, const void* scales, const void* dz, const float* weight, const float* mean, const float* rstd,
+                          const float* sums, float total_count, float eps, long M, int C, void* dx, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * IEEE fp16 activations -- the reference's AMP format (configs/MGNet-*.yaml SOLVER.AMP.ENABLED -> torch.cuda.amp: fp16 +
  * GradScaler, tools/train_net.py:162).  Every entry point above that reads or writes 16-bit activations has a twin with the
  * suffix _f16, identical in signature and semantics, in which "bf16" reads "IEEE fp16" (weight layouts included:
@@ -891,6 +936,21 @@ int mgn_iabn_bwd_apply_f16(const void* y, const void* dy, void* dx /*may alias d
 int mgn_iabn_bwd_apply_x_f16(const void* x, const void* dy, void* dx, int dtype, long M, int C, const float* weight,
     const float* bias, const float* scale, const float* offset, const float* saved, const float* sums, float
     total_count, float eps, int activation, float slope, void* stream);
+int mgn_q8_pack_f16(const void* x, int dtype, long M, int C, long sn, long sh, long sw, int H, int W, void* codes, void* scales, void* stream);
+int mgn_q8_unpack_f16(const void* codes, const void* scales, long M, int C, void* y, int dtype, void* stream);
+int mgn_q8_pack_weight_f16(const void* w, int dtype, long sr, long sc, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t, void*
+    stream);
+int mgn_q8_matmul_f16(const void* a, const void* a_scales, long M, const void* b, const void* b_scales, int N, int K, const float* bias, int act,
+    float slope, void* out, int out_f32, long ldo, void* stream);
+int mgn_q8_wgrad_f16(const void* dy, long ldy, long M, int N, const void* codes, const void* scales, int K, float* dw, float* db, void* workspace,
+    size_t workspace_bytes, void* stream);
+int mgn_q8_tail_stats_f16(const void* x, long M, int C, float* partials, float* shift, void* stream);
+int mgn_q8_tail_fwd_f16(const void* x, const void* shortcut, const float* scale, const float* offset, long M, int C, void* y, void* codes, void*
+    scales, void* relu_bits, void* stream);
+int mgn_q8_tail_bwd_reduce_f16(const void* codes, const void* scales, const void* g, const void* relu_bits, const float* mean, const float* rstd,
+    const float* weight, long M, int C, void* dz, float* partials, float* sums, float* dwb, void* stream);
+int mgn_q8_tail_bwd_apply_f16(const void* codes, const void* scales, const void* dz, const float* weight, const float* mean, const float* rstd, const
+    float* sums, float total_count, float eps, long M, int C, void* dx, void* stream);
 
 #ifdef __cplusplus
 }

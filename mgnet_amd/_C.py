@@ -31,8 +31,9 @@ SYMBOLS = ["mgn_version", "mgn_reproj_workspace_bytes", "mgn_reproj_loss_fwd", "
            "mgn_plan_begin", "mgn_plan_recorded", "mgn_plan_current", "mgn_plan_end", "mgn_plan_abort", "mgn_plan_node_count", "mgn_plan_node_info", "mgn_plan_node_args",
            "mgn_plan_compile", "mgn_plan_set_stream", "mgn_plan_run", "mgn_plan_prof_elapsed", "mgn_plan_free",
            "mgn_plan_trace", "mgn_plan_trace_read", "mgn_plan_set_skip", "mgn_plan_node_ro", "mgn_plan_node_ro_family", "mgn_plan_set_jitter", "mgn_plan_probe",
-           "mgn_abn_apply_pool", "mgn_att_abn_bwd_stats", "mgn_att_abn_bwd_sums", "mgn_att_abn_bwd_apply"]
-SYMBOLS_F16 = [n + "_f16" for n in ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply']]
+           "mgn_abn_apply_pool", "mgn_att_abn_bwd_stats", "mgn_att_abn_bwd_sums", "mgn_att_abn_bwd_apply",
+           "mgn_q8_bytes", "mgn_q8_pack", "mgn_q8_unpack", "mgn_q8_pack_weight", "mgn_q8_matmul", "mgn_q8_wgrad_workspace_bytes", "mgn_q8_wgrad", "mgn_q8_tail_partial_rows", "mgn_q8_tail_stats", "mgn_q8_tail_fwd", "mgn_q8_tail_bwd_reduce", "mgn_q8_tail_sums", "mgn_q8_tail_bwd_apply"]
+SYMBOLS_F16 = [n + "_f16" for n in ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply']]
 DEPTH_MAX_FILTER_IDS = 16
 MGN_MAX_TASKS = 8   # include/mgnet_hip.h
 
@@ -85,7 +86,7 @@ def plan_touch(reads=(), writes=()):
 
 
 H16 = (torch.bfloat16, torch.float16)   # the 16-bit activation formats: bf16 entry points, or their _f16 twins (csrc/h16.h)
-F16_TWINS = ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply']
+F16_TWINS = ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply']
 
 
 def _fn(name, t):
@@ -237,6 +238,19 @@ def lib():
         L.mgn_att_abn_bwd_stats.argtypes = [vp, vp, vp, vp, cf, ci, cf, ci, cl, ci, vp, vp, sz, vp]
         L.mgn_att_abn_bwd_sums.argtypes = [vp, vp, vp, ci, ci, ci, vp, vp, vp, vp]
         L.mgn_att_abn_bwd_apply.argtypes = [vp, vp, vp, vp, vp, ci, vp, vp, vp, vp, cf, cf, ci, cf, ci, cl, ci, vp]
+        L.mgn_q8_bytes.argtypes = [cl, ci, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        L.mgn_q8_pack.argtypes = [vp, ci, cl, ci, cl, cl, cl, ci, ci, vp, vp, vp]
+        L.mgn_q8_unpack.argtypes = [vp, vp, cl, ci, vp, ci, vp]
+        L.mgn_q8_pack_weight.argtypes = [vp, ci, cl, cl, ci, ci, vp, vp, vp, vp, vp]
+        L.mgn_q8_matmul.argtypes = [vp, vp, cl, vp, vp, ci, ci, vp, ci, cf, vp, ci, cl, vp]
+        L.mgn_q8_wgrad_workspace_bytes.argtypes = [cl, ci, ci, ctypes.POINTER(sz)]
+        L.mgn_q8_wgrad.argtypes = [vp, cl, cl, ci, vp, vp, ci, vp, vp, vp, sz, vp]
+        L.mgn_q8_tail_partial_rows.argtypes = [cl, ci, ctypes.POINTER(ci)]
+        L.mgn_q8_tail_stats.argtypes = [vp, cl, ci, vp, vp, vp]
+        L.mgn_q8_tail_fwd.argtypes = [vp, vp, vp, vp, cl, ci, vp, vp, vp, vp, vp]
+        L.mgn_q8_tail_bwd_reduce.argtypes = [vp, vp, vp, vp, vp, vp, vp, cl, ci, vp, vp, vp, vp, vp]
+        L.mgn_q8_tail_sums.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
+        L.mgn_q8_tail_bwd_apply.argtypes = [vp, vp, vp, vp, vp, vp, vp, cf, cf, cl, ci, vp, vp]
         for n in SYMBOLS[4:]:
             getattr(L, n).restype = ci
         L.mgn_p2p_mailbox_bytes.restype = sz
@@ -1603,3 +1617,100 @@ def project_bwd(points, A, t, g):
     check(lib().mgn_project_bwd(points.data_ptr(), A.data_ptr(), t.data_ptr(), _dev_f32(g, "grad").data_ptr(), B, H, W,
                                 d_pts.data_ptr(), part.data_ptr(), _stream()), "mgn_project_bwd")
     return (d_pts,) + _geo_sum(part)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# 8-bit codes with a power-of-two scale per block of 128 (csrc/q8.hip; ops.Q8Map)
+# ---------------------------------------------------------------------------------------------------------------
+def q8_alloc(M, C, device):
+    """empty (codes [M, ldc], scales [ceil(C/128), lds]) of an [M, C] matrix"""
+    return (torch.empty((M, (C + 15) // 16 * 16), dtype=torch.uint8, device=device),
+            torch.empty(((C + 127) // 128, (M + 15) // 16 * 16), dtype=torch.uint8, device=device))
+
+
+def q8_pack(x, M, C, sn, sh, sw, H, W):
+    """row (n, h, w) of x (element strides sn, sh, sw; unit channel stride) -> codes, scales"""
+    codes, scales = q8_alloc(M, C, x.device)
+    check(_fn("mgn_q8_pack", x)(x.data_ptr(), _act_dtype(x), M, C, sn, sh, sw, H, W, codes.data_ptr(), scales.data_ptr(), _stream()), "mgn_q8_pack")
+    return codes, scales
+
+
+def q8_unpack(codes, scales, M, C, out):
+    check(_fn("mgn_q8_unpack", out)(codes.data_ptr(), scales.data_ptr(), M, C, out.data_ptr(), _act_dtype(out), _stream()), "mgn_q8_unpack")
+    return out
+
+
+def q8_pack_weight(w, plain=True, transposed=False):
+    """w [N, K] (any strides) -> (codes, scales) of w and / or of its transpose, scales per 128 x 128 tile"""
+    N, K = w.shape
+    a = q8_alloc(N, K, w.device) if plain else (None, None)
+    t = q8_alloc(K, N, w.device) if transposed else (None, None)
+    p = lambda z: None if z is None else z.data_ptr()
+    check(_fn("mgn_q8_pack_weight", w)(w.data_ptr(), _act_dtype(w), w.stride(0), w.stride(1), N, K, p(a[0]), p(a[1]), p(t[0]), p(t[1]), _stream()),
+          "mgn_q8_pack_weight")
+    return a, t
+
+
+def q8_matmul(a, a_scales, M, b, b_scales, N, K, bias, act, slope, out):
+    """out [M, N] (rows out.stride(0) apart) = act(a b^T + bias)"""
+    check(_fn("mgn_q8_matmul", out)(a.data_ptr(), a_scales.data_ptr(), M, b.data_ptr(), b_scales.data_ptr(), N, K,
+                                    None if bias is None else bias.data_ptr(), act, float(slope), out.data_ptr(), int(out.dtype == torch.float32),
+                                    out.stride(0), _stream()), "mgn_q8_matmul")
+    return out
+
+
+def q8_wgrad(dy, ldy, M, N, codes, scales, K, want_db=True):
+    """dy: 16-bit rows of ldy elements -> dw [N, K], db [N] (or None), fp32"""
+    dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
+    db = torch.empty(N, dtype=torch.float32, device=dy.device) if want_db else None
+    nb = ctypes.c_size_t(0)
+    check(lib().mgn_q8_wgrad_workspace_bytes(M, N, K, ctypes.byref(nb)), "mgn_q8_wgrad_workspace_bytes")
+    ws = torch.empty(nb.value, dtype=torch.uint8, device=dy.device)
+    check(_fn("mgn_q8_wgrad", dy)(dy.data_ptr(), ldy, M, N, codes.data_ptr(), scales.data_ptr(), K, dw.data_ptr(), None if db is None else db.data_ptr(),
+                                  ws.data_ptr(), nb.value, _stream()), "mgn_q8_wgrad")
+    return dw, db
+
+
+def _q8_tail_partials(M, C, device):
+    rows = ctypes.c_int(0)
+    check(lib().mgn_q8_tail_partial_rows(M, C, ctypes.byref(rows)), "mgn_q8_tail_partial_rows")
+    return torch.empty((rows.value, C, 2), dtype=torch.float32, device=device)
+
+
+def q8_tail_stats(x, M, C):
+    """(partials, shift) of the batch statistics of x [M, C], the arguments of iabn_from_partials"""
+    part = _q8_tail_partials(M, C, x.device)
+    shift = torch.empty(C, dtype=torch.float32, device=x.device)
+    check(_fn("mgn_q8_tail_stats", x)(x.data_ptr(), M, C, part.data_ptr(), shift.data_ptr(), _stream()), "mgn_q8_tail_stats")
+    return part, shift
+
+
+def q8_tail_fwd(x, shortcut, coef, M, C, keep):
+    """relu(coef[0] * x + coef[1] + shortcut); keep: also (codes, scales) of x and the ReLU mask -> (y, codes, scales, bits)"""
+    y = torch.empty_like(x)
+    codes = scales = bits = None
+    if keep:
+        codes, scales = q8_alloc(M, C, x.device)
+        bits = torch.empty(M * C // 8, dtype=torch.uint8, device=x.device)
+    p = lambda t: None if t is None else t.data_ptr()
+    check(_fn("mgn_q8_tail_fwd", x)(x.data_ptr(), shortcut.data_ptr(), coef[0].data_ptr(), coef[1].data_ptr(), M, C, y.data_ptr(), p(codes), p(scales),
+                                    p(bits), _stream()), "mgn_q8_tail_fwd")
+    return y, codes, scales, bits
+
+
+def q8_tail_bwd_reduce(codes, scales, g, bits, coef, weight, M, C):
+    """-> (dz, sums [2, C], d_weight, d_bias)"""
+    dz = torch.empty_like(g)
+    part = _q8_tail_partials(M, C, g.device)
+    out = torch.empty((4, C), dtype=torch.float32, device=g.device)
+    check(_fn("mgn_q8_tail_bwd_reduce", g)(codes.data_ptr(), scales.data_ptr(), g.data_ptr(), bits.data_ptr(), coef[2].data_ptr(), coef[3].data_ptr(),
+                                           weight.data_ptr(), M, C, dz.data_ptr(), part.data_ptr(), out.data_ptr(), out[2].data_ptr(), _stream()),
+          "mgn_q8_tail_bwd_reduce")
+    return dz, out[:2], out[2], out[3]
+
+
+def q8_tail_bwd_apply(codes, scales, dz, weight, coef, sums, total_count, eps, M, C):
+    dx = torch.empty_like(dz)
+    check(_fn("mgn_q8_tail_bwd_apply", dz)(codes.data_ptr(), scales.data_ptr(), dz.data_ptr(), weight.data_ptr(), coef[2].data_ptr(), coef[3].data_ptr(),
+                                           sums.data_ptr(), float(total_count), float(eps), M, C, dx.data_ptr(), _stream()), "mgn_q8_tail_bwd_apply")
+    return dx

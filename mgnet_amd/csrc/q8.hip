@@ -1,0 +1,1142 @@
+// q8.hip -- activations and weights held in 8 bits with one power-of-two scale per block of 128, the matrix product that reads them and
+// the backward passes that read them instead of 16-bit activations.
+//
+// The format.  A block is 128 neighbouring channels of one row of an [M, C] matrix (a channels-last map is one, M = N*H*W), or a 128 x 128
+// tile of a weight matrix.  With a = the largest finite magnitude of the block,
+//     e = max(-111, smallest e with a <= 448 * 2^e),       code = e4m3(x / 2^e), round to nearest even,      x^ = code * 2^e.
+// Why a power of two: x / 2^e and x^ are exact, so rounding to the code is the ONLY rounding (relative 2^-4 down to 2^-6 * 2^e); x^ has 4
+// significant bits and is therefore a bf16 number (and an fp16 number, if x was one), so the 16-bit matrix cores consume it without a
+// second rounding; and 2^e is what the block-scaled MFMA of gfx950 takes as its E8M0 operand, so a scale costs the product no VALU work.
+// The smallest e keeps x^ in (224, 448] * 2^e for the largest element: nothing saturates, the top element keeps its 2^-4 as well.
+//   magnitudes above the largest e4m3 multiple of the source type (1.875 * 2^127; fp16 1.875 * 2^15) count as that number -- rounding up
+//   would give the type's infinity; NaN and infinities become the NaN code, and take no part in a; e >= -111 keeps every scale and every
+//   non-zero x^ (>= 2^-120) a normal fp32 number: magnitudes under 2^-121 are zero.
+//
+// Layout: codes [M][ldc] bytes, ldc = C rounded up to 16 (the tail is zero: 16-byte loads never need a column mask); scales
+// [ceil(C/128)][lds] bytes, lds = M rounded up to 16, biased by 127 -- block-major, so that a tile's rows of one block are one contiguous
+// run.  A weight matrix has the same layout (a 128 x 128 tile's scale repeated for its 128 rows): both operands of the product are read by
+// the same code, and because a tile's scale serves rows and columns alike the transposed matrix has the same values.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "h16.h"
+#include "mgnet_hip.h"
+
+namespace {
+
+constexpr int TPB = 256;
+constexpr int BLK = 128;                  // channels per scale
+constexpr int RPG = 8;                    // rows per lane group of the streaming kernels: 8 loads in flight, 8 scale bytes per store
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+constexpr int OOB = (int)0x80000000;      // an offset no buffer descriptor below admits: such a load returns (or leaves in LDS) zeros
+
+#ifdef MGN_F16
+constexpr float TOP16 = 61440.f;          // largest e4m3 multiple below the type's largest finite number
+#else
+constexpr float TOP16 = 1.875f * 1.7014118346046923e38f;
+#endif
+constexpr float TOP32 = 1.875f * 1.7014118346046923e38f;
+
+__device__ __forceinline__ float pow2(uint32_t biased) { return __uint_as_float(biased << 23); }
+// biased exponent of the scale: a <= 1.75 * 2^E  <=>  the mantissa bits of a do not exceed 0x600000
+__device__ __forceinline__ uint32_t scale_of(uint32_t amax_bits) {
+    const uint32_t e = (amax_bits + 0x1fffffu) >> 23;
+    return e < 24u ? 16u : e - 8u;
+}
+__device__ __forceinline__ float inv_scale(uint32_t s) { return pow2(254u - s); }
+
+// eight values -> their codes; |v| <= top for finite ones
+__device__ __forceinline__ uint2 encode8(const float (&f)[8], float inv, float top) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float c = __builtin_amdgcn_fmed3f(f[k], -top, top) * inv;
+        v[k] = (__float_as_uint(f[k]) & 0x7fffffffu) < 0x7f800000u ? c : __uint_as_float(0x7fc00000u);
+    }
+    uint2 r;
+    r.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    r.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], (int)r.x, true);
+    r.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+    r.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], (int)r.y, true);
+    return r;
+}
+__device__ __forceinline__ void decode8(uint2 c, float sc, float (&v)[8]) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, true);
+    const f32x2 d = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, true);
+    v[0] = a[0] * sc; v[1] = a[1] * sc; v[2] = b[0] * sc; v[3] = b[1] * sc;
+    v[4] = d[0] * sc; v[5] = d[1] * sc; v[6] = e[0] * sc; v[7] = e[1] * sc;
+}
+__device__ __forceinline__ uint32_t amax8(const float (&f)[8], float top) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t u = __float_as_uint(f[k]) & 0x7fffffffu;
+        const uint32_t w = u < 0x7f800000u ? u : 0u;
+        m = m > w ? m : w;
+    }
+    const uint32_t t = __float_as_uint(top);
+    return m < t ? m : t;
+}
+// maximum over LPB neighbouring lanes (4, 8 or 16: inside one DPP row), left in all of them
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t m) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, 0xf, 0xf, true);
+    return m > o ? m : o;
+}
+template <int LPB>
+__device__ __forceinline__ uint32_t group_max(uint32_t m) {
+    m = dpp_max<0xB1>(m);                 // quad: neighbour
+    m = dpp_max<0x4E>(m);                 // quad: other pair
+    if (LPB >= 8) m = dpp_max<0x141>(m);  // half row mirrored
+    if (LPB >= 16) m = dpp_max<0x140>(m); // row mirrored
+    return m;
+}
+
+__device__ __forceinline__ void unpack8(const uint4& r, float (&v)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) { v[2 * k] = mgn_lo2f(w[k]); v[2 * k + 1] = mgn_hi2f(w[k]); }
+}
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+    return make_uint4(mgn_pack2(v[0], v[1]), mgn_pack2(v[2], v[3]), mgn_pack2(v[4], v[5]), mgn_pack2(v[6], v[7]));
+}
+
+// ------------------------------------------------------------------------------------------------------
+// x -> codes, scales.  One pass: a group of LPB lanes owns one block of 8 consecutive rows (8 channels a lane), so a block's maximum is
+// four DPP steps and its eight scales leave in one store; the 8 rows are 8 independent 16-byte loads per lane.  Bound by HBM (3 bytes per
+// 16-bit value).
+// ------------------------------------------------------------------------------------------------------
+struct RowMap {                           // row r of the matrix = pixel (n, h, w) of a map with these strides (elements)
+    long sn, sh, sw;
+    int H, W;
+    int flat;                             // 1: row r starts at r * sw
+};
+__device__ __forceinline__ long row_offset(const RowMap& m, int r) {
+    if (m.flat) return (long)r * m.sw;
+    const int q = r / m.W, w = r - q * m.W, n = q / m.H, h = q - n * m.H;
+    return (long)n * m.sn + (long)h * m.sh + (long)w * m.sw;
+}
+
+template <typename T> struct Src;
+template <> struct Src<float> {
+    struct Raw { float4 a, b; };
+    static constexpr float TOP = TOP32;
+    __device__ static Raw zero() { return Raw{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)}; }
+    __device__ static Raw load(const float* p) { return Raw{reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]}; }
+    __device__ static float one(const float* p) { return *p; }
+    __device__ static void get(const Raw& r, float (&v)[8]) {
+        v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; v[4] = r.b.x; v[5] = r.b.y; v[6] = r.b.z; v[7] = r.b.w;
+    }
+};
+template <> struct Src<uint16_t> {
+    struct Raw { uint4 a; };
+    static constexpr float TOP = TOP16;
+    __device__ static Raw zero() { return Raw{make_uint4(0, 0, 0, 0)}; }
+    __device__ static Raw load(const uint16_t* p) { return Raw{*reinterpret_cast<const uint4*>(p)}; }
+    __device__ static float one(const uint16_t* p) { return mgn_h2f(*p); }
+    __device__ static void get(const Raw& r, float (&v)[8]) { unpack8(r.a, v); }
+};
+
+template <typename T, int LPB, bool VEC>
+__global__ __launch_bounds__(TPB) void q8_pack(const T* __restrict__ x, RowMap map, int M, int C, int nb, int ldc, long lds,
+                                               unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
+    const long gid = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
+    const int l = threadIdx.x % LPB;
+    const int kb = (int)(gid % nb);
+    const long r0l = gid / nb * RPG;
+    if (r0l >= M) return;                 // (whole groups leave together: the DPP steps below stay inside one group)
+    const int r0 = (int)r0l, c0 = kb * BLK + l * 8;
+    uint32_t sb[RPG];
+    auto finish = [&](int j, const float (&f)[8]) {
+        const uint32_t s = scale_of(group_max<LPB>(amax8(f, Src<T>::TOP)));
+        sb[j] = s;
+        if (r0 + j < M && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = encode8(f, inv_scale(s), Src<T>::TOP);
+    };
+    if (VEC) {                            // C % 8 == 0 and 16-byte aligned rows
+        typename Src<T>::Raw q[RPG];
+#pragma unroll
+        for (int j = 0; j < RPG; ++j) q[j] = (r0 + j < M && c0 < C) ? Src<T>::load(x + row_offset(map, r0 + j) + c0) : Src<T>::zero();
+#pragma unroll
+        for (int j = 0; j < RPG; ++j) {
+            float f[8];
+            Src<T>::get(q[j], f);
+            finish(j, f);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < RPG; ++j) {
+            float f[8];
+            const T* p = x + (r0 + j < M ? row_offset(map, r0 + j) : 0) + c0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = (r0 + j < M && c0 + k < C) ? Src<T>::one(p + k) : 0.f;
+            finish(j, f);
+        }
+    }
+    if (l == 0) {                         // lds is a multiple of 16: eight bytes from a row that is a multiple of 8 stay inside it
+        const uint2 w = make_uint2(sb[0] | (sb[1] << 8) | (sb[2] << 16) | (sb[3] << 24), sb[4] | (sb[5] << 8) | (sb[6] << 16) | (sb[7] << 24));
+        *reinterpret_cast<uint2*>(scales + kb * lds + r0) = w;
+    }
+}
+
+// codes, scales -> x^ [M][C] (rows of C contiguous values); the mirror image of q8_pack
+template <typename T, int LPB, bool VEC>
+__global__ __launch_bounds__(TPB) void q8_unpack(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, int M, int C,
+                                                 int nb, int ldc, long lds, T* __restrict__ y) {
+    const long gid = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
+    const int l = threadIdx.x % LPB;
+    const int kb = (int)(gid % nb);
+    const long r0l = gid / nb * RPG;
+    if (r0l >= M) return;
+    const int r0 = (int)r0l, c0 = kb * BLK + l * 8;
+    if (c0 >= C) return;
+    const uint2 w = *reinterpret_cast<const uint2*>(scales + kb * lds + r0);
+    uint2 q[RPG];
+#pragma unroll
+    for (int j = 0; j < RPG; ++j) q[j] = r0 + j < M ? *reinterpret_cast<const uint2*>(codes + (long)(r0 + j) * ldc + c0) : make_uint2(0, 0);
+#pragma unroll
+    for (int j = 0; j < RPG; ++j) {
+        if (r0 + j >= M) break;
+        float v[8];
+        decode8(q[j], pow2(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), v);
+        T* p = y + (long)(r0 + j) * C + c0;
+        if constexpr (sizeof(T) == 2) {
+            const uint4 o = pack8(v);
+            if (VEC) *reinterpret_cast<uint4*>(p) = o;
+            else {
+                const uint32_t u[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int k = 0; k < 8; ++k) if (c0 + k < C) p[k] = (T)(u[k >> 1] >> (16 * (k & 1)));
+            }
+        } else {
+            if (VEC) {
+                reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) if (c0 + k < C) p[k] = v[k];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------
+// a weight matrix W [N][K] (any strides) -> codes [N][ldc(K)] + scales [ceil(K/128)][lds(N)], and the same values transposed: codes
+// [K][ldc(N)] + scales [ceil(N/128)][lds(K)] (what the data gradient multiplies by).  A block per 128 x 128 tile; the tile goes through
+// LDS once so that both outputs leave in 16-byte stores.
+// ------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(TPB) void q8_pack_tile(const T* __restrict__ w, long sr, long sc, int N, int K, unsigned char* __restrict__ codes,
+                                                    unsigned char* __restrict__ scales, unsigned char* __restrict__ codes_t,
+                                                    unsigned char* __restrict__ scales_t) {
+    constexpr int PITCH = BLK + 16;       // (rows of 16-byte chunks; the transposing byte reads then spread over the banks)
+    __shared__ __attribute__((aligned(16))) unsigned char tile[BLK * PITCH];
+    __shared__ uint32_t part[TPB / 64];
+    const int n0 = blockIdx.x * BLK, k0 = blockIdx.y * BLK, tid = threadIdx.x;
+    const int ldk = (K + 15) & ~15, ldn = (N + 15) & ~15;
+    float f[64];
+    uint32_t m = 0;
+    // (lanes run along whichever axis is contiguous)
+    const bool kfast = sc == 1;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+        const int fast = tid & 127, slow = i * 2 + (tid >> 7);
+        const int r = kfast ? slow : fast, c = kfast ? fast : slow;
+        f[i] = (n0 + r < N && k0 + c < K) ? Src<T>::one(w + (long)(n0 + r) * sr + (long)(k0 + c) * sc) : 0.f;
+        const uint32_t u = __float_as_uint(f[i]) & 0x7fffffffu, v = u < 0x7f800000u ? u : 0u;
+        m = m > v ? m : v;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { const uint32_t o = (uint32_t)__shfl_xor((int)m, d); m = m > o ? m : o; }
+    if ((tid & 63) == 0) part[tid >> 6] = m;
+    __syncthreads();
+    m = part[0];
+#pragma unroll
+    for (int k = 1; k < TPB / 64; ++k) m = m > part[k] ? m : part[k];
+    const uint32_t top = __float_as_uint(Src<T>::TOP);
+    const uint32_t s = scale_of(m < top ? m : top);
+    const float inv = inv_scale(s);
+#pragma unroll
+    for (int i = 0; i < 64; i += 8) {
+        float g[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[k] = f[i + k];
+        const uint2 e = encode8(g, inv, Src<T>::TOP);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int fast = tid & 127, slow = (i + k) * 2 + (tid >> 7);
+            const int r = kfast ? slow : fast, c = kfast ? fast : slow;
+            tile[r * PITCH + c] = (unsigned char)((k < 4 ? e.x : e.y) >> (8 * (k & 3)));
+        }
+    }
+    __syncthreads();
+    for (int p = tid; p < BLK * (BLK / 16); p += TPB) {
+        const int r = p >> 3, ch = (p & 7) * 16;
+        if (codes && n0 + r < N && k0 + ch < ldk)
+            *reinterpret_cast<uint4*>(codes + (long)(n0 + r) * ldk + k0 + ch) = *reinterpret_cast<const uint4*>(tile + r * PITCH + ch);
+        if (codes_t && k0 + r < K && n0 + ch < ldn) {
+            uint32_t o[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const unsigned char* t = tile + (ch + 4 * q) * PITCH + r;
+                o[q] = (uint32_t)t[0] | ((uint32_t)t[PITCH] << 8) | ((uint32_t)t[2 * PITCH] << 16) | ((uint32_t)t[3 * PITCH] << 24);
+            }
+            *reinterpret_cast<uint4*>(codes_t + (long)(k0 + r) * ldn + n0 + ch) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    if (tid < BLK) {
+        if (codes && n0 + tid < N) scales[(long)blockIdx.y * ldn + n0 + tid] = (unsigned char)s;
+        if (codes_t && k0 + tid < K) scales_t[(long)blockIdx.x * ldk + k0 + tid] = (unsigned char)s;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------
+// out[m][n] = act( sum_k A[m][k] B[n][k] + bias[n] )
+//   v_mfma_scale_f32_32x32x64_f8f6f4 with the two blocks' exponents as its E8M0 operands: products of codes scaled in the matrix core,
+//   fp32 accumulation, one rounding at the end.  B's rows are the instruction's rows and A's its columns, so a lane ends up with 4
+//   consecutive n of one m.  The k order inside a block is free (both operands are read alike and share the block's scale).
+//   Precision, measured on the instruction: it adds the products of 8 neighbouring k before they join the fp32 accumulator, each cut
+//   towards zero to a multiple of 2^-13 of the largest one's binade.  1.3e-5 of a result (2-norm, Gaussian operands): far below the
+//   rounding to 16 bits (1.7e-3 / 2.1e-4) and the operands' own (2.6e-2); a 32-bit result carries it.
+// ------------------------------------------------------------------------------------------------------
+struct MmParams {
+    const unsigned char *a, *sa, *b, *sb;
+    const float* bias;
+    void* out;
+    int M, N, K, nb, ld;                  // ld: bytes per code row (both operands)
+    long lda_s, ldb_s, ldo;               // scale rows; elements per row of out
+    int act, out32, vec;                  // vec: rows of out are 4-element aligned
+    float slope;
+    int mt, nt, group;
+};
+MGN_PLAN_RO(MmParams, MGN_RO(a) MGN_RO(sa) MGN_RO(b) MGN_RO(sb) MGN_RO(bias))
+
+__device__ __forceinline__ float activate(float v, int act, float slope) { return act == 0 ? v : (v > 0.f ? v : (act == 1 ? (v == v ? 0.f : v) : v * slope)); }
+
+// four consecutive n of row m
+__device__ __forceinline__ void mm_emit(const MmParams& p, long m, int n, const float (&v)[4]) {
+    float r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float b = (p.bias && n + e < p.N) ? p.bias[n + e] : 0.f;
+        r[e] = activate(v[e] + b, p.act, p.slope);
+    }
+    if (p.out32) {
+        float* o = (float*)p.out + m * p.ldo + n;
+        if (p.vec && n + 3 < p.N) { *reinterpret_cast<float4*>(o) = make_float4(r[0], r[1], r[2], r[3]); return; }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (n + e < p.N) o[e] = r[e];
+    } else {
+        uint16_t* o = (uint16_t*)p.out + m * p.ldo + n;
+        const uint2 w = make_uint2(mgn_pack2(r[0], r[1]), mgn_pack2(r[2], r[3]));
+        if (p.vec && n + 3 < p.N) { *reinterpret_cast<uint2*>(o) = w; return; }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (n + e < p.N) o[e] = (uint16_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
+    }
+}
+
+template <int BM, int BN, int WVM, int WVN>
+struct MmTile {
+    static constexpr int NW = WVM * WVN, TM = BM / WVM / 32, TN = BN / WVN / 32;
+    static constexpr int ABYTES = BM * BLK, STAGE = (BM + BN) * BLK, SCALES = 512;   // [256 rows of A][256 rows of B]
+    static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;                           // 1-KB pieces (8 rows) per wave and stage
+    static constexpr int LDS = 2 * (STAGE + SCALES);
+    static_assert(PA * NW * 8 == BM && (PB * NW * 8 == BN) && BM <= 256 && BN <= 256 && NW % 2 == 0, "tile shape");
+};
+
+// A block computes a BM x BN tile; a step covers one block of 128 k.  Rows travel HBM/L2 -> LDS by LDS-DMA (16 bytes a lane, 8 rows a
+// piece), two stages; 16-byte chunk c of row r lies at position c ^ ((r >> 1) & 7), so that the 16-byte fragment reads of 16 neighbouring
+// rows cover every bank once.
+template <int BM, int BN, int WVM, int WVN>
+__device__ __forceinline__ void q8_mm_body(const MmParams& p) {
+    using Tl = MmTile<BM, BN, WVM, WVN>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // XCD x (= blockIdx % 8) owns the row tiles t with (t / group) % 8 == x, in groups of `group` row tiles that run through all column
+    // tiles together: a row tile is read from HBM by one XCD, and the tiles in flight on it share rows and columns
+    const int local = blockIdx.x >> 3, per = p.group * p.nt;
+    const int sg = local / per, in = local - sg * per;
+    const int mtile = (sg * 8 + (blockIdx.x & 7)) * p.group + in % p.group, ntile = in / p.group;
+    if (mtile >= p.mt) return;
+    const long m0 = (long)mtile * BM;
+    const int n0 = ntile * BN;
+    const int rowsA = (int)(p.M - m0 < BM ? p.M - m0 : BM), rowsB = p.N - n0 < BN ? p.N - n0 : BN;
+    const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a + m0 * p.ld), 0, (uint32_t)(rowsA * p.ld), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsB = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b + (long)n0 * p.ld), 0, (uint32_t)(rowsB * p.ld), 0x00020000);
+    // scale rows: 4 bytes a lane from row 4 * lane; rows are padded to 16, so whole words of this tile's rows never leave the scale row
+    const int sra = (rowsA + 3) >> 2, srb = (rowsB + 3) >> 2;
+
+    int offA[Tl::PA], offB[Tl::PB];
+    const int col = ((lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7)) << 4;   // (the swizzle of row r is the same for all pieces of a wave)
+#pragma unroll
+    for (int q = 0; q < Tl::PA; ++q) {
+        const int r = (wave + Tl::NW * q) * 8 + (lane >> 3);
+        offA[q] = r < rowsA ? r * p.ld + col : OOB;
+    }
+#pragma unroll
+    for (int q = 0; q < Tl::PB; ++q) {
+        const int r = (wave + Tl::NW * q) * 8 + (lane >> 3);
+        offB[q] = r < rowsB ? r * p.ld + col : OOB;
+    }
+    auto issue = [&](int kb, int buf) {
+        unsigned char* st = q8_sm + buf * (Tl::STAGE + Tl::SCALES);
+        const int k0 = kb * BLK;
+        const bool in = k0 + col < p.ld;   // (OOB + k0 stays beyond every descriptor)
+#pragma unroll
+        for (int q = 0; q < Tl::PA; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_ptr)(st + (wave + Tl::NW * q) * 1024), 16, in ? offA[q] + k0 : OOB, 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < Tl::PB; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_ptr)(st + Tl::ABYTES + (wave + Tl::NW * q) * 1024), 16, in ? offB[q] + k0 : OOB, 0, 0, 0);
+        if (wave < 2) {                   // wave 0: A's scales, wave 1: B's
+            const unsigned char* s = wave == 0 ? p.sa + (long)kb * p.lda_s + m0 : p.sb + (long)kb * p.ldb_s + n0;
+            const int words = wave == 0 ? sra : srb;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(s), 0, (uint32_t)(words * 4), 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(st + Tl::STAGE + wave * 256), 4, lane < words ? lane * 4 : OOB, 0, 0, 0);
+        }
+    };
+
+    const int wm = wave / WVN, wn = wave % WVN, lr = lane & 31, hi = lane >> 5;
+    f32x16 acc[Tl::TN][Tl::TM];
+#pragma unroll
+    for (int i = 0; i < Tl::TN; ++i)
+#pragma unroll
+        for (int j = 0; j < Tl::TM; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    const int sw = (lr >> 1) & 7;         // (tile bases are multiples of 32 rows)
+    issue(0, 0);
+    for (int kb = 0; kb < p.nb; ++kb) {
+        const int buf = kb & 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();     // everyone's rows of step kb have landed, and step kb - 1 has been read
+        if (kb + 1 < p.nb) issue(kb + 1, buf ^ 1);
+        const unsigned char* st = q8_sm + buf * (Tl::STAGE + Tl::SCALES);
+        int xs[Tl::TM], ws[Tl::TN];
+#pragma unroll
+        for (int j = 0; j < Tl::TM; ++j) xs[j] = st[Tl::STAGE + (wm * Tl::TM + j) * 32 + lr];
+#pragma unroll
+        for (int i = 0; i < Tl::TN; ++i) ws[i] = st[Tl::STAGE + 256 + (wn * Tl::TN + i) * 32 + lr];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int c0 = ((kk * 4 + hi * 2) ^ sw) << 4, c1 = ((kk * 4 + hi * 2 + 1) ^ sw) << 4;
+            i32x8 x[Tl::TM], w[Tl::TN];
+#pragma unroll
+            for (int j = 0; j < Tl::TM; ++j) {
+                const unsigned char* row = st + ((wm * Tl::TM + j) * 32 + lr) * BLK;
+                const int4 u = *reinterpret_cast<const int4*>(row + c0), v = *reinterpret_cast<const int4*>(row + c1);
+                x[j] = i32x8{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            }
+#pragma unroll
+            for (int i = 0; i < Tl::TN; ++i) {
+                const unsigned char* row = st + Tl::ABYTES + ((wn * Tl::TN + i) * 32 + lr) * BLK;
+                const int4 u = *reinterpret_cast<const int4*>(row + c0), v = *reinterpret_cast<const int4*>(row + c1);
+                w[i] = i32x8{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            }
+#pragma unroll
+            for (int i = 0; i < Tl::TN; ++i)
+#pragma unroll
+                for (int j = 0; j < Tl::TM; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], x[j], acc[i][j], 0, 0, 0, ws[i], 0, xs[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < Tl::TM; ++j) {
+        const long m = m0 + (wm * Tl::TM + j) * 32 + lr;
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int i = 0; i < Tl::TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = n0 + (wn * Tl::TN + i) * 32 + 8 * q + 4 * hi;
+                if (n >= p.N) continue;
+                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                mm_emit(p, m, n, v);
+            }
+    }
+}
+
+__global__ __launch_bounds__(512, 1) void q8_mm_256x256(MmParams p) { q8_mm_body<256, 256, 2, 4>(p); }
+__global__ __launch_bounds__(256, 2) void q8_mm_128x128(MmParams p) { q8_mm_body<128, 128, 2, 2>(p); }
+__global__ __launch_bounds__(256, 2) void q8_mm_128x32(MmParams p) { q8_mm_body<128, 32, 4, 1>(p); }
+
+// Few tiles: a block per 32 x 32 outputs, the blocks of k dealt to its four waves, operands straight from memory into registers, the four
+// partial tiles added through LDS in wave order.
+__global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
+    __shared__ float part[4][32][33];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, hi = lane >> 5;
+    const int n0 = blockIdx.x * 32;
+    const long m0 = (long)blockIdx.y * 32;
+    const bool am = m0 + lr < p.M, bn = n0 + lr < p.N;
+    const unsigned char* arow = p.a + (am ? m0 + lr : 0) * p.ld;
+    const unsigned char* brow = p.b + (long)(bn ? n0 + lr : 0) * p.ld;
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    for (int kb = wave; kb < p.nb; kb += 4) {
+        const int xs = am ? p.sa[(long)kb * p.lda_s + m0 + lr] : 0, ws = bn ? p.sb[(long)kb * p.ldb_s + n0 + lr] : 0;
+        int4 u[4], v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int c = kb * BLK + (q >> 1) * 64 + hi * 32 + (q & 1) * 16;
+            u[q] = (am && c < p.ld) ? *reinterpret_cast<const int4*>(arow + c) : make_int4(0, 0, 0, 0);
+            v[q] = (bn && c < p.ld) ? *reinterpret_cast<const int4*>(brow + c) : make_int4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const i32x8 x = {u[2 * kk].x, u[2 * kk].y, u[2 * kk].z, u[2 * kk].w, u[2 * kk + 1].x, u[2 * kk + 1].y, u[2 * kk + 1].z, u[2 * kk + 1].w};
+            const i32x8 w = {v[2 * kk].x, v[2 * kk].y, v[2 * kk].z, v[2 * kk].w, v[2 * kk + 1].x, v[2 * kk + 1].y, v[2 * kk + 1].z, v[2 * kk + 1].w};
+            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, acc, 0, 0, 0, ws, 0, xs);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) part[wave][lr][8 * (e >> 2) + 4 * hi + (e & 3)] = acc[e];
+    __syncthreads();
+    const int r = threadIdx.x >> 3, n = (threadIdx.x & 7) * 4;
+    if (m0 + r < p.M && n0 + n < p.N) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (part[0][r][n + e] + part[1][r][n + e]) + (part[2][r][n + e] + part[3][r][n + e]);
+        mm_emit(p, m0 + r, n0 + n, v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------
+// dW[n][k] = sum_m dy[m][n] x^[m][k], db[n] = sum_m dy[m][n]: dy in 16 bits, x^ from its codes.
+//   A block computes a 128 x 128 tile over one of `splits` row ranges.  dy rows go to LDS by LDS-DMA, codes through registers, where a
+//   value and its scale become the exact 16-bit x^ (one instruction for two); both tiles are read back with the transposing LDS reads,
+//   since the summed index is the row.  v_mfma_f32_32x32x16, fp32 accumulation; the splits' tiles are added by q8_wgrad_reduce in order.
+//   db: the same dy fragments times a column of ones, in the blocks of the first k tile.
+// ------------------------------------------------------------------------------------------------------
+struct WgradParams8 {
+    const uint16_t* dy;
+    const unsigned char *codes, *scales;
+    float* part;                          // [splits][N * K + N]
+    int M, N, K, ldy, ldc;
+    long lds;
+    int rows_per_split, splits, ntn, ntk;
+};
+MGN_PLAN_RO(WgradParams8, MGN_RO(dy) MGN_RO(codes) MGN_RO(scales))
+
+constexpr int WG_ROWS = 64;               // rows per step
+constexpr int WG_TILE = WG_ROWS * 256;    // bytes of a [64][128] 16-bit tile
+constexpr int WG_LDS = 4 * WG_TILE;
+
+__device__ __forceinline__ uint32_t decode2(uint32_t c, float s, int word) {
+#ifdef MGN_F16
+    return word ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, s, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, s, false));
+#else
+    return word ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, false));
+#endif
+}
+
+__global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+    // the tiles of one row range share an XCD (its rows are then read from HBM once)
+    const int tiles = p.ntn * p.ntk, local = blockIdx.x >> 3;
+    const int z = (local / tiles) * 8 + (blockIdx.x & 7), t = local % tiles;
+    if (z >= p.splits) return;
+    const int tn = t % p.ntn, tk = t / p.ntn;
+    const long mb = (long)z * p.rows_per_split;
+    const int rows = (int)(p.M - mb < p.rows_per_split ? p.M - mb : p.rows_per_split);   // >= 1 by the host's choice of splits
+    const int steps = (rows + WG_ROWS - 1) / WG_ROWS;
+    const __amdgpu_buffer_rsrc_t rsY = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p.dy + mb * p.ldy), 0, (uint32_t)(rows * p.ldy * 2), 0x00020000);
+    auto swz = [](int r) { return (r & 3) << 2; };
+    int yo[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int r = (wave + 4 * q) * 4 + (lane >> 4), ch = (lane & 15) ^ swz(r);
+        yo[q] = tn * 128 + ch * 8 < p.ldy ? r * p.ldy * 2 + (tn * 128 + ch * 8) * 2 : OOB;
+    }
+    auto issue = [&](int ks, int buf) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = ks * WG_ROWS + (wave + 4 * q) * 4 + (lane >> 4);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsY, (lds_ptr)(q8_sm + buf * WG_TILE + (wave + 4 * q) * 1024), 16,
+                                                     (r < rows && yo[q] != OOB) ? yo[q] + ks * WG_ROWS * p.ldy * 2 : OOB, 0, 0, 0);
+        }
+    };
+    // codes: thread = (row tid / 4, 32 columns)
+    const int cr = tid >> 2, cc = (tid & 3) * 32, kcol = tk * BLK + cc;
+    uint4 cq[2];
+    uint32_t cs = 0;
+    auto fetch = [&](int ks) {
+        const int r = ks * WG_ROWS + cr;
+        cq[0] = cq[1] = make_uint4(0, 0, 0, 0);
+        cs = 0;
+        if (r < rows) {
+            const unsigned char* src = p.codes + (mb + r) * p.ldc + kcol;
+            if (kcol < p.ldc) cq[0] = *reinterpret_cast<const uint4*>(src);
+            if (kcol + 16 < p.ldc) cq[1] = *reinterpret_cast<const uint4*>(src + 16);
+            cs = p.scales[(long)tk * p.lds + mb + r];
+        }
+    };
+    auto spread = [&](int buf) {
+        unsigned char* b = q8_sm + (2 + buf) * WG_TILE + cr * 256;
+        const float s = pow2(cs);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 c = cq[h];
+            const uint4 lo = make_uint4(decode2(c.x, s, 0), decode2(c.x, s, 1), decode2(c.y, s, 0), decode2(c.y, s, 1));
+            const uint4 up = make_uint4(decode2(c.z, s, 0), decode2(c.z, s, 1), decode2(c.w, s, 0), decode2(c.w, s, 1));
+            const int ch = (cc >> 3) + 2 * h;
+            *reinterpret_cast<uint4*>(b + ((ch ^ swz(cr)) << 4)) = lo;
+            *reinterpret_cast<uint4*>(b + (((ch + 1) ^ swz(cr)) << 4)) = up;
+        }
+    };
+    // transposed fragments: lane group g = lane >> 4 reads rows 8 * (g >> 1) + (i >> 2) [+ 4], columns 16 * (g & 1) + 4 * (i & 3)
+    const int g = lane >> 4, i4 = lane & 15, prow = 8 * (g >> 1) + (i4 >> 2);
+    int fa[2], fb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int ca = wm * 64 + i * 32 + (g & 1) * 16 + 4 * (i4 & 3), cb = wn * 64 + i * 32 + (g & 1) * 16 + 4 * (i4 & 3);
+        fa[i] = prow * 256 + (((ca >> 3) ^ swz(prow)) << 4) + (ca & 7) * 2;
+        fb[i] = 2 * WG_TILE + prow * 256 + (((cb >> 3) ^ swz(prow)) << 4) + (cb & 7) * 2;
+    }
+    typedef __attribute__((address_space(3))) s16x4* lp;
+    auto frag = [&](const unsigned char* q) {
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(q + 4 * 256));
+        return __builtin_bit_cast(h16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    f32x16 acc[2][2], accb[2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        acc[0][0][e] = acc[0][1][e] = acc[1][0][e] = acc[1][1][e] = 0.f;
+        accb[0][e] = accb[1][e] = 0.f;
+    }
+    h16x8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = (decltype(ones[0] + ones[0]))1.0f;
+    const bool with_db = tk == 0 && wn == 0;
+
+    issue(0, 0);
+    fetch(0);
+    for (int ks = 0; ks < steps; ++ks) {
+        const int buf = ks & 1;
+        spread(buf);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();     // step ks is in LDS; step ks - 1 has been read by everyone
+        if (ks + 1 < steps) {
+            issue(ks + 1, buf ^ 1);
+            fetch(ks + 1);
+        }
+        const unsigned char* st = q8_sm + buf * WG_TILE;
+#pragma unroll
+        for (int kk = 0; kk < WG_ROWS / 16; ++kk) {   // the swizzle depends on row bits 0..1: unchanged by + 16 rows
+            h16x8 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[i] = frag(st + fa[i] + kk * 16 * 256);
+                b[i] = frag(st + fb[i] + kk * 16 * 256);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = MGN_MFMA_32x32x16(a[i], b[j], acc[i][j]);
+            if (with_db) {
+                accb[0] = MGN_MFMA_32x32x16(a[0], ones, accb[0]);
+                accb[1] = MGN_MFMA_32x32x16(a[1], ones, accb[1]);
+            }
+        }
+    }
+    const long wsize = (long)p.N * p.K + p.N;
+    float* out = p.part + (long)z * wsize;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int n = tn * 128 + wm * 64 + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+            if (n >= p.N) continue;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int k = tk * BLK + wn * 64 + j * 32 + (lane & 31);
+                if (k < p.K) out[(long)n * p.K + k] = acc[i][j][e];
+            }
+            if (with_db && (lane & 31) == 0) out[(long)p.N * p.K + n] = accb[i][e];
+        }
+}
+
+// dw | db = the splits' partial results added in order; 16 groups of splits side by side, joined in group order
+__global__ __launch_bounds__(TPB) void q8_wgrad_reduce(const float* __restrict__ part, int splits, long total, long nk, float* __restrict__ dw,
+                                                       float* __restrict__ db) {
+    __shared__ float sh[16][17];
+    const int col = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const long i = (long)blockIdx.x * 16 + col;
+    float s = 0.f;
+    if (i < total)
+        for (int z = g; z < splits; z += 16) s += part[(long)z * total + i];
+    sh[g][col] = s;
+    __syncthreads();
+    if (g == 0 && i < total) {
+        float r = sh[0][col];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) r += sh[k][col];
+        if (i < nk) dw[i] = r;
+        else if (db) db[i - nk] = r;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------
+// block tail y = relu(norm(x) + shortcut) whose backward pass reads x^ instead of x.  Thread mapping of the four kernels: blockIdx.y = a
+// block of 128 channels, LPB lanes (8 channels each) per row -- a thread's channels never change, so their coefficients stay in
+// registers.  All are bound by HBM.
+// ------------------------------------------------------------------------------------------------------
+constexpr int TAIL_BLOCKS = 512;          // row blocks of the two reductions (= partial rows)
+
+// column sums of two quantities over this block's rows -> part[blockIdx.x][C][2]; NL rows in flight per thread
+template <int LPB>
+__device__ __forceinline__ void tail_flush(const float (&a)[8], const float (&b)[8], int C, float* part) {
+    __shared__ float sh[TPB / LPB][LPB * 16 + 1];
+    const int l = threadIdx.x % LPB, ty = threadIdx.x / LPB;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        sh[ty][(l * 8 + k) * 2] = a[k];
+        sh[ty][(l * 8 + k) * 2 + 1] = b[k];
+    }
+    __syncthreads();
+    const int base = blockIdx.y * BLK * 2;
+    for (int i = threadIdx.x; i < LPB * 16; i += TPB) {
+        float s = 0.f;
+        for (int y = 0; y < TPB / LPB; ++y) s += sh[y][i];
+        if (base + i < C * 2) part[(long)blockIdx.x * C * 2 + base + i] = s;
+    }
+}
+
+// sums of (x - x[0]) and their squares (around the first row: no cancellation for channels with a large mean); shift[C] = x[0]
+template <int LPB>
+__global__ __launch_bounds__(TPB) void q8_tail_stats(const uint16_t* __restrict__ x, int M, int C, float* __restrict__ part, float* __restrict__ shift) {
+    const int l = threadIdx.x % LPB, c0 = blockIdx.y * BLK + l * 8;
+    const bool on = c0 < C;
+    float s[8], a[8], b[8];
+    unpack8(on ? *reinterpret_cast<const uint4*>(x + c0) : make_uint4(0, 0, 0, 0), s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
+    const int stride = gridDim.x * (TPB / LPB);
+    auto add = [&](const uint4& q) {
+        float v[8];
+        unpack8(q, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { const float d = v[k] - s[k]; a[k] += d; b[k] = fmaf(d, d, b[k]); }
+    };
+    if (on) {
+        long r = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
+        for (; r + 7L * stride < M; r += 8L * stride) {
+            uint4 q[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = *reinterpret_cast<const uint4*>(x + (r + (long)j * stride) * C + c0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) add(q[j]);
+        }
+        for (; r < M; r += stride) add(*reinterpret_cast<const uint4*>(x + r * C + c0));
+        if (blockIdx.x == 0 && threadIdx.x < LPB) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) shift[c0 + k] = s[k];
+        }
+    }
+    tail_flush<LPB>(a, b, C, part);
+}
+
+// y = relu(scale * x + offset + shortcut); codes and scales of x; the mask y > 0, one byte per 8 outputs.  8 rows per lane group.
+// KEEP false (inference): y alone.
+template <int LPB, bool KEEP>
+__global__ __launch_bounds__(TPB) void q8_tail_fwd(const uint16_t* __restrict__ x, const uint16_t* __restrict__ shortcut, const float* __restrict__ scale,
+                                                   const float* __restrict__ offset, int M, int C, int ldc, long lds, uint16_t* __restrict__ y,
+                                                   unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, unsigned char* __restrict__ bits) {
+    const int l = threadIdx.x % LPB, c0 = blockIdx.y * BLK + l * 8;
+    const long r0l = ((long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB) * RPG;
+    if (r0l >= M) return;
+    const int r0 = (int)r0l;
+    const bool on = c0 < C;
+    uint4 q[RPG], t[RPG];
+#pragma unroll
+    for (int j = 0; j < RPG; ++j) {
+        const bool in = on && r0 + j < M;
+        const long o = (long)(r0 + j) * C + c0;
+        q[j] = in ? *reinterpret_cast<const uint4*>(x + o) : make_uint4(0, 0, 0, 0);
+        t[j] = in ? *reinterpret_cast<const uint4*>(shortcut + o) : make_uint4(0, 0, 0, 0);
+    }
+    float sc[8], of[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        sc[k] = on ? scale[c0 + k] : 0.f;
+        const float o = on ? offset[c0 + k] : 0.f;
+        // (an infinity in a channel makes its mean, and this offset, infinite: the channel is NaN, not the zeros that the ReLU of -inf is)
+        of[k] = (__float_as_uint(o) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : o;
+    }
+    uint32_t sb[RPG];
+#pragma unroll
+    for (int j = 0; j < RPG; ++j) {
+        float v[8], w[8];
+        unpack8(q[j], v);
+        unpack8(t[j], w);
+        const uint32_t s = KEEP ? scale_of(group_max<LPB>(amax8(v, TOP16))) : 0u;
+        sb[j] = s;
+        if (r0 + j >= M) continue;
+        const long o = (long)(r0 + j) * C + c0;
+        if (KEEP && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = encode8(v, inv_scale(s), TOP16);
+        if (!on) continue;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float z = fmaf(v[k], sc[k], of[k]) + w[k];
+            v[k] = z < 0.f ? 0.f : z;     // (NaN stays)
+        }
+        const uint4 r = pack8(v);
+        *reinterpret_cast<uint4*>(y + o) = r;
+        if (!KEEP) continue;
+        const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m |= (((u[k] & 0x7fffu) != 0u ? 1u : 0u) | ((u[k] & 0x7fff0000u) != 0u ? 2u : 0u)) << (2 * k);
+        bits[o >> 3] = (unsigned char)m;
+    }
+    if (KEEP && l == 0)
+        *reinterpret_cast<uint2*>(scales + blockIdx.y * lds + r0) =
+            make_uint2(sb[0] | (sb[1] << 8) | (sb[2] << 16) | (sb[3] << 24), sb[4] | (sb[5] << 8) | (sb[6] << 16) | (sb[7] << 24));
+}
+
+__device__ __forceinline__ uint32_t mask2(uint32_t e) { return ((e & 1u) * 0xffffu) | (((e >> 1) & 1u) * 0xffff0000u); }
+
+// dz = g * mask, written (the shortcut's gradient) and reduced: sum dz, sum dz * (x^ - mean)
+template <int LPB>
+__global__ __launch_bounds__(TPB) void q8_tail_bwd_reduce(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                                          const uint16_t* __restrict__ g, const unsigned char* __restrict__ bits,
+                                                          const float* __restrict__ mean, int M, int C, int ldc, long lds, uint16_t* __restrict__ dz,
+                                                          float* __restrict__ part) {
+    const int l = threadIdx.x % LPB, c0 = blockIdx.y * BLK + l * 8;
+    const bool on = c0 < C;
+    float mu[8], a[8], b[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { mu[k] = on ? mean[c0 + k] : 0.f; a[k] = b[k] = 0.f; }
+    const int stride = gridDim.x * (TPB / LPB);
+    const unsigned char* srow = scales + blockIdx.y * lds;
+    auto one = [&](long r, const uint2& c, uint32_t s, uint4 q, uint32_t e) {
+        q.x &= mask2(e); q.y &= mask2(e >> 2); q.z &= mask2(e >> 4); q.w &= mask2(e >> 6);
+        *reinterpret_cast<uint4*>(dz + r * C + c0) = q;
+        float v[8], w[8];
+        decode8(c, pow2(s), v);
+        unpack8(q, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { a[k] += w[k]; b[k] = fmaf(w[k], v[k] - mu[k], b[k]); }
+    };
+    if (on) {
+        long r = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
+        for (; r + 3L * stride < M; r += 4L * stride) {
+            uint2 c[4];
+            uint4 q[4];
+            uint32_t s[4], e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const long rr = r + (long)j * stride;
+                c[j] = *reinterpret_cast<const uint2*>(codes + rr * ldc + c0);
+                q[j] = *reinterpret_cast<const uint4*>(g + rr * C + c0);
+                s[j] = srow[rr];
+                e[j] = bits[(rr * C + c0) >> 3];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) one(r + (long)j * stride, c[j], s[j], q[j], e[j]);
+        }
+        for (; r < M; r += stride)
+            one(r, *reinterpret_cast<const uint2*>(codes + r * ldc + c0), srow[r], *reinterpret_cast<const uint4*>(g + r * C + c0), bits[(r * C + c0) >> 3]);
+    }
+    tail_flush<LPB>(a, b, C, part);
+}
+
+#ifndef MGN_F16
+// partial sums -> sums[2][C] = {sum dz, sum dz * x_hat}, dwb[2][C] = {sign(weight) * sums[1], sums[0]}; fixed order, 64-bit
+__global__ __launch_bounds__(TPB) void q8_tail_sums(const float* __restrict__ part, int rows, int C, const float* __restrict__ rstd,
+                                                    const float* __restrict__ weight, float* __restrict__ sums, float* __restrict__ dwb) {
+    __shared__ double sh[TPB / 8][8];
+    const int c0 = blockIdx.x * 4, col = threadIdx.x & 7, rg = threadIdx.x >> 3;
+    double s = 0.0;
+    for (int r = rg; r < rows; r += TPB / 8) s += (double)part[((long)r * C + c0) * 2 + col];
+    sh[rg][col] = s;
+    __syncthreads();
+    if (threadIdx.x < 4) {
+        double t1 = 0.0, t2 = 0.0;
+        for (int k = 0; k < TPB / 8; ++k) { t1 += sh[k][2 * threadIdx.x]; t2 += sh[k][2 * threadIdx.x + 1]; }
+        const int c = c0 + threadIdx.x;
+        const float s1 = (float)t1, s2 = (float)(t2 * (double)rstd[c]), w = weight[c];
+        sums[c] = s1;
+        sums[C + c] = s2;
+        dwb[c] = s2 * (float)((w > 0.f) - (w < 0.f));
+        dwb[C + c] = s1;
+    }
+}
+#endif
+
+// dx = gain * rstd * (dz - sums[0] / n - x_hat * sums[1] / n),  x_hat = (x^ - mean) * rstd,  gain = |weight| + eps
+template <int LPB>
+__global__ __launch_bounds__(TPB) void q8_tail_bwd_apply(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                                         const uint16_t* __restrict__ dz, const float* __restrict__ weight,
+                                                         const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ sums,
+                                                         float inv_n, float eps, int M, int C, int ldc, long lds, uint16_t* __restrict__ dx) {
+    const int l = threadIdx.x % LPB, c0 = blockIdx.y * BLK + l * 8;
+    const long r0l = ((long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB) * RPG;
+    if (r0l >= M || c0 >= C) return;
+    const int r0 = (int)r0l;
+    uint2 c[RPG];
+    uint4 q[RPG];
+    const uint2 sb = *reinterpret_cast<const uint2*>(scales + blockIdx.y * lds + r0);
+#pragma unroll
+    for (int j = 0; j < RPG; ++j) {
+        const bool in = r0 + j < M;
+        c[j] = in ? *reinterpret_cast<const uint2*>(codes + (long)(r0 + j) * ldc + c0) : make_uint2(0, 0);
+        q[j] = in ? *reinterpret_cast<const uint4*>(dz + (long)(r0 + j) * C + c0) : make_uint4(0, 0, 0, 0);
+    }
+    float A[8], m1[8], B[8], mu[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float rs = rstd[c0 + k];
+        A[k] = (fabsf(weight[c0 + k]) + eps) * rs;
+        m1[k] = sums[c0 + k] * inv_n;
+        B[k] = rs * (sums[C + c0 + k] * inv_n);
+        mu[k] = mean[c0 + k];
+    }
+#pragma unroll
+    for (int j = 0; j < RPG; ++j) {
+        if (r0 + j >= M) break;
+        float v[8], w[8];
+        decode8(c[j], pow2(((j < 4 ? sb.x : sb.y) >> (8 * (j & 3))) & 0xffu), v);
+        unpack8(q[j], w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = A[k] * ((w[k] - m1[k]) - (v[k] - mu[k]) * B[k]);
+        *reinterpret_cast<uint4*>(dx + (long)(r0 + j) * C + c0) = pack8(w);
+    }
+}
+
+inline int nblocks(int C) { return (C + BLK - 1) / BLK; }
+inline int code_ld(int C) { return (C + 15) & ~15; }
+inline long scale_ld(long M) { return (M + 15) & ~15L; }
+inline int lanes_for(int C) { return C > 64 ? 16 : (C > 32 ? 8 : 4); }
+inline bool aligned(const void* p, int n) { return ((uintptr_t)p & (uintptr_t)(n - 1)) == 0; }
+inline int done() { return hipGetLastError() == hipSuccess ? MGN_OK : MGN_ELAUNCH; }
+constexpr long MAX_ROWS = 0x7fffff00L;    // rows are counted in 32 bits (padded to 16), offsets in 64
+constexpr int MAX_COLS = 1 << 20;
+
+template <int BM, int BN, int WVM, int WVN>
+int launch_mm(void (*kernel)(MmParams), MmParams p, hipStream_t s) {
+    using Tl = MmTile<BM, BN, WVM, WVN>;
+    p.mt = (int)(((long)p.M + BM - 1) / BM);
+    p.nt = (p.N + BN - 1) / BN;
+    p.group = p.mt < 16 ? 1 : (p.mt >= 32 ? 4 : p.mt / 8);
+    const long blocks = ((long)p.mt + 8 * p.group - 1) / (8 * p.group) * p.group * p.nt * 8;
+    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    if (Tl::LDS > 65536) {
+        static bool ready[64] = {};
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MGN_ELAUNCH;
+        if (!ready[dev]) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Tl::LDS) != hipSuccess) return MGN_ELAUNCH;
+            ready[dev] = true;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WVM * WVN), Tl::LDS, s, p);
+    return done();
+}
+
+}  // namespace
+
+#define Q8_LANES(C, CALL) do { switch (lanes_for(C)) { case 16: { constexpr int LPB = 16; CALL; } break; case 8: { constexpr int LPB = 8; CALL; } break; default: { constexpr int LPB = 4; CALL; } } } while (0)
+
+extern "C" {
+
+#ifndef MGN_F16
+int mgn_q8_bytes(long M, int C, size_t* codes, size_t* scales) {
+    if (M < 0 || M > MAX_ROWS || C < 1 || C > MAX_COLS || !codes || !scales) return MGN_EINVAL;
+    *codes = (size_t)M * code_ld(C);
+    *scales = (size_t)nblocks(C) * scale_ld(M);
+    return MGN_OK;
+}
+#endif
+
+int MGN_SYM(mgn_q8_pack)(const void* x, int dtype, long M, int C, long sn, long sh, long sw, int H, int W, void* codes, void* scales, void* stream_) {
+    if (M < 0 || M > MAX_ROWS || C < 1 || C > MAX_COLS || (dtype != 0 && dtype != 1) || sn < 0 || sh < 0 || sw < 0) return MGN_EINVAL;
+    if (M == 0) return MGN_OK;
+    if (!x || !codes || !scales || H < 1 || W < 1 || M % ((long)H * W) != 0 || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(x, dtype ? 2 : 4)) return MGN_EINVAL;
+    long images = M / ((long)H * W);
+    if (W == 1) { W = H; H = 1; sw = sh; }                                  // (the stride of an axis of length one says nothing)
+    if (W == 1 && images <= 0x7fffffffL) { W = (int)images; sw = sn; images = 1; }
+    RowMap map = {sn, sh, sw, H, W, 0};
+    map.flat = (H == 1 || sh == (long)W * sw) && (images == 1 || sn == (long)H * W * sw);
+    const int nb = nblocks(C), ldc = code_ld(C), lpb = lanes_for(C);
+    const int el = dtype ? 8 : 4;         // elements in 16 bytes
+    const bool vec = C % 8 == 0 && aligned(x, 16) && sw % el == 0 && (map.flat || (sh % el == 0 && sn % el == 0));
+    const long groups = (M + RPG - 1) / RPG * nb, blocks = (groups * lpb + TPB - 1) / TPB;
+    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    hipStream_t s = (hipStream_t)stream_;
+#define Q8_PACK(T, V) Q8_LANES(C, (hipLaunchKernelGGL((q8_pack<T, LPB, V>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const T*)x, map, (int)M, C, nb, ldc, \
+                                                      scale_ld(M), (unsigned char*)codes, (unsigned char*)scales)))
+    if (dtype) { if (vec) Q8_PACK(uint16_t, true); else Q8_PACK(uint16_t, false); }
+    else { if (vec) Q8_PACK(float, true); else Q8_PACK(float, false); }
+#undef Q8_PACK
+    return done();
+}
+
+int MGN_SYM(mgn_q8_unpack)(const void* codes, const void* scales, long M, int C, void* y, int dtype, void* stream_) {
+    if (M < 0 || M > MAX_ROWS || C < 1 || C > MAX_COLS || (dtype != 0 && dtype != 1)) return MGN_EINVAL;
+    if (M == 0) return MGN_OK;
+    if (!codes || !scales || !y || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(y, dtype ? 2 : 4)) return MGN_EINVAL;
+    const int nb = nblocks(C), ldc = code_ld(C), lpb = lanes_for(C);
+    const bool vec = C % 8 == 0 && aligned(y, 16);
+    const long groups = (M + RPG - 1) / RPG * nb, blocks = (groups * lpb + TPB - 1) / TPB;
+    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    hipStream_t s = (hipStream_t)stream_;
+#define Q8_UNPACK(T, V) Q8_LANES(C, (hipLaunchKernelGGL((q8_unpack<T, LPB, V>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const unsigned char*)codes, \
+                                                        (const unsigned char*)scales, (int)M, C, nb, ldc, scale_ld(M), (T*)y)))
+    if (dtype) { if (vec) Q8_UNPACK(uint16_t, true); else Q8_UNPACK(uint16_t, false); }
+    else { if (vec) Q8_UNPACK(float, true); else Q8_UNPACK(float, false); }
+#undef Q8_UNPACK
+    return done();
+}
+
+int MGN_SYM(mgn_q8_pack_weight)(const void* w, int dtype, long sr, long sc, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t,
+                                void* stream_) {
+    if (N < 1 || K < 1 || N > MAX_COLS || K > MAX_COLS || (dtype != 0 && dtype != 1) || !w || sr < 0 || sc < 0 || !aligned(w, dtype ? 2 : 4)) return MGN_EINVAL;
+    if ((!codes && !codes_t) || !codes != !scales || !codes_t != !scales_t || !aligned(codes, 16) || !aligned(codes_t, 16)) return MGN_EINVAL;
+    const dim3 grid((unsigned)nblocks(N), (unsigned)nblocks(K));
+    hipStream_t s = (hipStream_t)stream_;
+    if (dtype) hipLaunchKernelGGL(q8_pack_tile<uint16_t>, grid, dim3(TPB), 0, s, (const uint16_t*)w, sr, sc, N, K, (unsigned char*)codes,
+                                  (unsigned char*)scales, (unsigned char*)codes_t, (unsigned char*)scales_t);
+    else hipLaunchKernelGGL(q8_pack_tile<float>, grid, dim3(TPB), 0, s, (const float*)w, sr, sc, N, K, (unsigned char*)codes, (unsigned char*)scales,
+                            (unsigned char*)codes_t, (unsigned char*)scales_t);
+    return done();
+}
+
+int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const void* b, const void* b_scales, int N, int K, const float* bias, int act,
+                           float slope, void* out, int out_f32, long ldo, void* stream_) {
+    if (M < 0 || M > MAX_ROWS || N < 1 || N > MAX_COLS || K < 1 || K > MAX_COLS || act < 0 || act > 2 || ldo < N) return MGN_EINVAL;
+    if (M == 0) return MGN_OK;
+    if (!a || !a_scales || !b || !b_scales || !out || !aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 16) || !aligned(b_scales, 16) ||
+        !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;
+    MmParams p = {(const unsigned char*)a, (const unsigned char*)a_scales, (const unsigned char*)b, (const unsigned char*)b_scales, bias, out,
+                  (int)M, N, K, nblocks(K), code_ld(K), scale_ld(M), scale_ld(N), ldo, act, out_f32, 0, slope, 0, 0, 1};
+    p.vec = ldo % 4 == 0 && aligned(out, out_f32 ? 16 : 8);
+    hipStream_t s = (hipStream_t)stream_;
+    auto tiles = [&](int BM, int BN) { return ((M + BM - 1) / BM) * ((N + BN - 1) / BN); };
+    if (M <= 64 || tiles(128, 128) < 64) {
+        const long gy = (M + 31) / 32;
+        if (gy > 65535) return MGN_EINVAL;
+        hipLaunchKernelGGL(q8_mm_small, dim3((unsigned)((N + 31) / 32), (unsigned)gy), dim3(TPB), 0, s, p);
+        return done();
+    }
+    if (N <= 32) return launch_mm<128, 32, 4, 1>(q8_mm_128x32, p, s);
+    if (N > 128 && tiles(256, 256) >= 512) return launch_mm<256, 256, 2, 4>(q8_mm_256x256, p, s);
+    return launch_mm<128, 128, 2, 2>(q8_mm_128x128, p, s);
+}
+
+#ifndef MGN_F16
+static int wgrad_splits(long M, int N, int K) {
+    const long tiles = (long)nblocks(N) * nblocks(K);
+    long z = 512 / tiles, most = (M + 4 * WG_ROWS - 1) / (4 * WG_ROWS);   // two blocks a CU, at least four steps a block
+    z = z < 1 ? 1 : z;
+    return (int)(z < most ? z : most);
+}
+int mgn_q8_wgrad_workspace_bytes(long M, int N, int K, size_t* bytes) {
+    if (M < 1 || M > MAX_ROWS || N < 1 || K < 1 || N > 65536 || K > 65536 || !bytes) return MGN_EINVAL;
+    *bytes = sizeof(float) * (size_t)(wgrad_splits(M, N, K) + 1) * ((size_t)N * K + N);
+    return MGN_OK;
+}
+#endif
+
+int MGN_SYM(mgn_q8_wgrad)(const void* dy, long ldy, long M, int N, const void* codes, const void* scales, int K, float* dw, float* db, void* ws,
+                          size_t ws_bytes, void* stream_) {
+    size_t need = 0;
+    const int rc = mgn_q8_wgrad_workspace_bytes(M, N, K, &need);
+    if (rc != MGN_OK) return rc;
+    if (!dy || !codes || !scales || !dw || !ws || !aligned(dy, 16) || !aligned(codes, 16) || ldy < N || ldy % 8 != 0 || ldy > 65536) return MGN_EINVAL;
+    if (ws_bytes < need) return MGN_ENOSPC;
+    const size_t one = sizeof(float) * ((size_t)N * K + N);
+    const int zmax = (int)(need / one) - 1;
+    // rows per split: whole steps, and a range whose bytes stay inside a 32-bit buffer descriptor
+    long rows = ((M + zmax - 1) / zmax + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
+    if (rows * ldy * 2 > 0x7fffffffL) return MGN_EINVAL;
+    WgradParams8 p = {(const uint16_t*)dy, (const unsigned char*)codes, (const unsigned char*)scales, (float*)ws, (int)M, N, K, (int)ldy, code_ld(K),
+                      scale_ld(M), (int)rows, (int)((M + rows - 1) / rows), nblocks(N), nblocks(K)};
+    const long blocks = (long)((p.splits + 7) / 8) * 8 * p.ntn * p.ntk;
+    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    hipStream_t s = (hipStream_t)stream_;
+    hipLaunchKernelGGL(q8_wgrad, dim3((unsigned)blocks), dim3(TPB), WG_LDS, s, p);
+    const long nk = (long)N * K, total = nk + N;
+    hipLaunchKernelGGL(q8_wgrad_reduce, dim3((unsigned)((total + 15) / 16)), dim3(TPB), 0, s, (const float*)ws, p.splits, total, nk, dw, db);
+    return done();
+}
+
+/* ---- block tail ---- */
+static int tail_shape(long M, int C) { return (M < 1 || M > MAX_ROWS || C < 8 || C % 8 != 0 || C > 8192) ? MGN_EINVAL : MGN_OK; }
+static unsigned tail_rows(long M, int C) {   // row blocks of the reductions: 16 rows a thread before there are more blocks than fill the chip
+    const int rpb = TPB / lanes_for(C);
+    const long b = (M + (long)rpb * 16 - 1) / ((long)rpb * 16);
+    return (unsigned)(b < 1 ? 1 : (b > TAIL_BLOCKS ? TAIL_BLOCKS : b));
+}
+static unsigned tail_grid(long M, int C) {
+    const int rows = TPB / lanes_for(C) * RPG;
+    return (unsigned)((M + rows - 1) / rows);
+}
+
+#ifndef MGN_F16
+int mgn_q8_tail_partial_rows(long M, int C, int* rows) {
+    if (tail_shape(M, C) != MGN_OK || !rows) return MGN_EINVAL;
+    *rows = (int)tail_rows(M, C);
+    return MGN_OK;
+}
+#endif
+
+int MGN_SYM(mgn_q8_tail_stats)(const void* x, long M, int C, float* partials, float* shift, void* stream_) {
+    if (tail_shape(M, C) != MGN_OK || !x || !partials || !shift || !aligned(x, 16)) return MGN_EINVAL;
+    const dim3 grid(tail_rows(M, C), (unsigned)nblocks(C));
+    Q8_LANES(C, (hipLaunchKernelGGL(q8_tail_stats<LPB>, grid, dim3(TPB), 0, (hipStream_t)stream_, (const uint16_t*)x, (int)M, C, partials, shift)));
+    return done();
+}
+
+int MGN_SYM(mgn_q8_tail_fwd)(const void* x, const void* shortcut, const float* scale, const float* offset, long M, int C, void* y, void* codes,
+                             void* scales, void* relu_bits, void* stream_) {
+    if (tail_shape(M, C) != MGN_OK || !x || !shortcut || !scale || !offset || !y || !codes != !scales || !codes != !relu_bits || !aligned(x, 16) ||
+        !aligned(shortcut, 16) || !aligned(y, 16) || !aligned(codes, 16) || !aligned(scales, 16)) return MGN_EINVAL;
+    const dim3 grid(tail_grid(M, C), (unsigned)nblocks(C));
+#define Q8_TAIL(K) Q8_LANES(C, (hipLaunchKernelGGL((q8_tail_fwd<LPB, K>), grid, dim3(TPB), 0, (hipStream_t)stream_, (const uint16_t*)x, \
+        (const uint16_t*)shortcut, scale, offset, (int)M, C, code_ld(C), scale_ld(M), (uint16_t*)y, (unsigned char*)codes, (unsigned char*)scales, \
+        (unsigned char*)relu_bits)))
+    if (codes) Q8_TAIL(true); else Q8_TAIL(false);
+#undef Q8_TAIL
+    return done();
+}
+
+int MGN_SYM(mgn_q8_tail_bwd_reduce)(const void* codes, const void* scales, const void* g, const void* relu_bits, const float* mean, const float* rstd,
+                                    const float* weight, long M, int C, void* dz, float* partials, float* sums, float* dwb, void* stream_) {
+    if (tail_shape(M, C) != MGN_OK || !codes || !scales || !g || !relu_bits || !mean || !rstd || !weight || !dz || !partials || !sums || !dwb ||
+        !aligned(codes, 16) || !aligned(g, 16) || !aligned(dz, 16)) return MGN_EINVAL;
+    const dim3 grid(tail_rows(M, C), (unsigned)nblocks(C));
+    hipStream_t s = (hipStream_t)stream_;
+    Q8_LANES(C, (hipLaunchKernelGGL(q8_tail_bwd_reduce<LPB>, grid, dim3(TPB), 0, s, (const unsigned char*)codes, (const unsigned char*)scales,
+                                    (const uint16_t*)g, (const unsigned char*)relu_bits, mean, (int)M, C, code_ld(C), scale_ld(M), (uint16_t*)dz, partials)));
+    return mgn_q8_tail_sums(partials, (int)grid.x, C, rstd, weight, sums, dwb, stream_);
+}
+
+#ifndef MGN_F16
+int mgn_q8_tail_sums(const float* partials, int rows, int C, const float* rstd, const float* weight, float* sums, float* dwb, void* stream_) {
+    if (!partials || rows < 1 || C < 8 || C % 8 != 0 || !rstd || !weight || !sums || !dwb) return MGN_EINVAL;
+    hipLaunchKernelGGL(q8_tail_sums, dim3((unsigned)(C / 4)), dim3(TPB), 0, (hipStream_t)stream_, partials, rows, C, rstd, weight, sums, dwb);
+    return done();
+}
+#endif
+
+int MGN_SYM(mgn_q8_tail_bwd_apply)(const void* codes, const void* scales, const void* dz, const float* weight, const float* mean, const float* rstd,
+                                   const float* sums, float total_count, float eps, long M, int C, void* dx, void* stream_) {
+    if (tail_shape(M, C) != MGN_OK || !codes || !scales || !dz || !weight || !mean || !rstd || !sums || !dx || !(total_count > 0.f) ||
+        !aligned(codes, 16) || !aligned(scales, 16) || !aligned(dz, 16) || !aligned(dx, 16)) return MGN_EINVAL;
+    const dim3 grid(tail_grid(M, C), (unsigned)nblocks(C));
+    Q8_LANES(C, (hipLaunchKernelGGL(q8_tail_bwd_apply<LPB>, grid, dim3(TPB), 0, (hipStream_t)stream_, (const unsigned char*)codes,
+                                    (const unsigned char*)scales, (const uint16_t*)dz, weight, mean, rstd, sums, 1.f / total_count, eps, (int)M, C,
+                                    code_ld(C), scale_ld(M), (uint16_t*)dx)));
+    return done();
+}
+
+}  // extern "C"
