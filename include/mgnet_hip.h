@@ -806,6 +806,9 @@ int mgn_project_bwd(const float* points, const float* A, const float* t, const f
  *                     transpose [K][N] (the same values).  A pair may be NULL.
  * mgn_q8_matmul     : out[m][n] = act( sum_k a[m][k] b[n][k] + bias[n] ), a [M][K], b [N][K] packed, fp32 accumulation, one rounding;
  *                     act 0 none | 1 ReLU | 2 leaky ReLU; out fp32 or 16-bit, rows ldo elements apart.
+ * mgn_q8_pack_matmul: mgn_q8_pack of the 16-bit matrix x [M][K] (rows ldx elements apart) and mgn_q8_matmul of its packed form in one pass
+ *                     over x; codes / scales: where the packed form is kept, or both NULL.  MGN_ENOTSUP (nothing done): K > 512, K % 8 or
+ *                     ldx % 8 != 0, x not 16-byte aligned -- pack first then.  Same result as the two calls up to the order of the fp32 sums.
  * mgn_q8_wgrad      : dw[n][k] = sum_m dy[m][n] x[m][k] with dy 16-bit (rows ldy elements apart, ldy % 8 == 0, 16-byte aligned; columns
  *                     N .. ldy are ignored) and x packed; db[n] = sum_m dy[m][n] (nullable).  Fixed summation order.
  * ---------------------------------------------------------------------------------------------- */
@@ -815,6 +818,8 @@ int mgn_q8_unpack(const void* codes, const void* scales, long M, int C, void* y,
 int mgn_q8_pack_weight(const void* w, int dtype, long sr, long sc, int N, int K, void* codes, void* scales, void* codes_t, void* scales_t, void* stream);
 int mgn_q8_matmul(const void* a, const void* a_scales, long M, const void* b, const void* b_scales, int N, int K, const float* bias, int act, float slope,
                   void* out, int out_f32, long ldo, void* stream);
+int mgn_q8_pack_matmul(const void* x, long M, int K, long ldx, void* codes, void* scales, const void* b, const void* b_scales, int N, const float* bias,
+                       int act, float slope, void* out, int out_f32, long ldo, void* stream);
 int mgn_q8_wgrad_workspace_bytes(long M, int N, int K, size_t* bytes);
 int mgn_q8_wgrad(const void* dy, long ldy, long M, int N, const void* codes, const void* scales, int K, float* dw, float* db, void* workspace,
                  size_t workspace_bytes, void* stream);
@@ -942,6 +947,8 @@ int mgn_q8_pack_weight_f16(const void* w, int dtype, long sr, long sc, int N, in
     stream);
 int mgn_q8_matmul_f16(const void* a, const void* a_scales, long M, const void* b, const void* b_scales, int N, int K, const float* bias, int act,
     float slope, void* out, int out_f32, long ldo, void* stream);
+int mgn_q8_pack_matmul_f16(const void* x, long M, int K, long ldx, void* codes, void* scales, const void* b, const void* b_scales, int N, const float* bias,
+                       int act, float slope, void* out, int out_f32, long ldo, void* stream);
 int mgn_q8_wgrad_f16(const void* dy, long ldy, long M, int N, const void* codes, const void* scales, int K, float* dw, float* db, void* workspace,
     size_t workspace_bytes, void* stream);
 int mgn_q8_tail_stats_f16(const void* x, long M, int C, float* partials, float* shift, void* stream);

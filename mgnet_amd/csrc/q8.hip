@@ -228,22 +228,23 @@ __global__ __launch_bounds__(TPB) void q8_unpack(const unsigned char* __restrict
 // [K][ldc(N)] + scales [ceil(N/128)][lds(K)] (what the data gradient multiplies by).  A block per 128 x 128 tile; the tile goes through
 // LDS once so that both outputs leave in 16-byte stores.
 // ------------------------------------------------------------------------------------------------------
+constexpr int TILE_TPB = 1024;             // (16 values a thread: with 64 the few blocks of a layer took 11 us, all of it their own latency)
 template <typename T>
-__global__ __launch_bounds__(TPB) void q8_pack_tile(const T* __restrict__ w, long sr, long sc, int N, int K, unsigned char* __restrict__ codes,
+__global__ __launch_bounds__(TILE_TPB) void q8_pack_tile(const T* __restrict__ w, long sr, long sc, int N, int K, unsigned char* __restrict__ codes,
                                                     unsigned char* __restrict__ scales, unsigned char* __restrict__ codes_t,
                                                     unsigned char* __restrict__ scales_t) {
     constexpr int PITCH = BLK + 16;       // (rows of 16-byte chunks; the transposing byte reads then spread over the banks)
     __shared__ __attribute__((aligned(16))) unsigned char tile[BLK * PITCH];
-    __shared__ uint32_t part[TPB / 64];
+    __shared__ uint32_t part[TILE_TPB / 64];
     const int n0 = blockIdx.x * BLK, k0 = blockIdx.y * BLK, tid = threadIdx.x;
     const int ldk = (K + 15) & ~15, ldn = (N + 15) & ~15;
-    float f[64];
+    float f[16];
     uint32_t m = 0;
     // (lanes run along whichever axis is contiguous)
     const bool kfast = sc == 1;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) {
-        const int fast = tid & 127, slow = i * 2 + (tid >> 7);
+    for (int i = 0; i < 16; ++i) {
+        const int fast = tid & 127, slow = i * 8 + (tid >> 7);
         const int r = kfast ? slow : fast, c = kfast ? fast : slow;
         f[i] = (n0 + r < N && k0 + c < K) ? Src<T>::one(w + (long)(n0 + r) * sr + (long)(k0 + c) * sc) : 0.f;
         const uint32_t u = __float_as_uint(f[i]) & 0x7fffffffu, v = u < 0x7f800000u ? u : 0u;
@@ -255,25 +256,25 @@ __global__ __launch_bounds__(TPB) void q8_pack_tile(const T* __restrict__ w, lon
     __syncthreads();
     m = part[0];
 #pragma unroll
-    for (int k = 1; k < TPB / 64; ++k) m = m > part[k] ? m : part[k];
+    for (int k = 1; k < TILE_TPB / 64; ++k) m = m > part[k] ? m : part[k];
     const uint32_t top = __float_as_uint(Src<T>::TOP);
     const uint32_t s = scale_of(m < top ? m : top);
     const float inv = inv_scale(s);
 #pragma unroll
-    for (int i = 0; i < 64; i += 8) {
+    for (int i = 0; i < 16; i += 8) {
         float g[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) g[k] = f[i + k];
         const uint2 e = encode8(g, inv, Src<T>::TOP);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int fast = tid & 127, slow = (i + k) * 2 + (tid >> 7);
+            const int fast = tid & 127, slow = (i + k) * 8 + (tid >> 7);
             const int r = kfast ? slow : fast, c = kfast ? fast : slow;
             tile[r * PITCH + c] = (unsigned char)((k < 4 ? e.x : e.y) >> (8 * (k & 3)));
         }
     }
     __syncthreads();
-    for (int p = tid; p < BLK * (BLK / 16); p += TPB) {
+    for (int p = tid; p < BLK * (BLK / 16); p += TILE_TPB) {
         const int r = p >> 3, ch = (p & 7) * 16;
         if (codes && n0 + r < N && k0 + ch < ldk)
             *reinterpret_cast<uint4*>(codes + (long)(n0 + r) * ldk + k0 + ch) = *reinterpret_cast<const uint4*>(tile + r * PITCH + ch);
@@ -317,7 +318,8 @@ MGN_PLAN_RO(MmParams, MGN_RO(a) MGN_RO(sa) MGN_RO(b) MGN_RO(sb) MGN_RO(bias))
 __device__ __forceinline__ float activate(float v, int act, float slope) { return act == 0 ? v : (v > 0.f ? v : (act == 1 ? (v == v ? 0.f : v) : v * slope)); }
 
 // four consecutive n of row m
-__device__ __forceinline__ void mm_emit(const MmParams& p, long m, int n, const float (&v)[4]) {
+template <typename P>
+__device__ __forceinline__ void mm_emit(const P& p, long m, int n, const float (&v)[4]) {
     float r[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -463,6 +465,202 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
 __global__ __launch_bounds__(512, 1) void q8_mm_256x256(MmParams p) { q8_mm_body<256, 256, 2, 4>(p); }
 __global__ __launch_bounds__(256, 2) void q8_mm_128x128(MmParams p) { q8_mm_body<128, 128, 2, 2>(p); }
 __global__ __launch_bounds__(256, 2) void q8_mm_128x32(MmParams p) { q8_mm_body<128, 32, 4, 1>(p); }
+
+// a lane's accumulators of NT 32-channel tiles: channels n0 + 32 t + 8 q + 4 hi + 0..3 of row m
+template <int NT, typename P>
+__device__ __forceinline__ void stream_store(const P& p, long m, int n0, int hi, const f32x16 (&acc)[NT]) {
+    const bool in = m < p.M;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        if (p.vec == 2) {
+            float v[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = n0 + t * 32 + 8 * q + 4 * hi;
+                const float4 b = (p.bias && n < p.N) ? *reinterpret_cast<const float4*>(p.bias + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[4 * q] = activate(acc[t][4 * q] + b.x, p.act, p.slope);
+                v[4 * q + 1] = activate(acc[t][4 * q + 1] + b.y, p.act, p.slope);
+                v[4 * q + 2] = activate(acc[t][4 * q + 2] + b.z, p.act, p.slope);
+                v[4 * q + 3] = activate(acc[t][4 * q + 3] + b.w, p.act, p.slope);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+                const auto s0 = __builtin_amdgcn_permlane32_swap(mgn_pack2(v[4 * q], v[4 * q + 1]), mgn_pack2(v[4 * q + 4], v[4 * q + 5]), false, false);
+                const auto s1 = __builtin_amdgcn_permlane32_swap(mgn_pack2(v[4 * q + 2], v[4 * q + 3]), mgn_pack2(v[4 * q + 6], v[4 * q + 7]), false, false);
+                const int n = n0 + t * 32 + 8 * (q + hi);
+                if (in && n < p.N) *reinterpret_cast<uint4*>((uint16_t*)p.out + m * p.ldo + n) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+            }
+        } else if (in) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = n0 + t * 32 + 8 * q + 4 * hi;
+                if (n >= p.N) continue;
+                const float v[4] = {acc[t][4 * q], acc[t][4 * q + 1], acc[t][4 * q + 2], acc[t][4 * q + 3]};
+                mm_emit(p, m, n, v);
+            }
+        }
+    }
+}
+
+// The product for short k (K <= 512) and many rows -- every 1x1 convolution of the network: bound by HBM (256 -> 256 at 1/8 resolution: 201 MB
+// for 34 GFLOP), so rows are streamed once through persistent blocks that keep their weights in REGISTERS.
+//   * a block owns 32 * NT * WN output channels; its waves hold the fragments of all KB blocks of k (NT * KB * 16 VGPRs);
+//   * a tile is BM whole rows (32 KB of source).  The next tile's rows are loaded into registers while the current one is multiplied, then
+//     become codes in one of two LDS tiles.  SRC 1 / 2: the source is 16-bit and the codes are made here exactly as q8_pack does (16 lanes
+//     per block of a row, four DPP steps) -- x is read once, and q8_pack's own pass (read x, write codes, read codes) disappears; SRC 2
+//     also stores codes and scales for the backward pass.  SRC 0: the source is packed already;
+//   * 16-byte chunk c of LDS row r at c ^ (r & 15) (KB = 1: c ^ ((r >> 1) & 7)): fragment reads of 16 neighbouring rows cover each bank once;
+//   * a lane ends up with 4 + 4 consecutive channels of a pixel; v_permlane32_swap joins them to 16-byte stores.
+// grid (row blocks, N / (32 NT WN)); the blocks of one row range sit on one XCD (grid.x % 8 == 0) and share its rows through L2.
+struct StreamParams {
+    const unsigned char* src;             // codes, or 16-bit rows of `ld` elements
+    const unsigned char* src_scales;
+    unsigned char *codes, *scales;        // SRC 2
+    const unsigned char *b, *sb;
+    const float* bias;
+    void* out;
+    int M, K, N, ld, ldc, ldb, ntiles;
+    long lds, ldb_s, ldo;
+    int act, out32, vec;                  // vec: 2 = 16-byte stores of 8 channels, 1 = of 4 elements, 0 = single elements
+    float slope;
+};
+MGN_PLAN_RO(StreamParams, MGN_RO(src) MGN_RO(src_scales) MGN_RO(b) MGN_RO(sb) MGN_RO(bias))
+
+template <int KB, int WN, int SRC>
+struct Stream {
+    static constexpr int TH = WN == 8 ? 512 : 256;                  // threads
+    static constexpr int BM = 128 / KB * (SRC == 0 ? 2 : 1) * (TH / 256);
+    static constexpr int PITCH = KB * BLK, TILE = BM * PITCH, LDS = 2 * (TILE + KB * BM);
+    static constexpr int LPU = SRC == 0 ? 8 : 16;                   // lanes per (row, block): 16 bytes of source each
+    static constexpr int PASS = BM * KB * LPU / TH;                  // 16-byte loads per thread and tile
+    static_assert(PASS == 8, "32 KB of source per 256 threads and tile");
+    __device__ static int swz(int r) { return KB == 1 ? (r >> 1) & 7 : r & 15; }
+};
+
+template <int KB, int NT, int WN, int SRC>
+__device__ __forceinline__ void q8_stream_body(const StreamParams& p) {
+    using S = Stream<KB, WN, SRC>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, hi = lane >> 5;
+    const int n0 = (blockIdx.y * WN + (WN == 1 ? 0 : wave)) * NT * 32;
+
+    // the wave's weights
+    i32x8 w[NT][KB * 2];
+    int ws[NT][KB];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int n = n0 + t * 32 + lr;
+        const unsigned char* row = p.b + (long)(n < p.N ? n : 0) * p.ldb;
+#pragma unroll
+        for (int kk = 0; kk < KB * 2; ++kk) {
+            int4 u[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = kk * 64 + hi * 32 + h * 16;
+                u[h] = (n < p.N && c < p.ldb) ? *reinterpret_cast<const int4*>(row + c) : make_int4(0, 0, 0, 0);
+            }
+            w[t][kk] = i32x8{u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) ws[t][kb] = (n < p.N && kb * BLK < p.K) ? p.sb[(long)kb * p.ldb_s + n] : 0;
+    }
+
+    // source: unit u = pass * (TH / LPU) + tid / LPU = (row u / KB, block u % KB)
+    const int ul = tid % S::LPU, u0 = tid / S::LPU, ukb = u0 % KB, urow = u0 / KB;   // (TH / LPU is a multiple of KB)
+    const int ucol = ukb * BLK + ul * (SRC == 0 ? 16 : 8);
+    constexpr int RSTEP = S::TH / S::LPU / KB;                       // rows per pass
+    uint4 q[8];
+    uint32_t qs = 0;
+    auto fetch = [&](int tile) {
+        const long r0 = (long)tile * S::BM;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const long r = r0 + urow + j * RSTEP;
+            q[j] = make_uint4(0, 0, 0, 0);
+            if (SRC == 0) {
+                if (r < p.M && ucol < p.ld) q[j] = *reinterpret_cast<const uint4*>(p.src + r * p.ld + ucol);
+            } else {
+                if (r < p.M && ucol < p.K) q[j] = *reinterpret_cast<const uint4*>(p.src + (r * p.ld + ucol) * 2);
+            }
+        }
+        if (SRC == 0 && tid < KB * S::BM / 4) {                      // four rows' scales of one block
+            const int kb = tid / (S::BM / 4);
+            const long r = r0 + (tid % (S::BM / 4)) * 4;
+            qs = (r < p.lds && kb * BLK < p.K) ? *reinterpret_cast<const uint32_t*>(p.src_scales + (long)kb * p.lds + r) : 0u;
+        }
+    };
+    auto settle = [&](int tile, int buf) {                           // registers -> LDS tile `buf` [-> packed form in memory]
+        unsigned char* st = q8_sm + buf * S::TILE;
+        unsigned char* sc = q8_sm + 2 * S::TILE + buf * KB * S::BM;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = urow + j * RSTEP;
+            if (SRC == 0) {
+                *reinterpret_cast<uint4*>(st + r * S::PITCH + (((ukb * 8 + ul) ^ S::swz(r)) << 4)) = q[j];
+            } else {
+                float f[8];
+                unpack8(q[j], f);
+                const uint32_t s = scale_of(group_max<16>(amax8(f, TOP16)));
+                const uint2 e = encode8(f, inv_scale(s), TOP16);
+                *reinterpret_cast<uint2*>(st + r * S::PITCH + (((ukb * 8 + (ul >> 1)) ^ S::swz(r)) << 4) + (ul & 1) * 8) = e;
+                if (ul == 0) sc[ukb * S::BM + r] = (unsigned char)s;
+                if (SRC == 2) {
+                    const long row = (long)tile * S::BM + r;
+                    if (row < p.M && ucol < p.ldc) *reinterpret_cast<uint2*>(p.codes + row * p.ldc + ucol) = e;
+                }
+            }
+        }
+        if (SRC == 0 && tid < KB * S::BM / 4) *reinterpret_cast<uint32_t*>(sc + tid * 4) = qs;
+    };
+
+    int tile = blockIdx.x, buf = 0;
+    if (tile < p.ntiles) fetch(tile);
+    for (; tile < p.ntiles; tile += gridDim.x, buf ^= 1) {
+        settle(tile, buf);
+        if (tile + (int)gridDim.x < p.ntiles) fetch(tile + gridDim.x);
+        __syncthreads();                  // this tile is in LDS; the tile before last, which the next settle() overwrites, has been read
+        const unsigned char* st = q8_sm + buf * S::TILE;
+        const unsigned char* sc = q8_sm + 2 * S::TILE + buf * KB * S::BM;
+        if (SRC == 2 && blockIdx.y == 0 && tid < KB * S::BM / 4) {
+            const int kb = tid / (S::BM / 4), r = (tid % (S::BM / 4)) * 4;
+            const long row = (long)tile * S::BM + r;
+            if (row < p.lds && kb * BLK < p.K) *reinterpret_cast<uint32_t*>(p.scales + (long)kb * p.lds + row) = *reinterpret_cast<const uint32_t*>(sc + kb * S::BM + r);
+        }
+#pragma unroll 1
+        for (int g = WN == 1 ? wave : 0; g < S::BM / 32; g += WN == 1 ? 4 : 1) {
+            const int r = g * 32 + lr;
+            const unsigned char* row = st + r * S::PITCH;
+            const int sw = S::swz(r);
+            f32x16 acc[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const int xs = sc[kb * S::BM + r];
+#pragma unroll
+                for (int kk = 2 * kb; kk < 2 * kb + 2; ++kk) {
+                    const int4 u = *reinterpret_cast<const int4*>(row + (((kk * 4 + hi * 2) ^ sw) << 4)), v = *reinterpret_cast<const int4*>(row + (((kk * 4 + hi * 2 + 1) ^ sw) << 4));
+                    const i32x8 x = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[t][kk], x, acc[t], 0, 0, 0, ws[t][kb], 0, xs);
+                }
+            }
+            const long m = (long)tile * S::BM + r;
+            stream_store<NT>(p, m, n0, hi, acc);
+        }
+    }
+}
+
+#define Q8_STREAM(KB, NT, WN) \
+    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##KB##_##NT##_##WN##_packed(StreamParams p) { q8_stream_body<KB, NT, WN, 0>(p); } \
+    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##KB##_##NT##_##WN##_h16(StreamParams p) { q8_stream_body<KB, NT, WN, 1>(p); } \
+    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##KB##_##NT##_##WN##_keep(StreamParams p) { q8_stream_body<KB, NT, WN, 2>(p); }
+Q8_STREAM(1, 1, 1) Q8_STREAM(2, 1, 1) Q8_STREAM(4, 1, 1)
+Q8_STREAM(1, 1, 4) Q8_STREAM(2, 1, 4) Q8_STREAM(4, 1, 4)
+Q8_STREAM(1, 2, 4) Q8_STREAM(2, 2, 4) Q8_STREAM(4, 1, 8)   // (4, 2, 4) would need 128 registers for the weights alone and spills
+#undef Q8_STREAM
 
 // Few tiles: a block per 32 x 32 outputs, the blocks of k dealt to its four waves, operands straight from memory into registers, the four
 // partial tiles added through LDS in wave order.
@@ -921,6 +1119,38 @@ inline int done() { return hipGetLastError() == hipSuccess ? MGN_OK : MGN_ELAUNC
 constexpr long MAX_ROWS = 0x7fffff00L;    // rows are counted in 32 bits (padded to 16), offsets in 64
 constexpr int MAX_COLS = 1 << 20;
 
+// The streaming product; MGN_ENOTSUP where another kernel is meant.  src_kind as SRC.
+int launch_stream(StreamParams p, int src_kind, hipStream_t s) {
+    const int KB = p.K <= 128 ? 1 : (p.K <= 256 ? 2 : 4);
+    if (p.K > 512) return MGN_ENOTSUP;
+    const int shape = p.N <= 32 ? 0 : (p.N <= 128 ? 1 : 2), chans = shape == 0 ? 32 : (shape == 1 ? 128 : 256);
+    const int th = KB == 4 && shape == 2 ? 512 : 256, BM = 128 / KB * (src_kind == 0 ? 2 : 1) * (th / 256), groups = (p.N + chans - 1) / chans;
+    p.ntiles = (int)(((long)p.M + BM - 1) / BM);
+    int gx = (512 * 256 / th) / groups & ~7;   // two blocks a CU (one of 512 threads)
+    if (gx < 8) return MGN_ENOTSUP;
+    gx = p.ntiles < gx ? p.ntiles : gx;
+    const int lds = 2 * (BM * KB * BLK + KB * BM);
+    typedef void (*K)(StreamParams);
+#define Q8_SHAPES(KB, LAST) {{q8_stream_##KB##_1_1_packed, q8_stream_##KB##_1_1_h16, q8_stream_##KB##_1_1_keep}, \
+                             {q8_stream_##KB##_1_4_packed, q8_stream_##KB##_1_4_h16, q8_stream_##KB##_1_4_keep}, \
+                             {q8_stream_##KB##_##LAST##_packed, q8_stream_##KB##_##LAST##_h16, q8_stream_##KB##_##LAST##_keep}}
+    static const K table[3][3][3] = {Q8_SHAPES(1, 2_4), Q8_SHAPES(2, 2_4), Q8_SHAPES(4, 1_8)};
+#undef Q8_SHAPES
+    K kernel = table[KB == 1 ? 0 : KB / 2][shape][src_kind];
+    if (lds > 65536) {                    
+        int dev = 0;
+        static bool ready[64][3][3][3] = {};
+        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MGN_ELAUNCH;
+        bool& r = ready[dev][KB == 1 ? 0 : KB / 2][shape][src_kind];
+        if (!r) {
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return MGN_ELAUNCH;
+            r = true;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)gx, (unsigned)groups), dim3(th), lds, s, p);
+    return done();
+}
+
 template <int BM, int BN, int WVM, int WVN>
 int launch_mm(void (*kernel)(MmParams), MmParams p, hipStream_t s) {
     using Tl = MmTile<BM, BN, WVM, WVN>;
@@ -1003,9 +1233,9 @@ int MGN_SYM(mgn_q8_pack_weight)(const void* w, int dtype, long sr, long sc, int 
     if ((!codes && !codes_t) || !codes != !scales || !codes_t != !scales_t || !aligned(codes, 16) || !aligned(codes_t, 16)) return MGN_EINVAL;
     const dim3 grid((unsigned)nblocks(N), (unsigned)nblocks(K));
     hipStream_t s = (hipStream_t)stream_;
-    if (dtype) hipLaunchKernelGGL(q8_pack_tile<uint16_t>, grid, dim3(TPB), 0, s, (const uint16_t*)w, sr, sc, N, K, (unsigned char*)codes,
+    if (dtype) hipLaunchKernelGGL(q8_pack_tile<uint16_t>, grid, dim3(TILE_TPB), 0, s, (const uint16_t*)w, sr, sc, N, K, (unsigned char*)codes,
                                   (unsigned char*)scales, (unsigned char*)codes_t, (unsigned char*)scales_t);
-    else hipLaunchKernelGGL(q8_pack_tile<float>, grid, dim3(TPB), 0, s, (const float*)w, sr, sc, N, K, (unsigned char*)codes, (unsigned char*)scales,
+    else hipLaunchKernelGGL(q8_pack_tile<float>, grid, dim3(TILE_TPB), 0, s, (const float*)w, sr, sc, N, K, (unsigned char*)codes, (unsigned char*)scales,
                             (unsigned char*)codes_t, (unsigned char*)scales_t);
     return done();
 }
@@ -1027,9 +1257,28 @@ int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const vo
         hipLaunchKernelGGL(q8_mm_small, dim3((unsigned)((N + 31) / 32), (unsigned)gy), dim3(TPB), 0, s, p);
         return done();
     }
+    if (K <= 512) {
+        StreamParams q = {p.a, p.sa, nullptr, nullptr, p.b, p.sb, bias, out, (int)M, K, N, p.ld, p.ld, p.ld, 0, p.lda_s, p.ldb_s, ldo, act, out_f32, p.vec, slope};
+        if (!out_f32 && N % 8 == 0 && ldo % 8 == 0 && aligned(out, 16) && aligned(bias, 16)) q.vec = 2;
+        const int rc = launch_stream(q, 0, s);
+        if (rc != MGN_ENOTSUP) return rc;
+    }
     if (N <= 32) return launch_mm<128, 32, 4, 1>(q8_mm_128x32, p, s);
     if (N > 128 && tiles(256, 256) >= 512) return launch_mm<256, 256, 2, 4>(q8_mm_256x256, p, s);
     return launch_mm<128, 128, 2, 2>(q8_mm_128x128, p, s);
+}
+
+int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* codes, void* scales, const void* b, const void* b_scales, int N,
+                                const float* bias, int act, float slope, void* out, int out_f32, long ldo, void* stream_) {
+    if (M < 0 || M > MAX_ROWS || N < 1 || N > MAX_COLS || K < 1 || K > MAX_COLS || act < 0 || act > 2 || ldo < N || ldx < K || ldx > MAX_COLS) return MGN_EINVAL;
+    if (M == 0) return MGN_OK;
+    if (!x || !b || !b_scales || !out || !codes != !scales || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(b, 16) || !aligned(x, 2) ||
+        !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;
+    if (K > 512 || K % 8 != 0 || ldx % 8 != 0 || !aligned(x, 16)) return MGN_ENOTSUP;
+    StreamParams p = {(const unsigned char*)x, nullptr, (unsigned char*)codes, (unsigned char*)scales, (const unsigned char*)b, (const unsigned char*)b_scales, bias, out,
+                      (int)M, K, N, (int)ldx, code_ld(K), code_ld(K), 0, scale_ld(M), scale_ld(N), ldo, act, out_f32, 0, slope};
+    p.vec = (!out_f32 && N % 8 == 0 && ldo % 8 == 0 && aligned(out, 16) && aligned(bias, 16)) ? 2 : (ldo % 4 == 0 && aligned(out, out_f32 ? 16 : 8));
+    return launch_stream(p, codes ? 2 : 1, (hipStream_t)stream_);
 }
 
 #ifndef MGN_F16

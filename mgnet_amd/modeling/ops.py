@@ -1434,6 +1434,19 @@ def q8_matmul(a, b, bias=None, act="none", slope=0.01, out_dtype=None):
     return out.view(N, H, W, n).permute(0, 3, 1, 2)
 
 
+def _q8_product(x, keep, wc, ws, n, bias, act, out):
+    """out [M, n] = act(q(x) w^T + bias) for a map or matrix x -> (codes, scales) of x (they may be None unless `keep`)"""
+    from .. import _C
+    C = x.shape[1]
+    if x.is_contiguous(memory_format=torch.channels_last) if x.dim() == 4 else x.is_contiguous():
+        r = _C.q8_pack_matmul(x, out.shape[0], C, C, keep, wc, ws, n, bias, act, 0.0, out)
+        if r is not None:
+            return r
+    codes, scales = _q8_rows(x)
+    _C.q8_matmul(codes, scales, out.shape[0], wc, ws, n, C, bias, act, 0.0, out)
+    return codes, scales
+
+
 class _Conv1x1Q8Fn(torch.autograd.Function):
     """[HIP] csrc/q8.hip.  What waits for the backward pass is the packed input (1 byte a value instead of 2) and the packed transpose of
     the weights; the data gradient is the 8-bit product of the packed dy with it, the weight gradient multiplies dy in 16 bits with the
@@ -1444,12 +1457,12 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
         from .. import _C
         N, C, H, W = x.shape
         Cout, M = weight.shape[0], N * H * W
-        codes, scales = _q8_rows(x)
         (wc, ws), (tc, ts) = _C.q8_pack_weight(weight.detach().reshape(Cout, C), True, ctx.needs_input_grad[0])
         b = None if bias is None else bias.detach().float().contiguous()
         y = torch.empty((N, Cout, H, W), dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
-        _C.q8_matmul(codes, scales, M, wc, ws, Cout, C, b, int(relu), 0.0, y.permute(0, 2, 3, 1).view(M, Cout))
-        ctx.save_for_backward(codes, scales, tc, ts, y if relu else None)
+        keep = ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2])
+        codes, scales = _q8_product(x.detach(), keep, wc, ws, Cout, b, int(relu), y.permute(0, 2, 3, 1).view(M, Cout))
+        ctx.save_for_backward(*((codes, scales) if keep else (None, None)), tc, ts, y if relu else None)
         ctx.cfg = (x.shape, x.dtype, weight.dtype, tuple(weight.shape), None if bias is None else bias.dtype)
         return y
 
@@ -1463,24 +1476,24 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
         want_dx, want_dw, want_db = ctx.needs_input_grad[:3]
         want_db = want_db and bdtype is not None
         dx = dw = db = None
-        with _on(codes):
+        dev = dy.device
+        with _on(dy):
             if M == 0:
-                return (torch.empty((N, C, H, W), dtype=dtype, device=codes.device) if want_dx else None,
-                        torch.zeros(wshape, dtype=wdtype, device=codes.device) if want_dw else None,
-                        torch.zeros(Cout, dtype=bdtype, device=codes.device) if want_db else None, None)
+                return (torch.empty((N, C, H, W), dtype=dtype, device=dev) if want_dx else None,
+                        torch.zeros(wshape, dtype=wdtype, device=dev) if want_dw else None,
+                        torch.zeros(Cout, dtype=bdtype, device=dev) if want_db else None, None)
             dy = dy.to(dtype).contiguous(memory_format=torch.channels_last)
             if y is not None:
                 dy = _C.relu_mask_bwd(dy, y) if _C.elt_supported(y) and _C.elt_supported(dy) else dy * (y > 0)
             rows = dy.permute(0, 2, 3, 1).reshape(M, Cout)     # (a view: dy is channels-last)
             if want_dx:
-                dc, ds = _C.q8_pack(rows, M, Cout, rows.stride(0) if M > 1 else Cout, 0, 0, 1, 1)
-                dx = torch.empty((N, C, H, W), dtype=dtype, device=codes.device, memory_format=torch.channels_last)
-                _C.q8_matmul(dc, ds, M, tc, ts, C, Cout, None, 0, 0.0, dx.permute(0, 2, 3, 1).view(M, C))
+                dx = torch.empty((N, C, H, W), dtype=dtype, device=dev, memory_format=torch.channels_last)
+                _q8_product(rows, False, tc, ts, C, None, 0, dx.permute(0, 2, 3, 1).view(M, C))
             if want_dw or want_db:
                 ldy = Cout
                 if Cout % 8 or rows.data_ptr() % 16:           # the kernel loads 16-byte pieces of rows
                     ldy = (Cout + 7) // 8 * 8
-                    padded = torch.empty((M, ldy), dtype=dtype, device=codes.device)
+                    padded = torch.empty((M, ldy), dtype=dtype, device=dev)
                     padded[:, :Cout].copy_(rows)
                     rows = padded
                 dw, db = _C.q8_wgrad(rows, ldy, M, Cout, codes, scales, C, want_db)
