@@ -807,8 +807,8 @@ int mgn_project_bwd(const float* points, const float* A, const float* t, const f
  * mgn_q8_matmul     : out[m][n] = act( sum_k a[m][k] b[n][k] + bias[n] ), a [M][K], b [N][K] packed, fp32 accumulation, one rounding;
  *                     act 0 none | 1 ReLU | 2 leaky ReLU; out fp32 or 16-bit, rows ldo elements apart.
  * mgn_q8_pack_matmul: mgn_q8_pack of the 16-bit matrix x [M][K] (rows ldx elements apart) and mgn_q8_matmul of its packed form in one pass
- *                     over x; codes / scales: where the packed form is kept, or both NULL.  MGN_ENOTSUP (nothing done): K > 512, K % 8 or
- *                     ldx % 8 != 0, x not 16-byte aligned -- pack first then.  Same result as the two calls up to the order of the fp32 sums.
+ *                     over x; codes / scales: where the packed form is kept, or both NULL.  MGN_ENOTSUP (nothing done; pack first then):
+ *                     K > 512, K % 8 or ldx % 8 != 0, x not 16-byte aligned; N > 32 with N % 8 or ldo % 8 != 0 or an fp32 result.  Same result as the two calls up to the order of the fp32 sums.
  * mgn_q8_wgrad      : dw[n][k] = sum_m dy[m][n] x[m][k] with dy 16-bit (rows ldy elements apart, ldy % 8 == 0, 16-byte aligned; columns
  *                     N .. ldy are ignored) and x packed; db[n] = sum_m dy[m][n] (nullable).  Fixed summation order.
  * ---------------------------------------------------------------------------------------------- */

@@ -303,19 +303,26 @@ __global__ __launch_bounds__(TILE_TPB) void q8_pack_tile(const T* __restrict__ w
 //   towards zero to a multiple of 2^-13 of the largest one's binade.  1.3e-5 of a result (2-norm, Gaussian operands): far below the
 //   rounding to 16 bits (1.7e-3 / 2.1e-4) and the operands' own (2.6e-2); a 32-bit result carries it.
 // ------------------------------------------------------------------------------------------------------
+// act(v) without a branch: ReLU is lo = 0, neg = 1; leaky ReLU lo = -inf, neg = slope; none lo = -inf, neg = 1 (a NaN passes all comparisons)
+struct Act { float lo, neg; };
+__device__ __forceinline__ float activate(float v, const Act& a) {
+    v = v < a.lo ? a.lo : v;
+    const float t = v * a.neg;
+    return v > 0.f ? v : t;
+}
+inline Act make_act(int act, float slope) { return Act{act == 1 ? 0.f : -__builtin_inff(), act == 2 ? slope : 1.f}; }
 struct MmParams {
     const unsigned char *a, *sa, *b, *sb;
     const float* bias;
     void* out;
     int M, N, K, nb, ld;                  // ld: bytes per code row (both operands)
     long lda_s, ldb_s, ldo;               // scale rows; elements per row of out
-    int act, out32, vec;                  // vec: rows of out are 4-element aligned
-    float slope;
+    Act act;
+    int out32, vec;                       // vec: rows of out are 4-element aligned
     int mt, nt, group;
 };
 MGN_PLAN_RO(MmParams, MGN_RO(a) MGN_RO(sa) MGN_RO(b) MGN_RO(sb) MGN_RO(bias))
 
-__device__ __forceinline__ float activate(float v, int act, float slope) { return act == 0 ? v : (v > 0.f ? v : (act == 1 ? (v == v ? 0.f : v) : v * slope)); }
 
 // four consecutive n of row m
 template <typename P>
@@ -324,7 +331,7 @@ __device__ __forceinline__ void mm_emit(const P& p, long m, int n, const float (
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const float b = (p.bias && n + e < p.N) ? p.bias[n + e] : 0.f;
-        r[e] = activate(v[e] + b, p.act, p.slope);
+        r[e] = activate(v[e] + b, p.act);
     }
     if (p.out32) {
         float* o = (float*)p.out + m * p.ldo + n;
@@ -466,42 +473,6 @@ __global__ __launch_bounds__(512, 1) void q8_mm_256x256(MmParams p) { q8_mm_body
 __global__ __launch_bounds__(256, 2) void q8_mm_128x128(MmParams p) { q8_mm_body<128, 128, 2, 2>(p); }
 __global__ __launch_bounds__(256, 2) void q8_mm_128x32(MmParams p) { q8_mm_body<128, 32, 4, 1>(p); }
 
-// a lane's accumulators of NT 32-channel tiles: channels n0 + 32 t + 8 q + 4 hi + 0..3 of row m
-template <int NT, typename P>
-__device__ __forceinline__ void stream_store(const P& p, long m, int n0, int hi, const f32x16 (&acc)[NT]) {
-    const bool in = m < p.M;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if (p.vec == 2) {
-            float v[16];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + t * 32 + 8 * q + 4 * hi;
-                const float4 b = (p.bias && n < p.N) ? *reinterpret_cast<const float4*>(p.bias + n) : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[4 * q] = activate(acc[t][4 * q] + b.x, p.act, p.slope);
-                v[4 * q + 1] = activate(acc[t][4 * q + 1] + b.y, p.act, p.slope);
-                v[4 * q + 2] = activate(acc[t][4 * q + 2] + b.z, p.act, p.slope);
-                v[4 * q + 3] = activate(acc[t][4 * q + 3] + b.w, p.act, p.slope);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; q += 2) {
-                const auto s0 = __builtin_amdgcn_permlane32_swap(mgn_pack2(v[4 * q], v[4 * q + 1]), mgn_pack2(v[4 * q + 4], v[4 * q + 5]), false, false);
-                const auto s1 = __builtin_amdgcn_permlane32_swap(mgn_pack2(v[4 * q + 2], v[4 * q + 3]), mgn_pack2(v[4 * q + 6], v[4 * q + 7]), false, false);
-                const int n = n0 + t * 32 + 8 * (q + hi);
-                if (in && n < p.N) *reinterpret_cast<uint4*>((uint16_t*)p.out + m * p.ldo + n) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
-            }
-        } else if (in) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + t * 32 + 8 * q + 4 * hi;
-                if (n >= p.N) continue;
-                const float v[4] = {acc[t][4 * q], acc[t][4 * q + 1], acc[t][4 * q + 2], acc[t][4 * q + 3]};
-                mm_emit(p, m, n, v);
-            }
-        }
-    }
-}
-
 // The product for short k (K <= 512) and many rows -- every 1x1 convolution of the network: bound by HBM (256 -> 256 at 1/8 resolution: 201 MB
 // for 34 GFLOP), so rows are streamed once through persistent blocks that keep their weights in REGISTERS.
 //   * a block owns 32 * NT * WN output channels; its waves hold the fragments of all KB blocks of k (NT * KB * 16 VGPRs);
@@ -521,23 +492,68 @@ struct StreamParams {
     void* out;
     int M, K, N, ld, ldc, ldb, ntiles;
     long lds, ldb_s, ldo;
-    int act, out32, vec;                  // vec: 2 = 16-byte stores of 8 channels, 1 = of 4 elements, 0 = single elements
-    float slope;
+    Act act;
+    int out32;
 };
 MGN_PLAN_RO(StreamParams, MGN_RO(src) MGN_RO(src_scales) MGN_RO(b) MGN_RO(sb) MGN_RO(bias))
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// a lane's accumulators of NT 32-channel tiles: channels n0 + 32 t + 8 q + 4 hi + 0..3 of row m; `bias` in LDS, from channel n0 on.
+// VEC: 16-byte stores of 8 channels through `rs` (rows of the tile from its first one on; what lies outside is dropped): no branch, so that
+// the number of stores in flight is known where the next tile's loads are waited for.
+template <int NT, bool VEC>
+__device__ __forceinline__ void stream_store(const StreamParams& p, __amdgpu_buffer_rsrc_t rs, long m0, int r, int n0, int hi, const float* bias, const f32x16 (&acc)[NT]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float v[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + t * 32 + 8 * q + 4 * hi);
+            v[4 * q] = activate(acc[t][4 * q] + b.x, p.act);
+            v[4 * q + 1] = activate(acc[t][4 * q + 1] + b.y, p.act);
+            v[4 * q + 2] = activate(acc[t][4 * q + 2] + b.z, p.act);
+            v[4 * q + 3] = activate(acc[t][4 * q + 3] + b.w, p.act);
+        }
+        if (VEC) {
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+                const auto s0 = __builtin_amdgcn_permlane32_swap(mgn_pack2(v[4 * q], v[4 * q + 1]), mgn_pack2(v[4 * q + 4], v[4 * q + 5]), false, false);
+                const auto s1 = __builtin_amdgcn_permlane32_swap(mgn_pack2(v[4 * q + 2], v[4 * q + 3]), mgn_pack2(v[4 * q + 6], v[4 * q + 7]), false, false);
+                const int n = n0 + t * 32 + 8 * (q + hi);
+                const u32x4 w = {(unsigned)s0[0], (unsigned)s1[0], (unsigned)s0[1], (unsigned)s1[1]};
+                __builtin_amdgcn_raw_buffer_store_b128(w, rs, n < p.N ? (r * (int)p.ldo + n) * 2 : OOB, 0, 0);
+            }
+        } else if (m0 + r < p.M) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = n0 + t * 32 + 8 * q + 4 * hi + e;
+                    if (n >= p.N) continue;
+                    if (p.out32) ((float*)p.out)[(m0 + r) * p.ldo + n] = v[4 * q + e];
+                    else ((uint16_t*)p.out)[(m0 + r) * p.ldo + n] = (uint16_t)mgn_f2h(v[4 * q + e]);
+                }
+        }
+    }
+}
+
+// bytes from the scale of row r0 of the first block to the end of the last block's scales
+__device__ __forceinline__ long scale_span(const StreamParams& p, long r0) { return (long)((p.K + BLK - 1) / BLK) * p.lds - r0; }
 
 template <int KB, int WN, int SRC>
 struct Stream {
     static constexpr int TH = WN == 8 ? 512 : 256;                  // threads
     static constexpr int BM = 128 / KB * (SRC == 0 ? 2 : 1) * (TH / 256);
-    static constexpr int PITCH = KB * BLK, TILE = BM * PITCH, LDS = 2 * (TILE + KB * BM);
+    static constexpr int PITCH = KB * BLK, TILE = BM * PITCH, LDS = 2 * (TILE + KB * BM) + 256 * 4;   // two tiles, their scales, the block's bias
     static constexpr int LPU = SRC == 0 ? 8 : 16;                   // lanes per (row, block): 16 bytes of source each
     static constexpr int PASS = BM * KB * LPU / TH;                  // 16-byte loads per thread and tile
     static_assert(PASS == 8, "32 KB of source per 256 threads and tile");
     __device__ static int swz(int r) { return KB == 1 ? (r >> 1) & 7 : r & 15; }
 };
 
-template <int KB, int NT, int WN, int SRC>
+template <int KB, int NT, int WN, int SRC, bool VEC>
 __device__ __forceinline__ void q8_stream_body(const StreamParams& p) {
     using S = Stream<KB, WN, SRC>;
     extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];
@@ -565,69 +581,78 @@ __device__ __forceinline__ void q8_stream_body(const StreamParams& p) {
         for (int kb = 0; kb < KB; ++kb) ws[t][kb] = (n < p.N && kb * BLK < p.K) ? p.sb[(long)kb * p.ldb_s + n] : 0;
     }
 
-    // source: unit u = pass * (TH / LPU) + tid / LPU = (row u / KB, block u % KB)
+    float* bias = reinterpret_cast<float*>(q8_sm + 2 * (S::TILE + KB * S::BM));
+    if (tid < NT * WN * 32) {
+        const int n = blockIdx.y * NT * WN * 32 + tid;
+        bias[tid] = (p.bias && n < p.N) ? p.bias[n] : 0.f;
+    }
+
+    // source: unit u = pass * (TH / LPU) + tid / LPU = (row u / KB, block u % KB).  All memory traffic of the loop goes through buffer
+    // descriptors of the tile's rows: rows and columns that are not there read as zeros and are not written, without a branch.
     const int ul = tid % S::LPU, u0 = tid / S::LPU, ukb = u0 % KB, urow = u0 / KB;   // (TH / LPU is a multiple of KB)
     const int ucol = ukb * BLK + ul * (SRC == 0 ? 16 : 8);
-    constexpr int RSTEP = S::TH / S::LPU / KB;                       // rows per pass
-    uint4 q[8];
+    constexpr int RSTEP = S::TH / S::LPU / KB;                      // rows per pass
+    constexpr int ES = SRC == 0 ? 1 : 2;                            // bytes per source element
+    const int soff = ucol < (SRC == 0 ? p.ld : p.K) ? (urow * p.ld + ucol) * ES : OOB;
+    const int srow = tid % (S::BM / 4) * 4, skb = tid / (S::BM / 4);   // the four scales this thread moves
+    const int qoff = tid < KB * S::BM / 4 && skb * BLK < p.K ? skb * (int)p.lds + srow : OOB;   // (p.lds < 2^31; see rsS)
+    u32x4 q[8];
     uint32_t qs = 0;
+    auto rows_of = [&](int tile) { const long left = p.M - (long)tile * S::BM; return (int)(left < S::BM ? (left > 0 ? left : 0) : S::BM); };
     auto fetch = [&](int tile) {
         const long r0 = (long)tile * S::BM;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.src + r0 * p.ld * ES), 0, (uint32_t)(rows_of(tile) * p.ld * ES), 0x00020000);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const long r = r0 + urow + j * RSTEP;
-            q[j] = make_uint4(0, 0, 0, 0);
-            if (SRC == 0) {
-                if (r < p.M && ucol < p.ld) q[j] = *reinterpret_cast<const uint4*>(p.src + r * p.ld + ucol);
-            } else {
-                if (r < p.M && ucol < p.K) q[j] = *reinterpret_cast<const uint4*>(p.src + (r * p.ld + ucol) * 2);
-            }
-        }
-        if (SRC == 0 && tid < KB * S::BM / 4) {                      // four rows' scales of one block
-            const int kb = tid / (S::BM / 4);
-            const long r = r0 + (tid % (S::BM / 4)) * 4;
-            qs = (r < p.lds && kb * BLK < p.K) ? *reinterpret_cast<const uint32_t*>(p.src_scales + (long)kb * p.lds + r) : 0u;
+        for (int j = 0; j < 8; ++j) q[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, soff + j * RSTEP * p.ld * ES, 0, 0);
+        if (SRC == 0) {
+            const __amdgpu_buffer_rsrc_t rsS = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.src_scales + r0), 0, (uint32_t)(tile < p.ntiles ? scale_span(p, r0) : 0), 0x00020000);
+            qs = __builtin_amdgcn_raw_buffer_load_b32(rsS, r0 + srow < p.lds ? qoff : OOB, 0, 0);
         }
     };
     auto settle = [&](int tile, int buf) {                           // registers -> LDS tile `buf` [-> packed form in memory]
         unsigned char* st = q8_sm + buf * S::TILE;
         unsigned char* sc = q8_sm + 2 * S::TILE + buf * KB * S::BM;
+        const __amdgpu_buffer_rsrc_t rs = SRC == 2 ? __builtin_amdgcn_make_buffer_rsrc(p.codes + (long)tile * S::BM * p.ldc, 0, blockIdx.y == 0 ? (uint32_t)(rows_of(tile) * p.ldc) : 0u, 0x00020000)
+                                                   : __builtin_amdgcn_make_buffer_rsrc(p.codes, 0, 0, 0x00020000);
+        const int coff = ucol < p.ldc ? urow * p.ldc + ucol : OOB;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int r = urow + j * RSTEP;
             if (SRC == 0) {
-                *reinterpret_cast<uint4*>(st + r * S::PITCH + (((ukb * 8 + ul) ^ S::swz(r)) << 4)) = q[j];
+                *reinterpret_cast<u32x4*>(st + r * S::PITCH + (((ukb * 8 + ul) ^ S::swz(r)) << 4)) = q[j];
             } else {
                 float f[8];
-                unpack8(q[j], f);
+                unpack8(make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]), f);
                 const uint32_t s = scale_of(group_max<16>(amax8(f, TOP16)));
                 const uint2 e = encode8(f, inv_scale(s), TOP16);
                 *reinterpret_cast<uint2*>(st + r * S::PITCH + (((ukb * 8 + (ul >> 1)) ^ S::swz(r)) << 4) + (ul & 1) * 8) = e;
                 if (ul == 0) sc[ukb * S::BM + r] = (unsigned char)s;
-                if (SRC == 2) {
-                    const long row = (long)tile * S::BM + r;
-                    if (row < p.M && ucol < p.ldc) *reinterpret_cast<uint2*>(p.codes + row * p.ldc + ucol) = e;
-                }
+                if (SRC == 2) __builtin_amdgcn_raw_buffer_store_b64(u32x2{e.x, e.y}, rs, coff + j * RSTEP * p.ldc, 0, 0);
             }
         }
         if (SRC == 0 && tid < KB * S::BM / 4) *reinterpret_cast<uint32_t*>(sc + tid * 4) = qs;
     };
 
     int tile = blockIdx.x, buf = 0;
-    if (tile < p.ntiles) fetch(tile);
-    for (; tile < p.ntiles; tile += gridDim.x, buf ^= 1) {
-        settle(tile, buf);
-        if (tile + (int)gridDim.x < p.ntiles) fetch(tile + gridDim.x);
-        __syncthreads();                  // this tile is in LDS; the tile before last, which the next settle() overwrites, has been read
+    if (tile >= p.ntiles) return;
+    fetch(tile);
+    settle(tile, 0);
+    for (;;) {
+        fetch(tile + gridDim.x);          // (behind the last tile there are no rows: nothing is loaded, and the loop keeps one shape)
+        __syncthreads();                  // this tile is in LDS; the tile before it, which settle() below overwrites, has been read
         const unsigned char* st = q8_sm + buf * S::TILE;
         const unsigned char* sc = q8_sm + 2 * S::TILE + buf * KB * S::BM;
-        if (SRC == 2 && blockIdx.y == 0 && tid < KB * S::BM / 4) {
-            const int kb = tid / (S::BM / 4), r = (tid % (S::BM / 4)) * 4;
-            const long row = (long)tile * S::BM + r;
-            if (row < p.lds && kb * BLK < p.K) *reinterpret_cast<uint32_t*>(p.scales + (long)kb * p.lds + row) = *reinterpret_cast<const uint32_t*>(sc + kb * S::BM + r);
+        const long m0 = (long)tile * S::BM;
+        if (SRC == 2) {
+            const __amdgpu_buffer_rsrc_t rsS = __builtin_amdgcn_make_buffer_rsrc(p.scales + m0, 0, blockIdx.y == 0 ? (uint32_t)scale_span(p, m0) : 0u, 0x00020000);
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(sc + (tid < KB * S::BM / 4 ? tid * 4 : 0));
+            __builtin_amdgcn_raw_buffer_store_b32(v, rsS, m0 + srow < p.lds ? qoff : OOB, 0, 0);
         }
-#pragma unroll 1
-        for (int g = WN == 1 ? wave : 0; g < S::BM / 32; g += WN == 1 ? 4 : 1) {
+        const __amdgpu_buffer_rsrc_t rsO = __builtin_amdgcn_make_buffer_rsrc((uint16_t*)p.out + m0 * p.ldo, 0, VEC ? (uint32_t)(rows_of(tile) * (int)p.ldo * 2) : 0u, 0x00020000);
+#pragma unroll
+        for (int gi = 0; gi < S::BM / 32; gi += WN == 1 ? 4 : 1) {
+            const int g = gi + (WN == 1 ? wave : 0);
+            if (WN == 1 && S::BM < 128 && g >= S::BM / 32) break;
             const int r = g * 32 + lr;
             const unsigned char* row = st + r * S::PITCH;
             const int sw = S::swz(r);
@@ -647,19 +672,23 @@ __device__ __forceinline__ void q8_stream_body(const StreamParams& p) {
                     for (int t = 0; t < NT; ++t) acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[t][kk], x, acc[t], 0, 0, 0, ws[t][kb], 0, xs);
                 }
             }
-            const long m = (long)tile * S::BM + r;
-            stream_store<NT>(p, m, n0, hi, acc);
+            stream_store<NT, VEC>(p, rsO, m0, r, n0, hi, bias + (WN == 1 ? 0 : wave) * NT * 32, acc);
         }
+        tile += gridDim.x;
+        if (tile >= p.ntiles) break;
+        buf ^= 1;
+        settle(tile, buf);                // (loads and the stores behind them lie in one piece of straight code: only the loads are waited for)
     }
 }
 
-#define Q8_STREAM(KB, NT, WN) \
-    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##KB##_##NT##_##WN##_packed(StreamParams p) { q8_stream_body<KB, NT, WN, 0>(p); } \
-    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##KB##_##NT##_##WN##_h16(StreamParams p) { q8_stream_body<KB, NT, WN, 1>(p); } \
-    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##KB##_##NT##_##WN##_keep(StreamParams p) { q8_stream_body<KB, NT, WN, 2>(p); }
-Q8_STREAM(1, 1, 1) Q8_STREAM(2, 1, 1) Q8_STREAM(4, 1, 1)
-Q8_STREAM(1, 1, 4) Q8_STREAM(2, 1, 4) Q8_STREAM(4, 1, 4)
-Q8_STREAM(1, 2, 4) Q8_STREAM(2, 2, 4) Q8_STREAM(4, 1, 8)   // (4, 2, 4) would need 128 registers for the weights alone and spills
+#define Q8_STREAM(NAME, KB, NT, WN, VEC) \
+    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##NAME##_packed(StreamParams p) { q8_stream_body<KB, NT, WN, 0, VEC>(p); } \
+    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##NAME##_h16(StreamParams p) { q8_stream_body<KB, NT, WN, 1, VEC>(p); } \
+    __global__ __launch_bounds__(WN == 8 ? 512 : 256, 2) void q8_stream_##NAME##_keep(StreamParams p) { q8_stream_body<KB, NT, WN, 2, VEC>(p); }
+Q8_STREAM(1_any, 1, 1, 1, false) Q8_STREAM(2_any, 2, 1, 1, false) Q8_STREAM(4_any, 4, 1, 1, false)      // N <= 32: any N and result type
+Q8_STREAM(1_32, 1, 1, 1, true) Q8_STREAM(2_32, 2, 1, 1, true) Q8_STREAM(4_32, 4, 1, 1, true)
+Q8_STREAM(1_128, 1, 1, 4, true) Q8_STREAM(2_128, 2, 1, 4, true) Q8_STREAM(4_128, 4, 1, 4, true)
+Q8_STREAM(1_256, 1, 2, 4, true) Q8_STREAM(2_256, 2, 2, 4, true) Q8_STREAM(4_256, 4, 1, 8, true)         // (<4, 2, 4>: 128 registers for the weights alone, spills)
 #undef Q8_STREAM
 
 // Few tiles: a block per 32 x 32 outputs, the blocks of k dealt to its four waves, operands straight from memory into registers, the four
@@ -1121,27 +1150,29 @@ constexpr int MAX_COLS = 1 << 20;
 
 // The streaming product; MGN_ENOTSUP where another kernel is meant.  src_kind as SRC.
 int launch_stream(StreamParams p, int src_kind, hipStream_t s) {
-    const int KB = p.K <= 128 ? 1 : (p.K <= 256 ? 2 : 4);
-    if (p.K > 512) return MGN_ENOTSUP;
-    const int shape = p.N <= 32 ? 0 : (p.N <= 128 ? 1 : 2), chans = shape == 0 ? 32 : (shape == 1 ? 128 : 256);
-    const int th = KB == 4 && shape == 2 ? 512 : 256, BM = 128 / KB * (src_kind == 0 ? 2 : 1) * (th / 256), groups = (p.N + chans - 1) / chans;
+    if (p.K > 512 || p.lds * 4 > 0x7fffffffL) return MGN_ENOTSUP;
+    const bool vec = !p.out32 && p.N % 8 == 0 && p.ldo % 8 == 0 && p.ldo <= MAX_COLS && aligned(p.out, 16);
+    if (!vec && p.N > 32) return MGN_ENOTSUP;
+    const int ki = p.K <= 128 ? 0 : (p.K <= 256 ? 1 : 2), KB = 1 << ki;
+    const int shape = !vec ? 0 : (p.N <= 32 ? 1 : (p.N <= 128 ? 2 : 3)), chans = shape <= 1 ? 32 : (shape == 2 ? 128 : 256);
+    const int th = KB == 4 && shape == 3 ? 512 : 256, BM = 128 / KB * (src_kind == 0 ? 2 : 1) * (th / 256), groups = (p.N + chans - 1) / chans;
     p.ntiles = (int)(((long)p.M + BM - 1) / BM);
     int gx = (512 * 256 / th) / groups & ~7;   // two blocks a CU (one of 512 threads)
     if (gx < 8) return MGN_ENOTSUP;
     gx = p.ntiles < gx ? p.ntiles : gx;
-    const int lds = 2 * (BM * KB * BLK + KB * BM);
+    const int lds = 2 * (BM * KB * BLK + KB * BM) + 1024;
     typedef void (*K)(StreamParams);
-#define Q8_SHAPES(KB, LAST) {{q8_stream_##KB##_1_1_packed, q8_stream_##KB##_1_1_h16, q8_stream_##KB##_1_1_keep}, \
-                             {q8_stream_##KB##_1_4_packed, q8_stream_##KB##_1_4_h16, q8_stream_##KB##_1_4_keep}, \
-                             {q8_stream_##KB##_##LAST##_packed, q8_stream_##KB##_##LAST##_h16, q8_stream_##KB##_##LAST##_keep}}
-    static const K table[3][3][3] = {Q8_SHAPES(1, 2_4), Q8_SHAPES(2, 2_4), Q8_SHAPES(4, 1_8)};
-#undef Q8_SHAPES
-    K kernel = table[KB == 1 ? 0 : KB / 2][shape][src_kind];
-    if (lds > 65536) {                    
+#define Q8_SRC(N) {q8_stream_##N##_packed, q8_stream_##N##_h16, q8_stream_##N##_keep}
+    static const K table[3][4][3] = {{Q8_SRC(1_any), Q8_SRC(1_32), Q8_SRC(1_128), Q8_SRC(1_256)},
+                                     {Q8_SRC(2_any), Q8_SRC(2_32), Q8_SRC(2_128), Q8_SRC(2_256)},
+                                     {Q8_SRC(4_any), Q8_SRC(4_32), Q8_SRC(4_128), Q8_SRC(4_256)}};
+#undef Q8_SRC
+    K kernel = table[ki][shape][src_kind];
+    if (lds > 65536) {
         int dev = 0;
-        static bool ready[64][3][3][3] = {};
+        static bool ready[64][3][4][3] = {};
         if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MGN_ELAUNCH;
-        bool& r = ready[dev][KB == 1 ? 0 : KB / 2][shape][src_kind];
+        bool& r = ready[dev][ki][shape][src_kind];
         if (!r) {
             if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return MGN_ELAUNCH;
             r = true;
@@ -1247,7 +1278,7 @@ int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const vo
     if (!a || !a_scales || !b || !b_scales || !out || !aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 16) || !aligned(b_scales, 16) ||
         !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;
     MmParams p = {(const unsigned char*)a, (const unsigned char*)a_scales, (const unsigned char*)b, (const unsigned char*)b_scales, bias, out,
-                  (int)M, N, K, nblocks(K), code_ld(K), scale_ld(M), scale_ld(N), ldo, act, out_f32, 0, slope, 0, 0, 1};
+                  (int)M, N, K, nblocks(K), code_ld(K), scale_ld(M), scale_ld(N), ldo, make_act(act, slope), out_f32, 0, 0, 0, 1};
     p.vec = ldo % 4 == 0 && aligned(out, out_f32 ? 16 : 8);
     hipStream_t s = (hipStream_t)stream_;
     auto tiles = [&](int BM, int BN) { return ((M + BM - 1) / BM) * ((N + BN - 1) / BN); };
@@ -1258,8 +1289,7 @@ int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const vo
         return done();
     }
     if (K <= 512) {
-        StreamParams q = {p.a, p.sa, nullptr, nullptr, p.b, p.sb, bias, out, (int)M, K, N, p.ld, p.ld, p.ld, 0, p.lda_s, p.ldb_s, ldo, act, out_f32, p.vec, slope};
-        if (!out_f32 && N % 8 == 0 && ldo % 8 == 0 && aligned(out, 16) && aligned(bias, 16)) q.vec = 2;
+        StreamParams q = {p.a, p.sa, nullptr, nullptr, p.b, p.sb, bias, out, (int)M, K, N, p.ld, p.ld, p.ld, 0, p.lda_s, p.ldb_s, ldo, make_act(act, slope), out_f32};
         const int rc = launch_stream(q, 0, s);
         if (rc != MGN_ENOTSUP) return rc;
     }
@@ -1276,8 +1306,7 @@ int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* co
         !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;
     if (K > 512 || K % 8 != 0 || ldx % 8 != 0 || !aligned(x, 16)) return MGN_ENOTSUP;
     StreamParams p = {(const unsigned char*)x, nullptr, (unsigned char*)codes, (unsigned char*)scales, (const unsigned char*)b, (const unsigned char*)b_scales, bias, out,
-                      (int)M, K, N, (int)ldx, code_ld(K), code_ld(K), 0, scale_ld(M), scale_ld(N), ldo, act, out_f32, 0, slope};
-    p.vec = (!out_f32 && N % 8 == 0 && ldo % 8 == 0 && aligned(out, 16) && aligned(bias, 16)) ? 2 : (ldo % 4 == 0 && aligned(out, out_f32 ? 16 : 8));
+                      (int)M, K, N, (int)ldx, code_ld(K), code_ld(K), 0, scale_ld(M), scale_ld(N), ldo, make_act(act, slope), out_f32};
     return launch_stream(p, codes ? 2 : 1, (hipStream_t)stream_);
 }
 
