@@ -390,8 +390,7 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
         const int r = (wave + Tl::NW * q) * 8 + (lane >> 3);
         offB[q] = r < rowsB ? r * p.ld + col : OOB;
     }
-    auto issue = [&](int kb, int buf) {
-        unsigned char* st = q8_sm + buf * (Tl::STAGE + Tl::SCALES);
+    auto issue = [&](int kb, unsigned char* st) {
         const int k0 = kb * BLK;
         const bool in = k0 + col < p.ld;   // (OOB + k0 stays beyond every descriptor)
 #pragma unroll
@@ -418,13 +417,11 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
     const int sw = (lr >> 1) & 7;         // (tile bases are multiples of 32 rows)
-    issue(0, 0);
-    for (int kb = 0; kb < p.nb; ++kb) {
-        const int buf = kb & 1;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();     // everyone's rows of step kb have landed, and step kb - 1 has been read
-        if (kb + 1 < p.nb) issue(kb + 1, buf ^ 1);
-        const unsigned char* st = q8_sm + buf * (Tl::STAGE + Tl::SCALES);
+    // One step: start the next stage's loads, multiply this one.  The two pointers are restrict (and the waits outside) because the compiler
+    // otherwise takes every LDS read after an LDS-DMA for a read of its target and puts a full s_waitcnt vmcnt(0) between the two, which
+    // makes the two stages one: measured 1.9x on a large product.
+    auto step = [&](int kb, const unsigned char* __restrict__ st, unsigned char* __restrict__ next) {
+        if (kb + 1 < p.nb) issue(kb + 1, next);
         int xs[Tl::TM], ws[Tl::TN];
 #pragma unroll
         for (int j = 0; j < Tl::TM; ++j) xs[j] = st[Tl::STAGE + (wm * Tl::TM + j) * 32 + lr];
@@ -452,6 +449,12 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
                 for (int j = 0; j < Tl::TM; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], x[j], acc[i][j], 0, 0, 0, ws[i], 0, xs[j]);
         }
+    };
+    issue(0, q8_sm);
+    for (int kb = 0; kb < p.nb; ++kb) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();     // everyone's rows of step kb have landed, and step kb - 1 has been read
+        step(kb, q8_sm + (kb & 1) * (Tl::STAGE + Tl::SCALES), q8_sm + (~kb & 1) * (Tl::STAGE + Tl::SCALES));
     }
 #pragma unroll
     for (int j = 0; j < Tl::TM; ++j) {
@@ -734,15 +737,15 @@ __global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
 
 // ------------------------------------------------------------------------------------------------------
 // dW[n][k] = sum_m dy[m][n] x^[m][k], db[n] = sum_m dy[m][n]: dy in 16 bits, x^ from its codes.
-//   A block computes a 128 x 128 tile over one of `splits` row ranges.  dy rows go to LDS by LDS-DMA, codes through registers, where a
-//   value and its scale become the exact 16-bit x^ (one instruction for two); both tiles are read back with the transposing LDS reads,
-//   since the summed index is the row.  v_mfma_f32_32x32x16, fp32 accumulation; the splits' tiles are added by q8_wgrad_reduce in order.
+//   A block computes a 128 x 128 tile over one of `splits` row ranges.  dy rows go to LDS by LDS-DMA (three stages), codes through
+//   registers, where a value and its scale become the exact 16-bit x^ (one instruction for two); both tiles are read back with the
+//   transposing LDS reads, since the summed index is the row.  Loads run two steps ahead (80 KB of LDS: two blocks a CU).  v_mfma_f32_32x32x16, fp32 accumulation; the splits' tiles are added by q8_wgrad_reduce in order.
 //   db: the same dy fragments times a column of ones, in the blocks of the first k tile.
 // ------------------------------------------------------------------------------------------------------
 struct WgradParams8 {
     const uint16_t* dy;
     const unsigned char *codes, *scales;
-    float* part;                          // [splits][N * K + N]
+    float* part;                          // [splits][N * K + N, padded to 4]
     int M, N, K, ldy, ldc;
     long lds;
     int rows_per_split, splits, ntn, ntk;
@@ -751,7 +754,7 @@ MGN_PLAN_RO(WgradParams8, MGN_RO(dy) MGN_RO(codes) MGN_RO(scales))
 
 constexpr int WG_ROWS = 64;               // rows per step
 constexpr int WG_TILE = WG_ROWS * 256;    // bytes of a [64][128] 16-bit tile
-constexpr int WG_LDS = 4 * WG_TILE;
+constexpr int WG_LDS = 5 * WG_TILE;       // dy x 3, x^ x 2
 
 __device__ __forceinline__ uint32_t decode2(uint32_t c, float s, int word) {
 #ifdef MGN_F16
@@ -782,37 +785,35 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
         const int r = (wave + 4 * q) * 4 + (lane >> 4), ch = (lane & 15) ^ swz(r);
         yo[q] = tn * 128 + ch * 8 < p.ldy ? r * p.ldy * 2 + (tn * 128 + ch * 8) * 2 : OOB;
     }
-    auto issue = [&](int ks, int buf) {
+    auto issue = [&](int ks, unsigned char* st) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int r = ks * WG_ROWS + (wave + 4 * q) * 4 + (lane >> 4);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsY, (lds_ptr)(q8_sm + buf * WG_TILE + (wave + 4 * q) * 1024), 16,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsY, (lds_ptr)(st + (wave + 4 * q) * 1024), 16,
                                                      (r < rows && yo[q] != OOB) ? yo[q] + ks * WG_ROWS * p.ldy * 2 : OOB, 0, 0, 0);
         }
     };
     // codes: thread = (row tid / 4, 32 columns)
     const int cr = tid >> 2, cc = (tid & 3) * 32, kcol = tk * BLK + cc;
-    uint4 cq[2];
-    uint32_t cs = 0;
+    const __amdgpu_buffer_rsrc_t rsX = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.codes + mb * p.ldc), 0, (uint32_t)(rows * p.ldc), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsC = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.scales + (long)tk * p.lds + mb), 0, (uint32_t)rows, 0x00020000);
+    const int xo0 = kcol < p.ldc ? cr * p.ldc + kcol : OOB, xo1 = kcol + 16 < p.ldc ? cr * p.ldc + kcol + 16 : OOB;
+    struct Fetched { u32x4 lo, hi; uint32_t s; };
     auto fetch = [&](int ks) {
-        const int r = ks * WG_ROWS + cr;
-        cq[0] = cq[1] = make_uint4(0, 0, 0, 0);
-        cs = 0;
-        if (r < rows) {
-            const unsigned char* src = p.codes + (mb + r) * p.ldc + kcol;
-            if (kcol < p.ldc) cq[0] = *reinterpret_cast<const uint4*>(src);
-            if (kcol + 16 < p.ldc) cq[1] = *reinterpret_cast<const uint4*>(src + 16);
-            cs = p.scales[(long)tk * p.lds + mb + r];
-        }
+        Fetched f;
+        f.lo = __builtin_amdgcn_raw_buffer_load_b128(rsX, xo0 + ks * WG_ROWS * p.ldc, 0, 0);
+        f.hi = __builtin_amdgcn_raw_buffer_load_b128(rsX, xo1 + ks * WG_ROWS * p.ldc, 0, 0);
+        f.s = __builtin_amdgcn_raw_buffer_load_b8(rsC, cr + ks * WG_ROWS, 0, 0);
+        return f;
     };
-    auto spread = [&](int buf) {
-        unsigned char* b = q8_sm + (2 + buf) * WG_TILE + cr * 256;
-        const float s = pow2(cs);
+    auto spread = [&](const Fetched& f, unsigned char* __restrict__ tile) {
+        unsigned char* b = tile + cr * 256;
+        const float s = pow2(f.s);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint4 c = cq[h];
-            const uint4 lo = make_uint4(decode2(c.x, s, 0), decode2(c.x, s, 1), decode2(c.y, s, 0), decode2(c.y, s, 1));
-            const uint4 up = make_uint4(decode2(c.z, s, 0), decode2(c.z, s, 1), decode2(c.w, s, 0), decode2(c.w, s, 1));
+            const u32x4 c = h ? f.hi : f.lo;
+            const uint4 lo = make_uint4(decode2(c[0], s, 0), decode2(c[0], s, 1), decode2(c[1], s, 0), decode2(c[1], s, 1));
+            const uint4 up = make_uint4(decode2(c[2], s, 0), decode2(c[2], s, 1), decode2(c[3], s, 0), decode2(c[3], s, 1));
             const int ch = (cc >> 3) + 2 * h;
             *reinterpret_cast<uint4*>(b + ((ch ^ swz(cr)) << 4)) = lo;
             *reinterpret_cast<uint4*>(b + (((ch + 1) ^ swz(cr)) << 4)) = up;
@@ -825,7 +826,7 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
     for (int i = 0; i < 2; ++i) {
         const int ca = wm * 64 + i * 32 + (g & 1) * 16 + 4 * (i4 & 3), cb = wn * 64 + i * 32 + (g & 1) * 16 + 4 * (i4 & 3);
         fa[i] = prow * 256 + (((ca >> 3) ^ swz(prow)) << 4) + (ca & 7) * 2;
-        fb[i] = 2 * WG_TILE + prow * 256 + (((cb >> 3) ^ swz(prow)) << 4) + (cb & 7) * 2;
+        fb[i] = prow * 256 + (((cb >> 3) ^ swz(prow)) << 4) + (cb & 7) * 2;
     }
     typedef __attribute__((address_space(3))) s16x4* lp;
     auto frag = [&](const unsigned char* q) {
@@ -844,25 +845,18 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
     for (int e = 0; e < 8; ++e) ones[e] = (decltype(ones[0] + ones[0]))1.0f;
     const bool with_db = tk == 0 && wn == 0;
 
-    issue(0, 0);
-    fetch(0);
-    for (int ks = 0; ks < steps; ++ks) {
-        const int buf = ks & 1;
-        spread(buf);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();     // step ks is in LDS; step ks - 1 has been read by everyone
-        if (ks + 1 < steps) {
-            issue(ks + 1, buf ^ 1);
-            fetch(ks + 1);
-        }
-        const unsigned char* st = q8_sm + buf * WG_TILE;
+    // In flight at the top of step ks: the loads of steps ks and ks + 1, 4 LDS-DMA and 3 register loads each, in this order.
+    // (restrict pointers, waits outside: see q8_mm_body)
+    auto multiply = [&](int ks, const unsigned char* __restrict__ sa, const unsigned char* __restrict__ sb, unsigned char* __restrict__ next, Fetched& f) {
+        issue(ks + 2, next);              // (rows behind the range load nothing)
+        f = fetch(ks + 2);
 #pragma unroll
         for (int kk = 0; kk < WG_ROWS / 16; ++kk) {   // the swizzle depends on row bits 0..1: unchanged by + 16 rows
             h16x8 a[2], b[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                a[i] = frag(st + fa[i] + kk * 16 * 256);
-                b[i] = frag(st + fb[i] + kk * 16 * 256);
+                a[i] = frag(sa + fa[i] + kk * 16 * 256);
+                b[i] = frag(sb + fb[i] + kk * 16 * 256);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -873,8 +867,31 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
                 accb[1] = MGN_MFMA_32x32x16(a[1], ones, accb[1]);
             }
         }
+    };
+    auto step = [&](int ks, int a_buf, Fetched& f) {
+        asm volatile("s_waitcnt vmcnt(7)" ::: "memory");   // step ks has landed
+        unsigned char* xb = q8_sm + (3 + (ks & 1)) * WG_TILE;
+        spread(f, xb);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();     // ... for everyone; step ks - 1 has been read
+        multiply(ks, q8_sm + a_buf * WG_TILE, xb, q8_sm + (a_buf == 0 ? 2 : a_buf - 1) * WG_TILE, f);
+    };
+    issue(0, q8_sm);
+    Fetched f0 = fetch(0);
+    __builtin_amdgcn_sched_barrier(0);    // (in this order: the loop's waits count on it)
+    issue(1, q8_sm + WG_TILE);
+    __builtin_amdgcn_sched_barrier(0);
+    Fetched f1 = fetch(1);
+    __builtin_amdgcn_sched_barrier(0);
+    int a_buf = 0;
+    for (int ks = 0; ks < steps; ks += 2) {   // (an odd last step multiplies rows of zeros)
+        step(ks, a_buf, f0);
+        a_buf = a_buf == 2 ? 0 : a_buf + 1;
+        step(ks + 1, a_buf, f1);
+        a_buf = a_buf == 2 ? 0 : a_buf + 1;
     }
-    const long wsize = (long)p.N * p.K + p.N;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no LDS-DMA outlives the block
+    const long wsize = ((long)p.N * p.K + p.N + 3) & ~3L;
     float* out = p.part + (long)z * wsize;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -891,23 +908,38 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
         }
 }
 
-// dw | db = the splits' partial results added in order; 16 groups of splits side by side, joined in group order
-__global__ __launch_bounds__(TPB) void q8_wgrad_reduce(const float* __restrict__ part, int splits, long total, long nk, float* __restrict__ dw,
-                                                       float* __restrict__ db) {
-    __shared__ float sh[16][17];
-    const int col = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const long i = (long)blockIdx.x * 16 + col;
-    float s = 0.f;
-    if (i < total)
-        for (int z = g; z < splits; z += 16) s += part[(long)z * total + i];
-    sh[g][col] = s;
-    __syncthreads();
-    if (g == 0 && i < total) {
-        float r = sh[0][col];
+// dw | db = the splits' partial results added in a fixed order: 16 waves take every 16th split of 256 neighbouring sums (1 KB a wave and
+// split, up to 8 splits in flight), joined in wave order
+__global__ __launch_bounds__(1024) void q8_wgrad_reduce(const float* __restrict__ part, int splits, long total, long nk, float* __restrict__ dw,
+                                                        float* __restrict__ db) {
+    __shared__ float4 sh[16][64];
+    const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const long stride = (total + 3) & ~3L, i = ((long)blockIdx.x * 64 + lane) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < stride) {
+        const float* src = part + i;
+        int z = g;
+        for (; z + 7 * 16 < splits; z += 8 * 16) {
+            float4 v[8];
 #pragma unroll
-        for (int k = 1; k < 16; ++k) r += sh[k][col];
-        if (i < nk) dw[i] = r;
-        else if (db) db[i - nk] = r;
+            for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const float4*>(src + (long)(z + 16 * k) * stride);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) { s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w; }
+        }
+        for (; z < splits; z += 16) {
+            const float4 v = *reinterpret_cast<const float4*>(src + (long)z * stride);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+    }
+    sh[g][lane] = s;
+    __syncthreads();
+    if (g != 0) return;
+    for (int k = 1; k < 16; ++k) { const float4 v = sh[k][lane]; s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; }
+    const float r[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (i + e < nk) dw[i + e] = r[e];
+        else if (db && i + e < total) db[i + e - nk] = r[e];
     }
 }
 
@@ -1311,15 +1343,23 @@ int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* co
 }
 
 #ifndef MGN_F16
+static size_t wgrad_floats(int N, int K) { return ((size_t)N * K + N + 3) & ~(size_t)3; }
+// Row ranges: the power of two that minimises (steps a CU goes through) + (writing and reading the partial results), with the step at
+// 0.5 us and the traffic at 5 TB/s, both as measured.  262144 x 256 x 256: 128; 16384 x 256 x 512: 32.
 static int wgrad_splits(long M, int N, int K) {
-    const long tiles = (long)nblocks(N) * nblocks(K);
-    long z = 512 / tiles, most = (M + 4 * WG_ROWS - 1) / (4 * WG_ROWS);   // two blocks a CU, at least four steps a block
-    z = z < 1 ? 1 : z;
-    return (int)(z < most ? z : most);
+    const double tiles = (double)nblocks(N) * nblocks(K), bytes = 8.0 * (double)wgrad_floats(N, K);
+    double best = 1e300;
+    int z = 1;
+    for (int c = 1; c <= 512 && (c == 1 || (long)c * WG_ROWS <= M * 2); c *= 2) {
+        const double steps = (double)((M + (long)c * WG_ROWS - 1) / ((long)c * WG_ROWS)), rounds = (double)((long)((tiles * c + 511) / 512));
+        const double t = steps * rounds * 0.5 + c * bytes / 5e6;
+        if (t < best) { best = t; z = c; }
+    }
+    return z;
 }
 int mgn_q8_wgrad_workspace_bytes(long M, int N, int K, size_t* bytes) {
     if (M < 1 || M > MAX_ROWS || N < 1 || K < 1 || N > 65536 || K > 65536 || !bytes) return MGN_EINVAL;
-    *bytes = sizeof(float) * (size_t)(wgrad_splits(M, N, K) + 1) * ((size_t)N * K + N);
+    *bytes = sizeof(float) * (size_t)wgrad_splits(M, N, K) * wgrad_floats(N, K);
     return MGN_OK;
 }
 #endif
@@ -1331,19 +1371,25 @@ int MGN_SYM(mgn_q8_wgrad)(const void* dy, long ldy, long M, int N, const void* c
     if (rc != MGN_OK) return rc;
     if (!dy || !codes || !scales || !dw || !ws || !aligned(dy, 16) || !aligned(codes, 16) || ldy < N || ldy % 8 != 0 || ldy > 65536) return MGN_EINVAL;
     if (ws_bytes < need) return MGN_ENOSPC;
-    const size_t one = sizeof(float) * ((size_t)N * K + N);
-    const int zmax = (int)(need / one) - 1;
+    const int zmax = (int)(need / (sizeof(float) * (((size_t)N * K + N + 3) & ~(size_t)3)));
     // rows per split: whole steps, and a range whose bytes stay inside a 32-bit buffer descriptor
     long rows = ((M + zmax - 1) / zmax + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
-    if (rows * ldy * 2 > 0x7fffffffL) return MGN_EINVAL;
+    if ((rows + 4 * WG_ROWS) * (ldy * 2 > code_ld(K) ? ldy * 2 : code_ld(K)) > 0x7fffffffL) return MGN_EINVAL;   // (offsets run up to four steps past the range)
     WgradParams8 p = {(const uint16_t*)dy, (const unsigned char*)codes, (const unsigned char*)scales, (float*)ws, (int)M, N, K, (int)ldy, code_ld(K),
                       scale_ld(M), (int)rows, (int)((M + rows - 1) / rows), nblocks(N), nblocks(K)};
     const long blocks = (long)((p.splits + 7) / 8) * 8 * p.ntn * p.ntk;
     if (blocks > 0x7fffffffL) return MGN_EINVAL;
     hipStream_t s = (hipStream_t)stream_;
+    static bool ready[64] = {};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MGN_ELAUNCH;
+    if (!ready[dev]) {
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(q8_wgrad), hipFuncAttributeMaxDynamicSharedMemorySize, WG_LDS) != hipSuccess) return MGN_ELAUNCH;
+        ready[dev] = true;
+    }
     hipLaunchKernelGGL(q8_wgrad, dim3((unsigned)blocks), dim3(TPB), WG_LDS, s, p);
     const long nk = (long)N * K, total = nk + N;
-    hipLaunchKernelGGL(q8_wgrad_reduce, dim3((unsigned)((total + 15) / 16)), dim3(TPB), 0, s, (const float*)ws, p.splits, total, nk, dw, db);
+    hipLaunchKernelGGL(q8_wgrad_reduce, dim3((unsigned)((total + 255) / 256)), dim3(1024), 0, s, (const float*)ws, p.splits, total, nk, dw, db);
     return done();
 }
 
