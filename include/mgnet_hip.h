@@ -823,6 +823,14 @@ int mgn_q8_pack_matmul(const void* x, long M, int K, long ldx, void* codes, void
 int mgn_q8_wgrad_workspace_bytes(long M, int N, int K, size_t* bytes);
 int mgn_q8_wgrad(const void* dy, long ldy, long M, int N, const void* codes, const void* scales, int K, float* dw, float* db, void* workspace,
                  size_t workspace_bytes, void* stream);
+/* The trained 1x1 convolution in one call each way.  x: as mgn_q8_pack (16-bit); w [N][C] with strides w_sr, w_sc (dtype as there); y, dy, dx:
+ * contiguous rows, 16-byte aligned.  `buffer` (mgn_q8_conv1x1_bytes, 16-byte aligned) holds the packed x (unless keep = 0), the packed
+ * weights and their transpose; the backward call reads it.  dx, dw [N][C], db [N] may be NULL (db only with dw). */
+int mgn_q8_conv1x1_bytes(long M, int C, int N, size_t* buffer, size_t* scratch);
+int mgn_q8_conv1x1_fwd(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, const void* w, int w_dtype, long w_sr, long w_sc, int N,
+                       const float* bias, int relu, void* y, int keep, void* buffer, size_t buffer_bytes, void* stream);
+int mgn_q8_conv1x1_bwd(const void* dy, long M, int C, int N, const void* buffer, void* dx, float* dw, float* db, void* scratch, size_t scratch_bytes,
+                       void* stream);
 /* Block tail y = relu(norm(x) + shortcut) (res_net.py:62-79) that keeps x in 8 bits for its backward pass.  All maps [M, C] channels-last,
  * 16-bit, 16-byte aligned, C % 8 == 0, C <= 8192.
  *   stats      : partials[rows][C][2] (rows = mgn_q8_tail_partial_rows) of (x - shift), (x - shift)^2 and shift[C] = x's first row, the
@@ -841,6 +849,14 @@ int mgn_q8_tail_bwd_reduce(const void* codes, const void* scales, const void* g,
 int mgn_q8_tail_sums(const float* partials, int rows, int C, const float* rstd, const float* weight, float* sums, float* dwb, void* stream);
 int mgn_q8_tail_bwd_apply(const void* codes, const void* scales, const void* dz, const float* weight, const float* mean, const float* rstd,
                           const float* sums, float total_count, float eps, long M, int C, void* dx, void* stream);
+/* one process: stats + mgn_iabn_coeffs_from_partials (coef [4][C], running statistics) + fwd, and bwd_reduce + bwd_apply (dx nullable;
+ * sums_dwb [4][C] = sums, d weight, d bias), in one call each; workspace from mgn_q8_tail_workspace_bytes */
+int mgn_q8_tail_workspace_bytes(long M, int C, size_t* bytes);
+int mgn_q8_tail_train_fwd(const void* x, const void* shortcut, long M, int C, const float* weight, const float* bias, float eps, float momentum,
+                          float* running_mean, float* running_var, float* coef, void* y, void* codes, void* scales, void* relu_bits, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int mgn_q8_tail_train_bwd(const void* codes, const void* scales, const void* g, const void* relu_bits, const float* coef, const float* weight, float eps,
+                          long M, int C, void* dz, void* dx, float* sums_dwb, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * IEEE fp16 activations -- the reference's AMP format (configs/MGNet-*.yaml SOLVER.AMP.ENABLED -> torch.cuda.amp: fp16 +
@@ -958,6 +974,15 @@ int mgn_q8_tail_bwd_reduce_f16(const void* codes, const void* scales, const void
     const float* weight, long M, int C, void* dz, float* partials, float* sums, float* dwb, void* stream);
 int mgn_q8_tail_bwd_apply_f16(const void* codes, const void* scales, const void* dz, const float* weight, const float* mean, const float* rstd, const
     float* sums, float total_count, float eps, long M, int C, void* dx, void* stream);
+int mgn_q8_conv1x1_fwd_f16(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, const void* w, int w_dtype, long w_sr, long w_sc,
+    int N, const float* bias, int relu, void* y, int keep, void* buffer, size_t buffer_bytes, void* stream);
+int mgn_q8_conv1x1_bwd_f16(const void* dy, long M, int C, int N, const void* buffer, void* dx, float* dw, float* db, void* scratch, size_t
+    scratch_bytes, void* stream);
+int mgn_q8_tail_train_fwd_f16(const void* x, const void* shortcut, long M, int C, const float* weight, const float* bias, float eps, float momentum,
+    float* running_mean, float* running_var, float* coef, void* y, void* codes, void* scales, void* relu_bits, void* workspace, size_t
+    workspace_bytes, void* stream);
+int mgn_q8_tail_train_bwd_f16(const void* codes, const void* scales, const void* g, const void* relu_bits, const float* coef, const float* weight,
+    float eps, long M, int C, void* dz, void* dx, float* sums_dwb, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

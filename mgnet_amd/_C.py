@@ -32,8 +32,9 @@ SYMBOLS = ["mgn_version", "mgn_reproj_workspace_bytes", "mgn_reproj_loss_fwd", "
            "mgn_plan_compile", "mgn_plan_set_stream", "mgn_plan_run", "mgn_plan_prof_elapsed", "mgn_plan_free",
            "mgn_plan_trace", "mgn_plan_trace_read", "mgn_plan_set_skip", "mgn_plan_node_ro", "mgn_plan_node_ro_family", "mgn_plan_set_jitter", "mgn_plan_probe",
            "mgn_abn_apply_pool", "mgn_att_abn_bwd_stats", "mgn_att_abn_bwd_sums", "mgn_att_abn_bwd_apply",
-           "mgn_q8_bytes", "mgn_q8_pack", "mgn_q8_unpack", "mgn_q8_pack_weight", "mgn_q8_matmul", "mgn_q8_pack_matmul", "mgn_q8_wgrad_workspace_bytes", "mgn_q8_wgrad", "mgn_q8_tail_partial_rows", "mgn_q8_tail_stats", "mgn_q8_tail_fwd", "mgn_q8_tail_bwd_reduce", "mgn_q8_tail_sums", "mgn_q8_tail_bwd_apply"]
-SYMBOLS_F16 = [n + "_f16" for n in ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_pack_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply']]
+           "mgn_q8_bytes", "mgn_q8_pack", "mgn_q8_unpack", "mgn_q8_pack_weight", "mgn_q8_matmul", "mgn_q8_pack_matmul", "mgn_q8_wgrad_workspace_bytes", "mgn_q8_wgrad", "mgn_q8_tail_partial_rows", "mgn_q8_tail_stats", "mgn_q8_tail_fwd", "mgn_q8_tail_bwd_reduce", "mgn_q8_tail_sums", "mgn_q8_tail_bwd_apply",
+           "mgn_q8_conv1x1_bytes", "mgn_q8_conv1x1_fwd", "mgn_q8_conv1x1_bwd", "mgn_q8_tail_workspace_bytes", "mgn_q8_tail_train_fwd", "mgn_q8_tail_train_bwd"]
+SYMBOLS_F16 = [n + "_f16" for n in ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_pack_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply', 'mgn_q8_conv1x1_fwd', 'mgn_q8_conv1x1_bwd', 'mgn_q8_tail_train_fwd', 'mgn_q8_tail_train_bwd']]
 DEPTH_MAX_FILTER_IDS = 16
 MGN_MAX_TASKS = 8   # include/mgnet_hip.h
 
@@ -86,7 +87,7 @@ def plan_touch(reads=(), writes=()):
 
 
 H16 = (torch.bfloat16, torch.float16)   # the 16-bit activation formats: bf16 entry points, or their _f16 twins (csrc/h16.h)
-F16_TWINS = ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_pack_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply']
+F16_TWINS = ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_pack_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply', 'mgn_q8_conv1x1_fwd', 'mgn_q8_conv1x1_bwd', 'mgn_q8_tail_train_fwd', 'mgn_q8_tail_train_bwd']
 
 
 def _fn(name, t):
@@ -252,6 +253,12 @@ def lib():
         L.mgn_q8_tail_bwd_reduce.argtypes = [vp, vp, vp, vp, vp, vp, vp, cl, ci, vp, vp, vp, vp, vp]
         L.mgn_q8_tail_sums.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
         L.mgn_q8_tail_bwd_apply.argtypes = [vp, vp, vp, vp, vp, vp, vp, cf, cf, cl, ci, vp, vp]
+        L.mgn_q8_conv1x1_bytes.argtypes = [cl, ci, ci, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        L.mgn_q8_conv1x1_fwd.argtypes = [vp, cl, ci, cl, cl, cl, ci, ci, vp, ci, cl, cl, ci, vp, ci, vp, ci, vp, sz, vp]
+        L.mgn_q8_conv1x1_bwd.argtypes = [vp, cl, ci, ci, vp, vp, vp, vp, vp, sz, vp]
+        L.mgn_q8_tail_workspace_bytes.argtypes = [cl, ci, ctypes.POINTER(sz)]
+        L.mgn_q8_tail_train_fwd.argtypes = [vp, vp, cl, ci, vp, vp, cf, cf, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        L.mgn_q8_tail_train_bwd.argtypes = [vp, vp, vp, vp, vp, vp, cf, cl, ci, vp, vp, vp, vp, sz, vp]
         for n in SYMBOLS[4:]:
             getattr(L, n).restype = ci
         L.mgn_p2p_mailbox_bytes.restype = sz
@@ -1621,110 +1628,141 @@ def project_bwd(points, A, t, g):
 
 
 # ---------------------------------------------------------------------------------------------------------------
-# 8-bit codes with a power-of-two scale per block of 128 (csrc/q8.hip; ops.Q8Map)
+# 8-bit codes with a power-of-two scale per block of 128 (csrc/q8.hip; modeling/q8.py).  A packed [M, C] matrix is one buffer: codes
+# [M, C rounded up to 16], then scales [ceil(C / 128), M rounded up to 16]
 # ---------------------------------------------------------------------------------------------------------------
-def q8_alloc(M, C, device):
-    """empty (codes [M, ldc], scales [ceil(C/128), lds]) of an [M, C] matrix"""
-    return (torch.empty((M, (C + 15) // 16 * 16), dtype=torch.uint8, device=device),
-            torch.empty(((C + 127) // 128, (M + 15) // 16 * 16), dtype=torch.uint8, device=device))
+def q8_code_bytes(M, C):
+    return M * ((C + 15) & ~15)
+
+
+def q8_bytes(M, C):
+    return M * ((C + 15) & ~15) + (C + 127) // 128 * ((M + 15) & ~15)
 
 
 def q8_pack(x, M, C, sn, sh, sw, H, W):
-    """row (n, h, w) of x (element strides sn, sh, sw; unit channel stride) -> codes, scales"""
-    codes, scales = q8_alloc(M, C, x.device)
-    check(_fn("mgn_q8_pack", x)(x.data_ptr(), _act_dtype(x), M, C, sn, sh, sw, H, W, codes.data_ptr(), scales.data_ptr(), _stream()), "mgn_q8_pack")
-    return codes, scales
+    """row (n, h, w) of x (element strides sn, sh, sw; unit channel stride) -> packed buffer"""
+    buf = torch.empty(q8_bytes(M, C), dtype=torch.uint8, device=x.device)
+    p = buf.data_ptr()
+    check(_fn("mgn_q8_pack", x)(x.data_ptr(), _act_dtype(x), M, C, sn, sh, sw, H, W, p, p + q8_code_bytes(M, C), _stream()), "mgn_q8_pack")
+    return buf
 
 
-def q8_unpack(codes, scales, M, C, out):
-    check(_fn("mgn_q8_unpack", out)(codes.data_ptr(), scales.data_ptr(), M, C, out.data_ptr(), _act_dtype(out), _stream()), "mgn_q8_unpack")
+def q8_unpack(buf, M, C, out):
+    p = buf.data_ptr()
+    check(_fn("mgn_q8_unpack", out)(p, p + q8_code_bytes(M, C), M, C, out.data_ptr(), _act_dtype(out), _stream()), "mgn_q8_unpack")
     return out
 
 
-def q8_pack_weight(w, plain=True, transposed=False):
-    """w [N, K] (any strides) -> (codes, scales) of w and / or of its transpose, scales per 128 x 128 tile"""
+def q8_pack_weight(w, transposed=False):
+    """w [N, K] (any strides) -> packed buffer with scales per 128 x 128 tile, of w or of its transpose [K, N] (the same values)"""
     N, K = w.shape
-    a = q8_alloc(N, K, w.device) if plain else (None, None)
-    t = q8_alloc(K, N, w.device) if transposed else (None, None)
-    p = lambda z: None if z is None else z.data_ptr()
-    check(_fn("mgn_q8_pack_weight", w)(w.data_ptr(), _act_dtype(w), w.stride(0), w.stride(1), N, K, p(a[0]), p(a[1]), p(t[0]), p(t[1]), _stream()),
-          "mgn_q8_pack_weight")
-    return a, t
+    M, C = (K, N) if transposed else (N, K)
+    buf = torch.empty(q8_bytes(M, C), dtype=torch.uint8, device=w.device)
+    p = buf.data_ptr()
+    pair = (p, p + q8_code_bytes(M, C))
+    check(_fn("mgn_q8_pack_weight", w)(w.data_ptr(), _act_dtype(w), w.stride(0), w.stride(1), N, K, *((None, None) + pair if transposed else pair + (None, None)),
+                                       _stream()), "mgn_q8_pack_weight")
+    return buf
 
 
-def q8_matmul(a, a_scales, M, b, b_scales, N, K, bias, act, slope, out):
-    """out [M, N] (rows out.stride(0) apart) = act(a b^T + bias)"""
-    check(_fn("mgn_q8_matmul", out)(a.data_ptr(), a_scales.data_ptr(), M, b.data_ptr(), b_scales.data_ptr(), N, K,
-                                    None if bias is None else bias.data_ptr(), act, float(slope), out.data_ptr(), int(out.dtype == torch.float32),
-                                    out.stride(0), _stream()), "mgn_q8_matmul")
+def q8_matmul(a, M, b, N, K, bias, act, slope, out):
+    """out [M, N] contiguous = act(a b^T + bias), a [M, K] and b [N, K] packed"""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    check(_fn("mgn_q8_matmul", out)(pa, pa + q8_code_bytes(M, K), M, pb, pb + q8_code_bytes(N, K), N, K, None if bias is None else bias.data_ptr(), act, slope,
+                                    out.data_ptr(), int(out.dtype == torch.float32), N, _stream()), "mgn_q8_matmul")
     return out
 
 
-def q8_pack_matmul(x, M, K, ldx, keep, b, b_scales, N, bias, act, slope, out):
-    """out = act(q(x) b^T + bias) in one pass over the 16-bit rows x -> (codes, scales) of x, or (None, None) unless `keep`; None where the
-    one-pass kernel does not take the shape (pack first then)"""
-    codes, scales = q8_alloc(M, K, out.device) if keep else (None, None)
+_Q8_SIZES = {}
+
+
+def _q8_conv_sizes(M, C, N):
+    r = _Q8_SIZES.get((M, C, N))
+    if r is None:
+        a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        check(lib().mgn_q8_conv1x1_bytes(M, C, N, ctypes.byref(a), ctypes.byref(b)), "mgn_q8_conv1x1_bytes")
+        if len(_Q8_SIZES) > 4096:
+            _Q8_SIZES.clear()
+        r = _Q8_SIZES[(M, C, N)] = (a.value, b.value)
+    return r
+
+
+def q8_conv1x1_fwd(x, M, C, sn, sh, sw, H, W, w, N, bias, relu, y, keep):
+    """y [M, N] = q(x) q(w)^T + bias [-> ReLU] -> the buffer q8_conv1x1_bwd reads"""
+    nb = _q8_conv_sizes(M, C, N)[0]
+    buf = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    check(_fn("mgn_q8_conv1x1_fwd", x)(x.data_ptr(), M, C, sn, sh, sw, H, W, w.data_ptr(), _act_dtype(w), w.stride(0), w.stride(1), N,
+                                       None if bias is None else bias.data_ptr(), relu, y.data_ptr(), keep, buf.data_ptr(), nb, _stream()), "mgn_q8_conv1x1_fwd")
+    return buf
+
+
+def q8_conv1x1_bwd(dy, M, C, N, buf, dx, dw, db):
+    nb = _q8_conv_sizes(M, C, N)[1]
+    ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
     p = lambda t: None if t is None else t.data_ptr()
-    rc = _fn("mgn_q8_pack_matmul", x)(x.data_ptr(), M, K, ldx, p(codes), p(scales), b.data_ptr(), b_scales.data_ptr(), N, p(bias), act, float(slope),
-                                      out.data_ptr(), int(out.dtype == torch.float32), out.stride(0), _stream())
-    if rc == -95:
-        return None
-    check(rc, "mgn_q8_pack_matmul")
-    return codes, scales
+    check(_fn("mgn_q8_conv1x1_bwd", dy)(dy.data_ptr(), M, C, N, buf.data_ptr(), p(dx), p(dw), p(db), ws.data_ptr(), nb, _stream()), "mgn_q8_conv1x1_bwd")
 
 
-def q8_wgrad(dy, ldy, M, N, codes, scales, K, want_db=True):
-    """dy: 16-bit rows of ldy elements -> dw [N, K], db [N] (or None), fp32"""
-    dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
-    db = torch.empty(N, dtype=torch.float32, device=dy.device) if want_db else None
-    nb = ctypes.c_size_t(0)
-    check(lib().mgn_q8_wgrad_workspace_bytes(M, N, K, ctypes.byref(nb)), "mgn_q8_wgrad_workspace_bytes")
-    ws = torch.empty(nb.value, dtype=torch.uint8, device=dy.device)
-    check(_fn("mgn_q8_wgrad", dy)(dy.data_ptr(), ldy, M, N, codes.data_ptr(), scales.data_ptr(), K, dw.data_ptr(), None if db is None else db.data_ptr(),
-                                  ws.data_ptr(), nb.value, _stream()), "mgn_q8_wgrad")
-    return dw, db
-
-
-def _q8_tail_partials(M, C, device):
-    rows = ctypes.c_int(0)
-    check(lib().mgn_q8_tail_partial_rows(M, C, ctypes.byref(rows)), "mgn_q8_tail_partial_rows")
-    return torch.empty((rows.value, C, 2), dtype=torch.float32, device=device)
+def _q8_tail_ws(M, C, device):
+    r = _Q8_SIZES.get((M, C))
+    if r is None:
+        a = ctypes.c_size_t(0)
+        check(lib().mgn_q8_tail_workspace_bytes(M, C, ctypes.byref(a)), "mgn_q8_tail_workspace_bytes")
+        r = _Q8_SIZES[(M, C)] = a.value
+    return torch.empty(r // 4, dtype=torch.float32, device=device)
 
 
 def q8_tail_stats(x, M, C):
     """(partials, shift) of the batch statistics of x [M, C], the arguments of iabn_from_partials"""
-    part = _q8_tail_partials(M, C, x.device)
-    shift = torch.empty(C, dtype=torch.float32, device=x.device)
+    ws = _q8_tail_ws(M, C, x.device)
+    part, shift = ws[:-C].view(-1, C, 2), ws[-C:]
     check(_fn("mgn_q8_tail_stats", x)(x.data_ptr(), M, C, part.data_ptr(), shift.data_ptr(), _stream()), "mgn_q8_tail_stats")
     return part, shift
 
 
-def q8_tail_fwd(x, shortcut, coef, M, C, keep):
-    """relu(coef[0] * x + coef[1] + shortcut); keep: also (codes, scales) of x and the ReLU mask -> (y, codes, scales, bits)"""
-    y = torch.empty_like(x)
-    codes = scales = bits = None
-    if keep:
-        codes, scales = q8_alloc(M, C, x.device)
-        bits = torch.empty(M * C // 8, dtype=torch.uint8, device=x.device)
-    p = lambda t: None if t is None else t.data_ptr()
-    check(_fn("mgn_q8_tail_fwd", x)(x.data_ptr(), shortcut.data_ptr(), coef[0].data_ptr(), coef[1].data_ptr(), M, C, y.data_ptr(), p(codes), p(scales),
-                                    p(bits), _stream()), "mgn_q8_tail_fwd")
-    return y, codes, scales, bits
+def q8_tail_buffer(M, C, device):
+    """what the tail keeps of x [M, C]: codes, scales, ReLU mask (one bit a value)"""
+    return torch.empty(q8_bytes(M, C) + M * C // 8, dtype=torch.uint8, device=device)
 
 
-def q8_tail_bwd_reduce(codes, scales, g, bits, coef, weight, M, C):
-    """-> (dz, sums [2, C], d_weight, d_bias)"""
-    dz = torch.empty_like(g)
-    part = _q8_tail_partials(M, C, g.device)
+def q8_tail_fwd(x, shortcut, coef, M, C, y, buf):
+    """y = relu(coef[0] * x + coef[1] + shortcut); buf (q8_tail_buffer, or None): x and the ReLU mask for the backward pass"""
+    p, c = None if buf is None else buf.data_ptr(), coef.data_ptr()
+    kept = (None, None, None) if p is None else (p, p + q8_code_bytes(M, C), p + q8_bytes(M, C))
+    check(_fn("mgn_q8_tail_fwd", x)(x.data_ptr(), shortcut.data_ptr(), c, c + 4 * C, M, C, y.data_ptr(), *kept, _stream()), "mgn_q8_tail_fwd")
+
+
+def q8_tail_train_fwd(x, shortcut, M, C, weight, bias, eps, momentum, running_mean, running_var, coef, y, buf):
+    """one process: batch statistics -> coef [4, C] and running statistics -> q8_tail_fwd, in one call"""
+    ws = _q8_tail_ws(M, C, x.device)
+    p = None if buf is None else buf.data_ptr()
+    kept = (None, None, None) if p is None else (p, p + q8_code_bytes(M, C), p + q8_bytes(M, C))
+    check(_fn("mgn_q8_tail_train_fwd", x)(x.data_ptr(), shortcut.data_ptr(), M, C, weight.data_ptr(), bias.data_ptr(), eps, momentum, running_mean.data_ptr(),
+                                          running_var.data_ptr(), coef.data_ptr(), y.data_ptr(), *kept, ws.data_ptr(), ws.numel() * 4, _stream()),
+          "mgn_q8_tail_train_fwd")
+
+
+def q8_tail_bwd_reduce(buf, g, coef, weight, M, C, dz):
+    """dz = g * mask; -> out [4, C]: sums (2 rows), d weight, d bias"""
+    ws = _q8_tail_ws(M, C, g.device)
     out = torch.empty((4, C), dtype=torch.float32, device=g.device)
-    check(_fn("mgn_q8_tail_bwd_reduce", g)(codes.data_ptr(), scales.data_ptr(), g.data_ptr(), bits.data_ptr(), coef[2].data_ptr(), coef[3].data_ptr(),
-                                           weight.data_ptr(), M, C, dz.data_ptr(), part.data_ptr(), out.data_ptr(), out[2].data_ptr(), _stream()),
-          "mgn_q8_tail_bwd_reduce")
-    return dz, out[:2], out[2], out[3]
+    p, c, o = buf.data_ptr(), coef.data_ptr(), out.data_ptr()
+    check(_fn("mgn_q8_tail_bwd_reduce", g)(p, p + q8_code_bytes(M, C), g.data_ptr(), p + q8_bytes(M, C), c + 8 * C, c + 12 * C, weight.data_ptr(), M, C,
+                                           dz.data_ptr(), ws.data_ptr(), o, o + 8 * C, _stream()), "mgn_q8_tail_bwd_reduce")
+    return out
 
 
-def q8_tail_bwd_apply(codes, scales, dz, weight, coef, sums, total_count, eps, M, C):
-    dx = torch.empty_like(dz)
-    check(_fn("mgn_q8_tail_bwd_apply", dz)(codes.data_ptr(), scales.data_ptr(), dz.data_ptr(), weight.data_ptr(), coef[2].data_ptr(), coef[3].data_ptr(),
-                                           sums.data_ptr(), float(total_count), float(eps), M, C, dx.data_ptr(), _stream()), "mgn_q8_tail_bwd_apply")
-    return dx
+def q8_tail_bwd_apply(buf, dz, coef, weight, sums, total_count, eps, M, C, dx):
+    p, c = buf.data_ptr(), coef.data_ptr()
+    check(_fn("mgn_q8_tail_bwd_apply", dz)(p, p + q8_code_bytes(M, C), dz.data_ptr(), weight.data_ptr(), c + 8 * C, c + 12 * C, sums.data_ptr(), float(total_count),
+                                           eps, M, C, dx.data_ptr(), _stream()), "mgn_q8_tail_bwd_apply")
+
+
+def q8_tail_train_bwd(buf, g, coef, weight, eps, M, C, dz, dx):
+    """one process: q8_tail_bwd_reduce and (dx not None) q8_tail_bwd_apply in one call -> out [4, C]"""
+    ws = _q8_tail_ws(M, C, g.device)
+    out = torch.empty((4, C), dtype=torch.float32, device=g.device)
+    p = buf.data_ptr()
+    check(_fn("mgn_q8_tail_train_bwd", g)(p, p + q8_code_bytes(M, C), g.data_ptr(), p + q8_bytes(M, C), coef.data_ptr(), weight.data_ptr(), eps, M, C, dz.data_ptr(),
+                                          None if dx is None else dx.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel() * 4, _stream()), "mgn_q8_tail_train_bwd")
+    return out

@@ -943,6 +943,22 @@ __global__ __launch_bounds__(1024) void q8_wgrad_reduce(const float* __restrict_
     }
 }
 
+// dy rows of N 16-bit values -> rows of ld (a multiple of 8) with zeros behind: what the 16-byte loads of the two gradients want
+__global__ __launch_bounds__(TPB) void q8_pad_rows(const uint16_t* __restrict__ src, long M, int N, int ld, uint4* __restrict__ dst) {
+    const int per = ld / 8;
+    const long i = (long)blockIdx.x * TPB + threadIdx.x;
+    if (i >= M * per) return;
+    const long r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = c + 2 * k < N ? src[r * N + c + 2 * k] : 0, hi = c + 2 * k + 1 < N ? src[r * N + c + 2 * k + 1] : 0;
+        w[k] = lo | (hi << 16);
+    }
+    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // ------------------------------------------------------------------------------------------------------
 // block tail y = relu(norm(x) + shortcut) whose backward pass reads x^ instead of x.  Thread mapping of the four kernels: blockIdx.y = a
 // block of 128 channels, LPB lanes (8 channels each) per row -- a thread's channels never change, so their coefficients stay in
@@ -1393,6 +1409,94 @@ int MGN_SYM(mgn_q8_wgrad)(const void* dy, long ldy, long M, int N, const void* c
     return done();
 }
 
+/* ---- the trained 1x1 convolution in two calls ---- */
+struct ConvBuffer { size_t codes, scales, tcodes, tscales, wcodes, wscales, total; };   // offsets; every piece is a multiple of 16 bytes
+static ConvBuffer conv_buffer(long M, int C, int N) {
+    ConvBuffer b;
+    b.codes = 0;
+    b.scales = b.codes + (size_t)M * code_ld(C);
+    b.tcodes = b.scales + (size_t)nblocks(C) * scale_ld(M);
+    b.tscales = b.tcodes + (size_t)C * code_ld(N);
+    b.wcodes = b.tscales + (size_t)nblocks(N) * scale_ld(C);
+    b.wscales = b.wcodes + (size_t)N * code_ld(C);
+    b.total = b.wscales + (size_t)nblocks(C) * scale_ld(N);
+    return b;
+}
+static bool conv_shape(long M, int C, int N) { return M >= 0 && M <= MAX_ROWS && C >= 1 && C <= 65536 && N >= 1 && N <= 65536; }
+static int pad8(int n) { return (n + 7) & ~7; }
+// what the backward call needs: [dy padded][dy packed, where the product does not pack it on the fly][partial weight gradients]
+struct ConvScratch { size_t pad, codes, scales, part, total; };
+static ConvScratch conv_scratch(long M, int C, int N, size_t part_bytes) {
+    ConvScratch b;
+    b.pad = 0;
+    b.codes = N % 8 ? (size_t)M * pad8(N) * 2 : 0;
+    b.scales = b.codes + (size_t)M * code_ld(N);
+    b.part = b.scales + (size_t)nblocks(N) * scale_ld(M);
+    b.total = b.part + part_bytes;
+    return b;
+}
+
+#ifndef MGN_F16
+int mgn_q8_conv1x1_bytes(long M, int C, int N, size_t* buffer, size_t* scratch) {
+    if (!conv_shape(M, C, N) || !buffer || !scratch) return MGN_EINVAL;
+    *buffer = conv_buffer(M, C, N).total;
+    size_t part = 0;
+    if (M > 0) { const int rc = mgn_q8_wgrad_workspace_bytes(M, N, C, &part); if (rc != MGN_OK) return rc; }
+    *scratch = conv_scratch(M, C, N, part).total;
+    return MGN_OK;
+}
+#endif
+
+int MGN_SYM(mgn_q8_conv1x1_fwd)(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, const void* w, int w_dtype, long w_sr, long w_sc,
+                                int N, const float* bias, int relu, void* y, int keep, void* buffer, size_t buffer_bytes, void* stream_) {
+    if (!conv_shape(M, C, N) || !w || (!y && M > 0) || !buffer || !aligned(buffer, 16)) return MGN_EINVAL;
+    const ConvBuffer b = conv_buffer(M, C, N);
+    if (buffer_bytes < b.total) return MGN_ENOSPC;
+    unsigned char* p = (unsigned char*)buffer;
+    int rc = MGN_SYM(mgn_q8_pack_weight)(w, w_dtype, w_sr, w_sc, N, C, p + b.wcodes, p + b.wscales, p + b.tcodes, p + b.tscales, stream_);
+    if (rc != MGN_OK || M == 0) return rc;
+    const long images = H < 1 || W < 1 ? 0 : M / ((long)H * W);
+    const bool flat = (W == 1 || sw == C) && (H == 1 || sh == (long)W * C) && (images == 1 || sn == (long)H * W * C);
+    rc = MGN_ENOTSUP;
+    if (flat) rc = MGN_SYM(mgn_q8_pack_matmul)(x, M, C, C, keep ? p + b.codes : nullptr, keep ? p + b.scales : nullptr, p + b.wcodes, p + b.wscales, N, bias,
+                                               relu ? 1 : 0, 0.f, y, 0, N, stream_);
+    if (rc != MGN_ENOTSUP) return rc;
+    rc = MGN_SYM(mgn_q8_pack)(x, 1, M, C, sn, sh, sw, H, W, p + b.codes, p + b.scales, stream_);
+    if (rc != MGN_OK) return rc;
+    return MGN_SYM(mgn_q8_matmul)(p + b.codes, p + b.scales, M, p + b.wcodes, p + b.wscales, N, C, bias, relu ? 1 : 0, 0.f, y, 0, N, stream_);
+}
+
+int MGN_SYM(mgn_q8_conv1x1_bwd)(const void* dy, long M, int C, int N, const void* buffer, void* dx, float* dw, float* db, void* scratch,
+                                size_t scratch_bytes, void* stream_) {
+    size_t need = 0, have = 0, part = 0;
+    int rc = mgn_q8_conv1x1_bytes(M, C, N, &have, &need);
+    if (rc != MGN_OK) return rc;
+    if (M < 1 || !dy || !buffer || !scratch || (!dx && !dw) || (db && !dw) || !aligned(dy, 16) || !aligned(buffer, 16) || !aligned(scratch, 16)) return MGN_EINVAL;
+    if (scratch_bytes < need) return MGN_ENOSPC;
+    mgn_q8_wgrad_workspace_bytes(M, N, C, &part);
+    const ConvBuffer b = conv_buffer(M, C, N);
+    const ConvScratch t = conv_scratch(M, C, N, part);
+    const unsigned char* p = (const unsigned char*)buffer;
+    unsigned char* s = (unsigned char*)scratch;
+    const int ldy = pad8(N);
+    if (N % 8) {
+        const long blocks = (M * (ldy / 8) + TPB - 1) / TPB;
+        if (blocks > 0x7fffffffL) return MGN_EINVAL;
+        hipLaunchKernelGGL(q8_pad_rows, dim3((unsigned)blocks), dim3(TPB), 0, (hipStream_t)stream_, (const uint16_t*)dy, M, N, ldy, (uint4*)(s + t.pad));
+        dy = s + t.pad;
+    }
+    if (dx) {   // (K = N padded: the columns behind N are zeros on both sides)
+        rc = MGN_SYM(mgn_q8_pack_matmul)(dy, M, ldy, ldy, nullptr, nullptr, p + b.tcodes, p + b.tscales, C, nullptr, 0, 0.f, dx, 0, C, stream_);
+        if (rc == MGN_ENOTSUP) {
+            rc = MGN_SYM(mgn_q8_pack)(dy, 1, M, N, ldy, 0, 0, 1, 1, s + t.codes, s + t.scales, stream_);
+            if (rc == MGN_OK) rc = MGN_SYM(mgn_q8_matmul)(s + t.codes, s + t.scales, M, p + b.tcodes, p + b.tscales, C, N, nullptr, 0, 0.f, dx, 0, C, stream_);
+        }
+        if (rc != MGN_OK) return rc;
+    }
+    if (dw) return MGN_SYM(mgn_q8_wgrad)(dy, ldy, M, N, p + b.codes, p + b.scales, C, dw, db, s + t.part, part, stream_);
+    return MGN_OK;
+}
+
 /* ---- block tail ---- */
 static int tail_shape(long M, int C) { return (M < 1 || M > MAX_ROWS || C < 8 || C % 8 != 0 || C > 8192) ? MGN_EINVAL : MGN_OK; }
 static unsigned tail_rows(long M, int C) {   // row blocks of the reductions: 16 rows a thread before there are more blocks than fill the chip
@@ -1461,6 +1565,44 @@ int MGN_SYM(mgn_q8_tail_bwd_apply)(const void* codes, const void* scales, const 
                                     (const unsigned char*)scales, (const uint16_t*)dz, weight, mean, rstd, sums, 1.f / total_count, eps, (int)M, C,
                                     code_ld(C), scale_ld(M), (uint16_t*)dx)));
     return done();
+}
+
+#ifndef MGN_F16
+int mgn_q8_tail_workspace_bytes(long M, int C, size_t* bytes) {
+    if (tail_shape(M, C) != MGN_OK || !bytes) return MGN_EINVAL;
+    *bytes = sizeof(float) * ((size_t)tail_rows(M, C) * C * 2 + C);
+    return MGN_OK;
+}
+#endif
+
+int MGN_SYM(mgn_q8_tail_train_fwd)(const void* x, const void* shortcut, long M, int C, const float* weight, const float* bias, float eps, float momentum,
+                                   float* running_mean, float* running_var, float* coef, void* y, void* codes, void* scales, void* relu_bits, void* ws,
+                                   size_t ws_bytes, void* stream_) {
+    size_t need = 0;
+    int rc = mgn_q8_tail_workspace_bytes(M, C, &need);
+    if (rc != MGN_OK) return rc;
+    if (!ws || !coef) return MGN_EINVAL;
+    if (ws_bytes < need) return MGN_ENOSPC;
+    const int rows = (int)tail_rows(M, C);
+    float *part = (float*)ws, *shift = part + (size_t)rows * C * 2;
+    rc = MGN_SYM(mgn_q8_tail_stats)(x, M, C, part, shift, stream_);
+    if (rc == MGN_OK) rc = mgn_iabn_coeffs_from_partials(part, rows, C, M, shift, weight, bias, eps, momentum, running_mean, running_var, coef, nullptr, stream_);
+    if (rc == MGN_OK) rc = MGN_SYM(mgn_q8_tail_fwd)(x, shortcut, coef, coef + C, M, C, y, codes, scales, relu_bits, stream_);
+    return rc;
+}
+
+int MGN_SYM(mgn_q8_tail_train_bwd)(const void* codes, const void* scales, const void* g, const void* relu_bits, const float* coef, const float* weight,
+                                   float eps, long M, int C, void* dz, void* dx, float* sums_dwb, void* ws, size_t ws_bytes, void* stream_) {
+    size_t need = 0;
+    int rc = mgn_q8_tail_workspace_bytes(M, C, &need);
+    if (rc != MGN_OK) return rc;
+    if (!ws || !coef || !sums_dwb) return MGN_EINVAL;
+    if (ws_bytes < need) return MGN_ENOSPC;
+    rc = MGN_SYM(mgn_q8_tail_bwd_reduce)(codes, scales, g, relu_bits, coef + 2 * (size_t)C, coef + 3 * (size_t)C, weight, M, C, dz, (float*)ws, sums_dwb,
+                                         sums_dwb + 2 * (size_t)C, stream_);
+    if (rc == MGN_OK && dx) rc = MGN_SYM(mgn_q8_tail_bwd_apply)(codes, scales, dz, weight, coef + 2 * (size_t)C, coef + 3 * (size_t)C, sums_dwb, (float)M, eps, M, C,
+                                                                dx, stream_);
+    return rc;
 }
 
 }  // extern "C"

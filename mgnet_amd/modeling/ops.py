@@ -1312,274 +1312,4 @@ def uncertainty_weighting(losses, log_vars, k0=0):
     return ({k: weighted[i] for i, k in enumerate(keys)}, {k: raw[i].detach() for i, k in enumerate(keys)}, {k: unc[i] for i, k in enumerate(keys)})
 
 
-# ---------------------------------------------------------------------------------------------------------------
-# 8-bit activations and weights: e4m3 codes with one power-of-two scale per block of 128 (csrc/q8.hip)
-# ---------------------------------------------------------------------------------------------------------------
-class Q8Map:
-    """An [M, C] matrix, or the channels-last map [N, C, H, W] with M = N*H*W pixels, in 8 bits: `codes` uint8 [M, C rounded up to 16],
-    `scales` uint8 [ceil(C / 128), M rounded up to 16] (exponent + 127 of block k of row r at [k, r]).  A block is 128 neighbouring channels
-    of a row; with tile=True (weights) all 128 rows of a tile share a scale.  Made by q8_pack; `dtype` is the source's."""
-
-    def __init__(self, codes, scales, shape, dtype):
-        self.codes, self.scales, self.shape, self.dtype = codes, scales, tuple(shape), dtype
-
-    @property
-    def device(self):
-        return self.codes.device
-
-    @property
-    def channels(self):
-        return self.shape[1]
-
-    @property
-    def rows(self):
-        return self.codes.shape[0]
-
-    def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
-
-    def unpack(self, dtype=None):
-        """the values, in the source's type (exact) or `dtype` (rounded once); maps come back channels-last"""
-        from .. import _C
-        dtype = self.dtype if dtype is None else dtype
-        if dtype != torch.float32 and dtype not in _C.H16:
-            raise ValueError(f"Q8Map.unpack: float32, bfloat16 or float16, got {dtype}")
-        with _on(self.codes):
-            if len(self.shape) == 2:
-                out = torch.empty(self.shape, dtype=dtype, device=self.device)
-            else:
-                out = torch.empty(self.shape, dtype=dtype, device=self.device, memory_format=torch.channels_last)
-            return _C.q8_unpack(self.codes, self.scales, self.rows, self.channels, out)
-
-
-def _on(t):
-    """launches go to the tensor's own device, whichever is current"""
-    import contextlib
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _q8_source(x, what):
-    from .. import _C
-    if not isinstance(x, torch.Tensor) or x.dim() not in (2, 4):
-        raise ValueError(f"{what}: an [M, C] matrix or an [N, C, H, W] map, got {tuple(x.shape) if isinstance(x, torch.Tensor) else type(x).__name__}")
-    if not x.is_cuda:
-        raise RuntimeError(f"{what}: the 8-bit operators have HIP kernels only (no CPU form), got a {x.device} tensor")
-    if x.dtype != torch.float32 and x.dtype not in _C.H16:
-        raise ValueError(f"{what}: float32, bfloat16 or float16, got {x.dtype}")
-    if x.shape[1] < 1:
-        raise ValueError(f"{what}: no channels in {tuple(x.shape)}")
-
-
-def _q8_rows(x):
-    """codes, scales of the rows of x (a matrix, or a map's pixels); any strides"""
-    from .. import _C
-    x = x.detach()
-    if x.dim() == 2:
-        M, C = x.shape
-        if x.stride(1) != 1 and C > 1:
-            x = x.contiguous()
-        return _C.q8_pack(x, M, C, x.stride(0), 0, 0, 1, 1)
-    N, C, H, W = x.shape
-    if x.stride(1) != 1 and C > 1:
-        x = x.contiguous(memory_format=torch.channels_last)
-        if x.stride(1) != 1:        # (a map of one pixel an image is contiguous in either order, with any strides)
-            return _C.q8_pack(x, N * H * W, C, C, 0, 0, 1, 1)
-    return _C.q8_pack(x, N * H * W, C, x.stride(0), x.stride(2), x.stride(3), max(H, 1), max(W, 1))
-
-
-def q8_pack(x, tile=False):
-    """x [M, C] or [N, C, H, W], float32 / bfloat16 / float16, any strides -> Q8Map.  value = code * 2^e with the smallest e >= -111 that
-    keeps the block's largest finite magnitude within 448 * 2^e: relative error at most 2^-4 down to 2^-6 * 2^e, absolute 2^-10 * 2^e below;
-    NaN and infinities become NaN.  tile: a weight matrix [N, K], one scale per 128 x 128 tile.  Not differentiable (see conv1x1_q8)."""
-    from .. import _C
-    _q8_source(x, "q8_pack")
-    with _on(x):
-        if tile:
-            if x.dim() != 2 or 0 in x.shape:
-                raise ValueError(f"q8_pack: tile scales are for a weight matrix [N, K], got {tuple(x.shape)}")
-            codes, scales = _C.q8_pack_weight(x.detach())[0]
-        else:
-            codes, scales = _q8_rows(x)
-    return Q8Map(codes, scales, x.shape, x.dtype)
-
-
-_Q8_ACT = {"none": 0, "relu": 1, "leaky_relu": 2}
-
-
-def q8_matmul(a, b, bias=None, act="none", slope=0.01, out_dtype=None):
-    """act(a b^T + bias) of two packed matrices a [M, K] (or a map [N, K, H, W]: the result is the map [N, n, H, W]) and b [n, K]; products
-    of codes scaled in the matrix cores, fp32 accumulation, one rounding to out_dtype (default: a's source type).  act: none | relu |
-    leaky_relu (slope).  No gradient (conv1x1_q8 has one)."""
-    from .. import _C
-    if not (isinstance(a, Q8Map) and isinstance(b, Q8Map)):
-        raise ValueError("q8_matmul: two Q8Map operands (ops.q8_pack)")
-    if len(b.shape) != 2 or a.channels != b.channels:
-        raise ValueError(f"q8_matmul: a [M, K] and b [n, K] with one K, got {a.shape} and {b.shape}")
-    if a.device != b.device or (bias is not None and bias.device != a.device):
-        raise ValueError("q8_matmul: operands on different devices")
-    out_dtype = a.dtype if out_dtype is None else out_dtype
-    if act not in _Q8_ACT or (out_dtype != torch.float32 and out_dtype not in _C.H16):
-        raise ValueError(f"q8_matmul: act one of {sorted(_Q8_ACT)}, a float32 / bfloat16 / float16 result; got {act}, {out_dtype}")
-    n, K, M = b.shape[0], a.channels, a.rows
-    if bias is not None:
-        if tuple(bias.shape) != (n,):
-            raise ValueError(f"q8_matmul: bias [{n}], got {tuple(bias.shape)}")
-        bias = bias.detach().float().contiguous()
-    with _on(a.codes):
-        out = torch.empty((M, n), dtype=out_dtype, device=a.device)
-        _C.q8_matmul(a.codes, a.scales, M, b.codes, b.scales, n, K, bias, _Q8_ACT[act], slope, out)
-    if len(a.shape) == 2:
-        return out
-    N, _, H, W = a.shape
-    return out.view(N, H, W, n).permute(0, 3, 1, 2)
-
-
-def _q8_product(x, keep, wc, ws, n, bias, act, out):
-    """out [M, n] = act(q(x) w^T + bias) for a map or matrix x -> (codes, scales) of x (they may be None unless `keep`)"""
-    from .. import _C
-    C = x.shape[1]
-    if x.is_contiguous(memory_format=torch.channels_last) if x.dim() == 4 else x.is_contiguous():
-        r = _C.q8_pack_matmul(x, out.shape[0], C, C, keep, wc, ws, n, bias, act, 0.0, out)
-        if r is not None:
-            return r
-    codes, scales = _q8_rows(x)
-    _C.q8_matmul(codes, scales, out.shape[0], wc, ws, n, C, bias, act, 0.0, out)
-    return codes, scales
-
-
-class _Conv1x1Q8Fn(torch.autograd.Function):
-    """[HIP] csrc/q8.hip.  What waits for the backward pass is the packed input (1 byte a value instead of 2) and the packed transpose of
-    the weights; the data gradient is the 8-bit product of the packed dy with it, the weight gradient multiplies dy in 16 bits with the
-    exact 16-bit value of the codes."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, relu):
-        from .. import _C
-        N, C, H, W = x.shape
-        Cout, M = weight.shape[0], N * H * W
-        (wc, ws), (tc, ts) = _C.q8_pack_weight(weight.detach().reshape(Cout, C), True, ctx.needs_input_grad[0])
-        b = None if bias is None else bias.detach().float().contiguous()
-        y = torch.empty((N, Cout, H, W), dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
-        keep = ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2])
-        codes, scales = _q8_product(x.detach(), keep, wc, ws, Cout, b, int(relu), y.permute(0, 2, 3, 1).view(M, Cout))
-        ctx.save_for_backward(*((codes, scales) if keep else (None, None)), tc, ts, y if relu else None)
-        ctx.cfg = (x.shape, x.dtype, weight.dtype, tuple(weight.shape), None if bias is None else bias.dtype)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        from .. import _C
-        codes, scales, tc, ts, y = ctx.saved_tensors
-        (N, C, H, W), dtype, wdtype, wshape, bdtype = ctx.cfg
-        Cout, M = wshape[0], N * H * W
-        want_dx, want_dw, want_db = ctx.needs_input_grad[:3]
-        want_db = want_db and bdtype is not None
-        dx = dw = db = None
-        dev = dy.device
-        with _on(dy):
-            if M == 0:
-                return (torch.empty((N, C, H, W), dtype=dtype, device=dev) if want_dx else None,
-                        torch.zeros(wshape, dtype=wdtype, device=dev) if want_dw else None,
-                        torch.zeros(Cout, dtype=bdtype, device=dev) if want_db else None, None)
-            dy = dy.to(dtype).contiguous(memory_format=torch.channels_last)
-            if y is not None:
-                dy = _C.relu_mask_bwd(dy, y) if _C.elt_supported(y) and _C.elt_supported(dy) else dy * (y > 0)
-            rows = dy.permute(0, 2, 3, 1).reshape(M, Cout)     # (a view: dy is channels-last)
-            if want_dx:
-                dx = torch.empty((N, C, H, W), dtype=dtype, device=dev, memory_format=torch.channels_last)
-                _q8_product(rows, False, tc, ts, C, None, 0, dx.permute(0, 2, 3, 1).view(M, C))
-            if want_dw or want_db:
-                ldy = Cout
-                if Cout % 8 or rows.data_ptr() % 16:           # the kernel loads 16-byte pieces of rows
-                    ldy = (Cout + 7) // 8 * 8
-                    padded = torch.empty((M, ldy), dtype=dtype, device=dev)
-                    padded[:, :Cout].copy_(rows)
-                    rows = padded
-                dw, db = _C.q8_wgrad(rows, ldy, M, Cout, codes, scales, C, want_db)
-                dw = dw.view(wshape).to(wdtype) if want_dw else None
-                db = db.to(bdtype) if want_db else None
-        return dx, dw, db, None
-
-
-def conv1x1_q8(x, weight, bias=None, relu=False):
-    """A 1x1 convolution (stride 1) trained in 8 bits: y = q(x) q(W)^T + bias [-> ReLU], dx = q(dy) q(W), dW = dy^T q(x), db = sum dy, with
-    q(.) the block format of q8_pack (x and dy per 128 channels of a pixel, W per 128 x 128 tile), products accumulated in fp32.  Of the
-    input only its packed form is kept for the backward pass.
-    x [N, C, H, W] bfloat16 / float16 (any strides; the result is channels-last), weight [Cout, C, 1, 1], bias [Cout] or None."""
-    from .. import _C
-    _q8_source(x, "conv1x1_q8")
-    if x.dim() != 4 or x.dtype not in _C.H16:
-        raise ValueError(f"conv1x1_q8: a bfloat16 or float16 map [N, C, H, W], got {x.dtype} {tuple(x.shape)}")
-    if weight.dim() != 4 or tuple(weight.shape[1:]) != (x.shape[1], 1, 1) or weight.shape[0] < 1:
-        raise ValueError(f"conv1x1_q8: weights [Cout, {x.shape[1]}, 1, 1], got {tuple(weight.shape)}")
-    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
-        raise ValueError(f"conv1x1_q8: bias [{weight.shape[0]}], got {tuple(bias.shape)}")
-    if weight.device != x.device or (bias is not None and bias.device != x.device):
-        raise ValueError("conv1x1_q8: operands on different devices")
-    if max(x.shape[1], weight.shape[0]) > 65536:
-        raise ValueError("conv1x1_q8: at most 65536 channels")
-    with _on(x):
-        return _Conv1x1Q8Fn.apply(x, weight, bias, bool(relu))
-
-
-class _AbnAddReluQ8Fn(torch.autograd.Function):
-    """[HIP] csrc/q8.hip: the residual block's tail relu(norm(x) + shortcut) as _AbnAddReluFn, with x kept for the backward pass in 8 bits
-    (the norm's x_hat is recomputed from there) and the ReLU mask in one bit a value; y is not kept."""
-
-    @staticmethod
-    def forward(ctx, x, shortcut, weight, bias, running_mean, running_var, training, momentum, eps, group, pstats):
-        from .. import _C
-        N, C, H, W = x.shape
-        M = N * H * W
-        w32, b32 = weight.detach().float().contiguous(), bias.detach().float().contiguous()
-        world = dist.get_world_size(group) if _dist_active(group) else 1
-        if training:
-            coef = _train_coef(x, M, C, w32, b32, eps, momentum, running_mean, running_var, world, group, pstats or _C.q8_tail_stats(x, M, C))
-        else:
-            coef = _C.iabn_eval_coeffs(w32, b32, running_mean, running_var, eps)
-        keep = training and any(ctx.needs_input_grad[:4])
-        y, codes, scales, bits = _C.q8_tail_fwd(x, shortcut, coef, M, C, keep)
-        ctx.save_for_backward(codes, scales, bits, w32, coef)
-        ctx.cfg = (M, C, eps, group, world, training, float(M) * world, weight.dtype, x.dtype)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        from .. import _C
-        codes, scales, bits, w32, coef = ctx.saved_tensors
-        M, C, eps, group, world, training, total, wdtype, dtype = ctx.cfg
-        if not training:
-            raise NotImplementedError("backward through eval-mode InPlaceABNSync is not on the training path")
-        with _on(codes):
-            g = _cl(g, dtype)
-            if g.data_ptr() % 16:
-                g = g.clone(memory_format=torch.channels_last)
-            dz, sums, d_weight, d_bias = _C.q8_tail_bwd_reduce(codes, scales, g, bits, coef, w32, M, C)
-            if world > 1:
-                sums = _allreduce_sums(sums, group)
-            dx = _C.q8_tail_bwd_apply(codes, scales, dz, w32, coef, sums, total, eps, M, C) if ctx.needs_input_grad[0] else None
-        return dx, dz, d_weight.to(wdtype), d_bias.to(wdtype), None, None, None, None, None, None, None
-
-
-def abn_add_relu_q8(x, norm, shortcut):
-    """`relu_(norm(x) + shortcut)` for an identity-activation InPlaceABNSync (abn_add_relu) that keeps x in 8 bits for the backward pass:
-    forward values are those of the 16-bit x (rounded once), the backward pass uses x_hat of the packed x.  x, shortcut [N, C, H, W]
-    bfloat16 or float16, C % 8 == 0; the batch statistics are exchanged over norm.group as in every norm."""
-    from .. import _C
-    _q8_source(x, "abn_add_relu_q8")
-    if x.dim() != 4 or x.dtype not in _C.H16 or x.shape[1] % 8 or x.shape[1] > 8192 or x.numel() == 0:
-        raise ValueError(f"abn_add_relu_q8: a non-empty bfloat16 or float16 map [N, C, H, W] with C % 8 == 0, got {x.dtype} {tuple(x.shape)}")
-    if shortcut.shape != x.shape or shortcut.dtype != x.dtype or shortcut.device != x.device:
-        raise ValueError("abn_add_relu_q8: the shortcut must match x in shape, type and device")
-    if norm.activation != "identity" or norm.num_features != x.shape[1]:
-        raise ValueError(f"abn_add_relu_q8: an identity-activation norm of {x.shape[1]} channels, got {norm.activation}, {norm.num_features}")
-    pstats = _pstats(x)
-
-    def ready(t):    # rows of C contiguous channels, 16-byte aligned
-        t = t.contiguous(memory_format=torch.channels_last)
-        return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.channels_last)
-    with _on(x):
-        return _AbnAddReluQ8Fn.apply(ready(x), ready(shortcut), norm.weight, norm.bias, norm.running_mean, norm.running_var, norm.training, norm.momentum,
-                                     norm.eps, norm.group, pstats)
+from .q8 import Q8Map, abn_add_relu_q8, conv1x1_q8, q8_matmul, q8_pack  # noqa: E402,F401  (8-bit operators: they use the helpers above)

@@ -87,10 +87,7 @@ def check_packed(q, x2, tile=False):
     val, exps = q8_ref(x2, tile)
     M, C = x2.shape
     assert torch.equal(q.scales[:, :M].long(), exps)
-    got = torch.empty((M, C), dtype=F32, device=x2.device)
-    from mgnet_amd import _C
-    _C.q8_unpack(q.codes, q.scales, M, C, got)
-    assert equal(got.double(), val)
+    assert equal(q.unpack(F32).double().permute(*((0, 2, 3, 1) if len(q.shape) == 4 else (0, 1))).reshape(M, C), val)
     assert not bool(q.codes[:, C:].any())       # the padding columns are zero
 
 
@@ -164,10 +161,9 @@ def test_pack_weight_and_its_transpose(N, K, dtype):
     w = rand((N, K), dtype, N + K)
     check_packed(ops().q8_pack(w, tile=True), w, tile=True)
     check_packed(ops().q8_pack(w.t(), tile=True), w.t(), tile=True)
-    (c, s), (ct, st) = _C.q8_pack_weight(w, True, True)
     a, b = torch.empty((N, K), device="cuda"), torch.empty((K, N), device="cuda")
-    _C.q8_unpack(c, s, N, K, a)
-    _C.q8_unpack(ct, st, K, N, b)
+    _C.q8_unpack(_C.q8_pack_weight(w), N, K, a)
+    _C.q8_unpack(_C.q8_pack_weight(w, transposed=True), K, N, b)
     assert torch.equal(a, b.t())
 
 
