@@ -1342,7 +1342,10 @@ int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const vo
         if (rc != MGN_ENOTSUP) return rc;
     }
     if (N <= 32) return launch_mm<128, 32, 4, 1>(q8_mm_128x32, p, s);
-    if (N > 128 && tiles(256, 256) >= 512) return launch_mm<256, 256, 2, 4>(q8_mm_256x256, p, s);
+    // 256 x 256 tiles run at 2.4 PFLOP/s and 128 x 128 tiles at 1.8 where they fill the chip (256 and 512 blocks at a time): the better of the
+    // two rates after the share of idle slots in the last round
+    auto share = [](long t, long slots) { return (double)t / (double)((t + slots - 1) / slots * slots); };
+    if (N > 128 && share(tiles(256, 256), 256) >= 0.75 * share(tiles(128, 128), 512)) return launch_mm<256, 256, 2, 4>(q8_mm_256x256, p, s);
     return launch_mm<128, 128, 2, 2>(q8_mm_128x128, p, s);
 }
 
