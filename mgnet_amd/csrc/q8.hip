@@ -105,6 +105,44 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
     return make_uint4(mgn_pack2(v[0], v[1]), mgn_pack2(v[2], v[3]), mgn_pack2(v[4], v[5]), mgn_pack2(v[6], v[7]));
 }
 
+// one block's share of a lane, eight 16-bit values: scale of the block (LPB lanes) and codes.  The maximum is taken on the 16-bit words
+// (packed), and the conversion divides by the scale itself: a third of the instructions of the general form, which is left for blocks with a
+// NaN, an infinity or a magnitude beyond the last e4m3 multiple (all of the group's lanes go one way)
+#ifdef MGN_F16
+constexpr uint32_t TOPWORD = 0x7b80u;
+#define MGN_CVT_FP8(OLD, W, SC, HI) __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(OLD, __builtin_bit_cast(h16x2, W), SC, HI)
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t word_bits(uint32_t m) { return __float_as_uint(mgn_h2f((uint16_t)m)); }
+#else
+constexpr uint32_t TOPWORD = 0x7f70u;
+#define MGN_CVT_FP8(OLD, W, SC, HI) __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(OLD, __builtin_bit_cast(h16x2, W), SC, HI)
+typedef __bf16 h16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t word_bits(uint32_t m) { return m << 16; }
+#endif
+template <int LPB>
+__device__ __forceinline__ uint2 quantize8(const uint4& q, uint32_t& s) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 a = __builtin_bit_cast(u16x2, q.x & 0x7fff7fffu), b = __builtin_bit_cast(u16x2, q.y & 0x7fff7fffu);
+    const u16x2 c = __builtin_bit_cast(u16x2, q.z & 0x7fff7fffu), d = __builtin_bit_cast(u16x2, q.w & 0x7fff7fffu);
+    const u16x2 t = __builtin_elementwise_max(__builtin_elementwise_max(a, b), __builtin_elementwise_max(c, d));
+    const uint32_t m = group_max<LPB>(t[0] > t[1] ? t[0] : t[1]);
+    if (__builtin_expect(m > TOPWORD, 0)) {
+        float f[8];
+        unpack8(q, f);
+        s = scale_of(group_max<LPB>(amax8(f, TOP16)));
+        return encode8(f, inv_scale(s), TOP16);
+    }
+    s = scale_of(word_bits(m));
+    const float sc = pow2(s);
+    s16x2 lo = {0, 0}, hi = {0, 0};
+    lo = MGN_CVT_FP8(lo, q.x, sc, false);
+    lo = MGN_CVT_FP8(lo, q.y, sc, true);
+    hi = MGN_CVT_FP8(hi, q.z, sc, false);
+    hi = MGN_CVT_FP8(hi, q.w, sc, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
 // ------------------------------------------------------------------------------------------------------
 // x -> codes, scales.  One pass: a group of LPB lanes owns one block of 8 consecutive rows (8 channels a lane), so a block's maximum is
 // four DPP steps and its eight scales leave in one store; the 8 rows are 8 independent 16-byte loads per lane.  Bound by HBM (3 bytes per
@@ -162,9 +200,14 @@ __global__ __launch_bounds__(TPB) void q8_pack(const T* __restrict__ x, RowMap m
         for (int j = 0; j < RPG; ++j) q[j] = (r0 + j < M && c0 < C) ? Src<T>::load(x + row_offset(map, r0 + j) + c0) : Src<T>::zero();
 #pragma unroll
         for (int j = 0; j < RPG; ++j) {
-            float f[8];
-            Src<T>::get(q[j], f);
-            finish(j, f);
+            if constexpr (sizeof(T) == 2) {
+                const uint2 e = quantize8<LPB>(q[j].a, sb[j]);
+                if (r0 + j < M && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = e;
+            } else {
+                float f[8];
+                Src<T>::get(q[j], f);
+                finish(j, f);
+            }
         }
     } else {
 #pragma unroll
@@ -624,10 +667,8 @@ __device__ __forceinline__ void q8_stream_body(const StreamParams& p) {
             if (SRC == 0) {
                 *reinterpret_cast<u32x4*>(st + r * S::PITCH + (((ukb * 8 + ul) ^ S::swz(r)) << 4)) = q[j];
             } else {
-                float f[8];
-                unpack8(make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]), f);
-                const uint32_t s = scale_of(group_max<16>(amax8(f, TOP16)));
-                const uint2 e = encode8(f, inv_scale(s), TOP16);
+                uint32_t s;
+                const uint2 e = quantize8<16>(make_uint4(q[j][0], q[j][1], q[j][2], q[j][3]), s);
                 *reinterpret_cast<uint2*>(st + r * S::PITCH + (((ukb * 8 + (ul >> 1)) ^ S::swz(r)) << 4) + (ul & 1) * 8) = e;
                 if (ul == 0) sc[ukb * S::BM + r] = (unsigned char)s;
                 if (SRC == 2) __builtin_amdgcn_raw_buffer_store_b64(u32x2{e.x, e.y}, rs, coff + j * RSTEP * p.ldc, 0, 0);
@@ -793,30 +834,32 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
                                                      (r < rows && yo[q] != OOB) ? yo[q] + ks * WG_ROWS * p.ldy * 2 : OOB, 0, 0, 0);
         }
     };
-    // codes: thread = (row tid / 4, 32 columns)
-    const int cr = tid >> 2, cc = (tid & 3) * 32, kcol = tk * BLK + cc;
+    // codes: thread = (rows tid / 8 and 32 further, 16 columns); the two 16-byte halves of its x^ leave in an order that alternates with the row,
+    // so that the 16 lanes of two neighbouring rows write every bank once
+    const int cr = tid >> 3, cc = (tid & 7) * 16, kcol = tk * BLK + cc, odd = cr & 1;
     const __amdgpu_buffer_rsrc_t rsX = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.codes + mb * p.ldc), 0, (uint32_t)(rows * p.ldc), 0x00020000);
     const __amdgpu_buffer_rsrc_t rsC = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.scales + (long)tk * p.lds + mb), 0, (uint32_t)rows, 0x00020000);
-    const int xo0 = kcol < p.ldc ? cr * p.ldc + kcol : OOB, xo1 = kcol + 16 < p.ldc ? cr * p.ldc + kcol + 16 : OOB;
-    struct Fetched { u32x4 lo, hi; uint32_t s; };
+    const int xo = kcol < p.ldc ? cr * p.ldc + kcol : OOB;
+    struct Fetched { u32x4 c[2]; uint32_t s[2]; };
     auto fetch = [&](int ks) {
         Fetched f;
-        f.lo = __builtin_amdgcn_raw_buffer_load_b128(rsX, xo0 + ks * WG_ROWS * p.ldc, 0, 0);
-        f.hi = __builtin_amdgcn_raw_buffer_load_b128(rsX, xo1 + ks * WG_ROWS * p.ldc, 0, 0);
-        f.s = __builtin_amdgcn_raw_buffer_load_b8(rsC, cr + ks * WG_ROWS, 0, 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            f.c[h] = __builtin_amdgcn_raw_buffer_load_b128(rsX, xo + (ks * WG_ROWS + 32 * h) * p.ldc, 0, 0);
+            f.s[h] = __builtin_amdgcn_raw_buffer_load_b8(rsC, cr + ks * WG_ROWS + 32 * h, 0, 0);
+        }
         return f;
     };
     auto spread = [&](const Fetched& f, unsigned char* __restrict__ tile) {
-        unsigned char* b = tile + cr * 256;
-        const float s = pow2(f.s);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const u32x4 c = h ? f.hi : f.lo;
-            const uint4 lo = make_uint4(decode2(c[0], s, 0), decode2(c[0], s, 1), decode2(c[1], s, 0), decode2(c[1], s, 1));
-            const uint4 up = make_uint4(decode2(c[2], s, 0), decode2(c[2], s, 1), decode2(c[3], s, 0), decode2(c[3], s, 1));
-            const int ch = (cc >> 3) + 2 * h;
-            *reinterpret_cast<uint4*>(b + ((ch ^ swz(cr)) << 4)) = lo;
-            *reinterpret_cast<uint4*>(b + (((ch + 1) ^ swz(cr)) << 4)) = up;
+            unsigned char* b = tile + (cr + 32 * h) * 256;
+            const float s = pow2(f.s[h]);
+            const u32x4 c = f.c[h];
+            const uint32_t a0 = odd ? c[2] : c[0], a1 = odd ? c[3] : c[1], b0 = odd ? c[0] : c[2], b1 = odd ? c[1] : c[3];
+            const int ch = (cc >> 3) + odd;
+            *reinterpret_cast<uint4*>(b + ((ch ^ swz(cr)) << 4)) = make_uint4(decode2(a0, s, 0), decode2(a0, s, 1), decode2(a1, s, 0), decode2(a1, s, 1));
+            *reinterpret_cast<uint4*>(b + (((ch ^ 1) ^ swz(cr)) << 4)) = make_uint4(decode2(b0, s, 0), decode2(b0, s, 1), decode2(b1, s, 0), decode2(b1, s, 1));
         }
     };
     // transposed fragments: lane group g = lane >> 4 reads rows 8 * (g >> 1) + (i >> 2) [+ 4], columns 16 * (g & 1) + 4 * (i & 3)
@@ -845,7 +888,7 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
     for (int e = 0; e < 8; ++e) ones[e] = (decltype(ones[0] + ones[0]))1.0f;
     const bool with_db = tk == 0 && wn == 0;
 
-    // In flight at the top of step ks: the loads of steps ks and ks + 1, 4 LDS-DMA and 3 register loads each, in this order.
+    // In flight at the top of step ks: the loads of steps ks and ks + 1, 4 LDS-DMA and 4 register loads each, in this order.
     // (restrict pointers, waits outside: see q8_mm_body)
     auto multiply = [&](int ks, const unsigned char* __restrict__ sa, const unsigned char* __restrict__ sb, unsigned char* __restrict__ next, Fetched& f) {
         issue(ks + 2, next);              // (rows behind the range load nothing)
@@ -869,7 +912,7 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
         }
     };
     auto step = [&](int ks, int a_buf, Fetched& f) {
-        asm volatile("s_waitcnt vmcnt(7)" ::: "memory");   // step ks has landed
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // step ks has landed
         unsigned char* xb = q8_sm + (3 + (ks & 1)) * WG_TILE;
         spread(f, xb);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1052,11 +1095,12 @@ __global__ __launch_bounds__(TPB) void q8_tail_fwd(const uint16_t* __restrict__ 
         float v[8], w[8];
         unpack8(q[j], v);
         unpack8(t[j], w);
-        const uint32_t s = KEEP ? scale_of(group_max<LPB>(amax8(v, TOP16))) : 0u;
-        sb[j] = s;
+        uint2 e = make_uint2(0, 0);
+        sb[j] = 0;
+        if (KEEP) e = quantize8<LPB>(q[j], sb[j]);
         if (r0 + j >= M) continue;
         const long o = (long)(r0 + j) * C + c0;
-        if (KEEP && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = encode8(v, inv_scale(s), TOP16);
+        if (KEEP && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = e;
         if (!on) continue;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
