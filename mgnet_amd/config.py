@@ -212,6 +212,9 @@ _MGNET_KEYS = {
                        "FFM_CHANNELS": 256, "HEAD_CHANNELS": 256, "INIT_METHOD": "default", "MSC_LOSS": True,
                        "SSIM_LOSS_WEIGHT": 0.85, "PHOTOMETRIC_LOSS_WEIGHT": 1.0, "SMOOTHING_LOSS_WEIGHT": 0.001,
                        "AUTOMASK_LOSS": True, "PHOTOMETRIC_REDUCE_OP": "min", "PADDING_MODE": "zeros"},
+        # (keys added by mgnet_amd) 8-bit training, off by default.  BLOCK_TAILS: the residual blocks' tails keep their input in 8 bits for the
+        # backward pass (ops.abn_add_relu_q8); POINTWISE: the 1x1 predictors and pose convolutions run as 8-bit products (ops.conv1x1_q8)
+        "Q8": {"BLOCK_TAILS": False, "POINTWISE": False},
         "POST_PROCESSING": {"STUFF_AREA": 2048, "CENTER_THRESHOLD": 0.3, "NMS_KERNEL": 7, "USE_DGC_SCALING": True},
     },
     "TEST": {"AMP": {"ENABLED": True}, "MSC_FLIP_EVAL": False, "EVAL_SEMANTIC": True, "EVAL_INSTANCE": False,

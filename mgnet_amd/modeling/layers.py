@@ -81,12 +81,16 @@ class Conv2d(nn.Conv2d):
 
 
 class PlainConv2d(nn.Conv2d):
-    """nn.Conv2d whose forward goes through ops.conv2d (predictors, PoseCNN decoder convs)."""
+    """nn.Conv2d whose forward goes through ops.conv2d (predictors, PoseCNN decoder convs).
+    q8 (MODEL.Q8.POINTWISE): a 1x1 convolution of this kind trains through ops.conv1x1_q8 (inference stays in 16 bits)."""
+    q8 = False
 
     def forward(self, x, relu=False, keep_pad=False):
         """relu: `torch.relu_(conv(x))` with the ReLU in the convolution's epilogue (and its mask in the backward) on the GPU path.
         keep_pad: a few-channel predictor may return its 32-channel-padded output as an ops.PaddedMap (training path: the fused
         losses / ops.head_activation read it in place and hand back a padded gradient)"""
+        if self.q8 and ops.conv1x1_q8_supported(x, self):
+            return ops.conv1x1_q8_layer(x, self.weight, self.bias, relu, keep_pad)
         if relu and os.environ.get("MGN_NO_POSERELU"):
             return torch.relu_(ops.conv2d(x, self.weight, self.bias, self.stride, self.padding))
         return ops.conv2d(x, self.weight, self.bias, self.stride, self.padding, relu=relu, keep_pad=keep_pad)

@@ -17,7 +17,8 @@ from ..registry import (DEPTH_HEADS_REGISTRY, INS_EMBED_HEADS_REGISTRY, META_ARC
                         configurable)
 from ..structures import ImageList
 from . import ops
-from .layers import GlobalContextModule, MGNetDecoder, MGNetHead, PoseCNN
+from .layers import GlobalContextModule, MGNetDecoder, MGNetHead, PlainConv2d, PoseCNN
+from .res_net import BasicBlock
 from .loss import DeepLabCE, MultiViewPhotometricLoss, OhemCE
 
 __all__ = ["MGNet", "INS_EMBED_HEADS_REGISTRY", "build_ins_embed_head", "DEPTH_HEADS_REGISTRY", "build_depth_head",
@@ -39,6 +40,16 @@ def _decoder_kwargs(node, input_shape, feature_node=None):
     return dict(input_shape={k: v for k, v in input_shape.items() if k in feats}, common_stride=node.COMMON_STRIDE,
                 arm_channels=node.ARM_CHANNELS, refine_channels=node.REFINE_CHANNELS, ffm_channels=node.FFM_CHANNELS,
                 head_channels=node.HEAD_CHANNELS, init_method=node.INIT_METHOD)
+
+
+def _set_q8(node, parts):
+    """MODEL.Q8 -> the modules' own switches (layers.PlainConv2d.q8, res_net.BasicBlock.q8)"""
+    for part in parts:
+        for m in part.modules() if part is not None else ():
+            if isinstance(m, BasicBlock):
+                m.q8 = bool(node.BLOCK_TAILS)
+            elif isinstance(m, PlainConv2d) and m.kernel_size == (1, 1):
+                m.q8 = bool(node.POINTWISE)
 
 
 @META_ARCH_REGISTRY.register()
@@ -78,6 +89,7 @@ class MGNet(nn.Module):
             sem, ins = build_sem_seg_head(cfg, shapes), build_ins_embed_head(cfg, shapes)
         if cfg.WITH_DEPTH:
             dep, pose = build_depth_head(cfg, shapes), PoseCNN(cfg)
+        _set_q8(cfg.MODEL.Q8, (backbone, sem, ins, dep, pose))
         meta = MetadataCatalog.get(cfg.DATASETS.TRAIN[0] if len(cfg.DATASETS.TRAIN) else "cityscapes")  # mg_net.py:147
         pan_fn = dep_fn = ins_fn = None
         if cfg.TEST.EVAL_INSTANCE:   # mg_net.py:145-153

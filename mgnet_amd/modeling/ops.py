@@ -1312,4 +1312,5 @@ def uncertainty_weighting(losses, log_vars, k0=0):
     return ({k: weighted[i] for i, k in enumerate(keys)}, {k: raw[i].detach() for i, k in enumerate(keys)}, {k: unc[i] for i, k in enumerate(keys)})
 
 
-from .q8 import Q8Map, abn_add_relu_q8, conv1x1_q8, q8_matmul, q8_pack  # noqa: E402,F401  (8-bit operators: they use the helpers above)
+from .q8 import (Q8Map, abn_add_relu_q8, abn_add_relu_q8_supported, conv1x1_q8, conv1x1_q8_layer, conv1x1_q8_supported,  # noqa: E402,F401
+                 q8_matmul, q8_pack)   # (8-bit operators: they use the helpers above)

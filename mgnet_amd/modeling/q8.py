@@ -2,11 +2,12 @@
 `ops`: q8_pack / Q8Map, q8_matmul, conv1x1_q8, abn_add_relu_q8.  [HIP] only: a CPU tensor raises."""
 import torch
 import torch.distributed as dist
+import torch.nn.functional as F
 
 from .. import _C
-from .ops import _allreduce_sums, _dist_active, _pstats, _train_coef
+from .ops import PaddedMap, _allreduce_sums, _dist_active, _pstats, _train_coef
 
-__all__ = ["Q8Map", "q8_pack", "q8_matmul", "conv1x1_q8", "abn_add_relu_q8"]
+__all__ = ["Q8Map", "q8_pack", "q8_matmul", "conv1x1_q8", "conv1x1_q8_supported", "conv1x1_q8_layer", "abn_add_relu_q8", "abn_add_relu_q8_supported"]
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _CL = torch.channels_last
@@ -212,6 +213,22 @@ def conv1x1_q8(x, weight, bias=None, relu=False):
     return _Conv1x1Q8Fn.apply(x, weight, bias, relu)
 
 
+def conv1x1_q8_supported(x, conv):
+    """a training call of an nn.Conv2d that conv1x1_q8 covers; vectors (1 x 1 maps) keep their 16 bits: nothing is saved there"""
+    return (x.is_cuda and x.dtype in _C.H16 and x.dim() == 4 and conv.training and torch.is_grad_enabled() and conv.kernel_size == (1, 1)
+            and conv.stride == (1, 1) and conv.padding == (0, 0) and conv.groups == 1 and conv.in_channels == x.shape[1]
+            and x.shape[2] * x.shape[3] > 1 and x.shape[0] > 0)
+
+
+def conv1x1_q8_layer(x, weight, bias=None, relu=False, keep_pad=False):
+    """conv1x1_q8 behind ops.conv2d's interface: with keep_pad, output channels that are not a multiple of 32 come as the 32-padded PaddedMap"""
+    Cout = weight.shape[0]
+    pad = -Cout % 32
+    if not (keep_pad and pad):
+        return conv1x1_q8(x, weight, bias, relu)
+    return PaddedMap(conv1x1_q8(x, F.pad(weight, (0, 0, 0, 0, 0, 0, 0, pad)), None if bias is None else F.pad(bias, (0, pad)), relu), Cout)
+
+
 class _AbnAddReluQ8Fn(torch.autograd.Function):
     """[HIP] csrc/q8.hip: the residual block's tail relu(norm(x) + shortcut) as ops._AbnAddReluFn, with x kept for the backward pass in 8 bits
     (the norm's x_hat is recomputed from there) and the ReLU mask in one bit a value; y is not kept."""
@@ -282,3 +299,10 @@ def abn_add_relu_q8(x, norm, shortcut):
         with torch.cuda.device(x.device):
             return _AbnAddReluQ8Fn.apply(*args)
     return _AbnAddReluQ8Fn.apply(*args)
+
+
+def abn_add_relu_q8_supported(x, norm, shortcut):
+    """a training call of a block tail that abn_add_relu_q8 covers"""
+    return (x.is_cuda and x.dtype in _C.H16 and norm.training and torch.is_grad_enabled() and norm.activation == "identity" and x.shape[1] % 8 == 0
+            and x.shape[1] <= 8192 and x.numel() > 0 and x.shape == shortcut.shape and x.dtype == shortcut.dtype
+            and norm.running_mean.dtype == torch.float32)

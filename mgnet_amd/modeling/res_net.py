@@ -18,6 +18,8 @@ def c2_msra_fill(module):
 
 
 class BasicBlock(nn.Module):  # res_net.py:11-79
+    q8 = False   # MODEL.Q8.BLOCK_TAILS: the tail keeps its input in 8 bits for the backward pass
+
     def __init__(self, in_channels, out_channels, *, stride=1):
         super().__init__()
         self.in_channels, self.out_channels, self.stride = in_channels, out_channels, stride
@@ -50,7 +52,10 @@ class BasicBlock(nn.Module):  # res_net.py:11-79
             out, skip = self.conv1(x, with_skip=True)   # res_net.py:62-79; `skip` is x: the shortcut's gradient joins conv1's dgrad
             sc = skip if self.shortcut is None else self.shortcut(skip)
         c2 = self.conv2   # conv -> InPlaceABNSync(identity) -> + shortcut -> ReLU; norm, add and ReLU run as one fused op on the GPU
-        return ops.abn_add_relu(ops.conv2d(out, c2.weight, c2.bias, c2.stride, c2.padding, stats_for=c2.norm), c2.norm, sc)
+        y = ops.conv2d(out, c2.weight, c2.bias, c2.stride, c2.padding, stats_for=c2.norm)
+        if self.q8 and ops.abn_add_relu_q8_supported(y, c2.norm, sc):
+            return ops.abn_add_relu_q8(y, c2.norm, sc)
+        return ops.abn_add_relu(y, c2.norm, sc)
 
 
 class BasicStem(nn.Module):  # res_net.py:82-110
