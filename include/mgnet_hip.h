@@ -805,7 +805,8 @@ int mgn_project_bwd(const float* points, const float* A, const float* t, const f
  * mgn_q8_pack_weight: w [N][K] with element strides sr, sc -> tile scales; codes/scales of [N][K] and / or codes_t/scales_t of its
  *                     transpose [K][N] (the same values).  A pair may be NULL.
  * mgn_q8_matmul     : out[m][n] = act( sum_k a[m][k] b[n][k] + bias[n] ), a [M][K], b [N][K] packed, fp32 accumulation, one rounding;
- *                     act 0 none | 1 ReLU | 2 leaky ReLU; out fp32 or 16-bit, rows ldo elements apart.
+ *                     act 0 none | 1 ReLU | 2 leaky ReLU (0 <= slope <= 1); out fp32 or 16-bit, rows ldo elements
+ *                     apart.
  * mgn_q8_pack_matmul: mgn_q8_pack of the 16-bit matrix x [M][K] (rows ldx elements apart) and mgn_q8_matmul of its packed form in one pass
  *                     over x; codes / scales: where the packed form is kept, or both NULL.  MGN_ENOTSUP (nothing done; pack first then):
  *                     K > 512, K % 8 or ldx % 8 != 0, x not 16-byte aligned; N > 32 with N % 8 or ldo % 8 != 0 or an fp32 result.  Same result as the two calls up to the order of the fp32 sums.

@@ -346,14 +346,18 @@ __global__ __launch_bounds__(TILE_TPB) void q8_pack_tile(const T* __restrict__ w
 //   towards zero to a multiple of 2^-13 of the largest one's binade.  1.3e-5 of a result (2-norm, Gaussian operands): far below the
 //   rounding to 16 bits (1.7e-3 / 2.1e-4) and the operands' own (2.6e-2); a 32-bit result carries it.
 // ------------------------------------------------------------------------------------------------------
-// act(v) without a branch: ReLU is lo = 0, neg = 1; leaky ReLU lo = -inf, neg = slope; none lo = -inf, neg = 1 (a NaN passes all comparisons)
+// act(v) without a branch: ReLU is lo = 0, neg = 1; leaky ReLU lo = -inf, neg = slope (0 < slope <= 1); none lo = -inf, neg = 1.  `maximum`
+// passes a NaN on.
 struct Act { float lo, neg; };
 __device__ __forceinline__ float activate(float v, const Act& a) {
-    v = v < a.lo ? a.lo : v;
-    const float t = v * a.neg;
-    return v > 0.f ? v : t;
+    v = __builtin_elementwise_maximum(v, a.lo);
+    return __builtin_elementwise_maximum(v, v * a.neg);
 }
-inline Act make_act(int act, float slope) { return Act{act == 1 ? 0.f : -__builtin_inff(), act == 2 ? slope : 1.f}; }
+inline Act make_act(int act, float slope) {
+    const bool relu = act == 1 || (act == 2 && slope == 0.f);
+    return Act{relu ? 0.f : -__builtin_inff(), act == 2 && !relu ? slope : 1.f};
+}
+inline bool act_ok(int act, float slope) { return act == 0 || act == 1 || (act == 2 && slope >= 0.f && slope <= 1.f); }
 struct MmParams {
     const unsigned char *a, *sa, *b, *sb;
     const float* bias;
@@ -606,33 +610,6 @@ __device__ __forceinline__ void q8_stream_body(const StreamParams& p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, hi = lane >> 5;
     const int n0 = (blockIdx.y * WN + (WN == 1 ? 0 : wave)) * NT * 32;
 
-    // the wave's weights
-    i32x8 w[NT][KB * 2];
-    int ws[NT][KB];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int n = n0 + t * 32 + lr;
-        const unsigned char* row = p.b + (long)(n < p.N ? n : 0) * p.ldb;
-#pragma unroll
-        for (int kk = 0; kk < KB * 2; ++kk) {
-            int4 u[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = kk * 64 + hi * 32 + h * 16;
-                u[h] = (n < p.N && c < p.ldb) ? *reinterpret_cast<const int4*>(row + c) : make_int4(0, 0, 0, 0);
-            }
-            w[t][kk] = i32x8{u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-        }
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) ws[t][kb] = (n < p.N && kb * BLK < p.K) ? p.sb[(long)kb * p.ldb_s + n] : 0;
-    }
-
-    float* bias = reinterpret_cast<float*>(q8_sm + 2 * (S::TILE + KB * S::BM));
-    if (tid < NT * WN * 32) {
-        const int n = blockIdx.y * NT * WN * 32 + tid;
-        bias[tid] = (p.bias && n < p.N) ? p.bias[n] : 0.f;
-    }
-
     // source: unit u = pass * (TH / LPU) + tid / LPU = (row u / KB, block u % KB).  All memory traffic of the loop goes through buffer
     // descriptors of the tile's rows: rows and columns that are not there read as zeros and are not written, without a branch.
     const int ul = tid % S::LPU, u0 = tid / S::LPU, ukb = u0 % KB, urow = u0 / KB;   // (TH / LPU is a multiple of KB)
@@ -680,6 +657,36 @@ __device__ __forceinline__ void q8_stream_body(const StreamParams& p) {
     int tile = blockIdx.x, buf = 0;
     if (tile >= p.ntiles) return;
     fetch(tile);
+
+    // the wave's weights
+    i32x8 w[NT][KB * 2];
+    int ws[NT][KB];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int n = n0 + t * 32 + lr;
+        const unsigned char* row = p.b + (long)(n < p.N ? n : 0) * p.ldb;
+#pragma unroll
+        for (int kk = 0; kk < KB * 2; ++kk) {
+            int4 u[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = kk * 64 + hi * 32 + h * 16;
+                u[h] = (n < p.N && c < p.ldb) ? *reinterpret_cast<const int4*>(row + c) : make_int4(0, 0, 0, 0);
+            }
+            w[t][kk] = i32x8{u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) ws[t][kb] = (n < p.N && kb * BLK < p.K) ? p.sb[(long)kb * p.ldb_s + n] : 0;
+    }
+
+    float* bias = reinterpret_cast<float*>(q8_sm + 2 * (S::TILE + KB * S::BM));
+    if (tid < NT * WN * 32) {
+        const int n = blockIdx.y * NT * WN * 32 + tid;
+        bias[tid] = (p.bias && n < p.N) ? p.bias[n] : 0.f;
+    }
+
+    // (the weights have arrived before the loop: waited for at their first use inside it, every round would wait for the stores before it too)
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
     settle(tile, 0);
     for (;;) {
         fetch(tile + gridDim.x);          // (behind the last tile there are no rows: nothing is loaded, and the loop keeps one shape)
@@ -1365,7 +1372,7 @@ int MGN_SYM(mgn_q8_pack_weight)(const void* w, int dtype, long sr, long sc, int 
 
 int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const void* b, const void* b_scales, int N, int K, const float* bias, int act,
                            float slope, void* out, int out_f32, long ldo, void* stream_) {
-    if (M < 0 || M > MAX_ROWS || N < 1 || N > MAX_COLS || K < 1 || K > MAX_COLS || act < 0 || act > 2 || ldo < N) return MGN_EINVAL;
+    if (M < 0 || M > MAX_ROWS || N < 1 || N > MAX_COLS || K < 1 || K > MAX_COLS || !act_ok(act, slope) || ldo < N) return MGN_EINVAL;
     if (M == 0) return MGN_OK;
     if (!a || !a_scales || !b || !b_scales || !out || !aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 16) || !aligned(b_scales, 16) ||
         !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;
@@ -1395,7 +1402,7 @@ int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const vo
 
 int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* codes, void* scales, const void* b, const void* b_scales, int N,
                                 const float* bias, int act, float slope, void* out, int out_f32, long ldo, void* stream_) {
-    if (M < 0 || M > MAX_ROWS || N < 1 || N > MAX_COLS || K < 1 || K > MAX_COLS || act < 0 || act > 2 || ldo < N || ldx < K || ldx > MAX_COLS) return MGN_EINVAL;
+    if (M < 0 || M > MAX_ROWS || N < 1 || N > MAX_COLS || K < 1 || K > MAX_COLS || !act_ok(act, slope) || ldo < N || ldx < K || ldx > MAX_COLS) return MGN_EINVAL;
     if (M == 0) return MGN_OK;
     if (!x || !b || !b_scales || !out || !codes != !scales || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(b, 16) || !aligned(x, 2) ||
         !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;

@@ -108,7 +108,7 @@ _ACT = {"none": 0, "relu": 1, "leaky_relu": 2}
 def q8_matmul(a, b, bias=None, act="none", slope=0.01, out_dtype=None):
     """act(a b^T + bias) of two packed matrices a [M, K] (or a map [N, K, H, W]: the result is the map [N, n, H, W]) and b [n, K]; products
     of codes scaled in the matrix cores, fp32 accumulation, one rounding to out_dtype (default: a's source type).  act: none | relu |
-    leaky_relu (slope).  No gradient (conv1x1_q8 has one)."""
+    leaky_relu (0 <= slope <= 1).  No gradient (conv1x1_q8 has one)."""
     if not (isinstance(a, Q8Map) and isinstance(b, Q8Map)):
         raise ValueError("q8_matmul: two Q8Map operands (ops.q8_pack)")
     if len(b.shape) != 2 or a.channels != b.channels:
@@ -117,8 +117,8 @@ def q8_matmul(a, b, bias=None, act="none", slope=0.01, out_dtype=None):
     if dev != b.buf.device or (bias is not None and bias.device != dev):
         raise ValueError("q8_matmul: operands on different devices")
     out_dtype = a.dtype if out_dtype is None else out_dtype
-    if act not in _ACT or out_dtype not in _FLOATS:
-        raise ValueError(f"q8_matmul: act one of {sorted(_ACT)}, a float32 / bfloat16 / float16 result; got {act}, {out_dtype}")
+    if act not in _ACT or out_dtype not in _FLOATS or not 0 <= slope <= 1:
+        raise ValueError(f"q8_matmul: act one of {sorted(_ACT)}, 0 <= slope <= 1, a float32 / bfloat16 / float16 result; got {act}, {slope}, {out_dtype}")
     n, M = b.rows, a.rows
     if n < 1:
         raise ValueError("q8_matmul: b has no rows")

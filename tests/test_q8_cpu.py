@@ -45,9 +45,9 @@ def test_c_refusals(sfx):
     weight = lambda w=BUF, dt=0, N=4, K=4, c=BUF, s=BUF, ct=None, st=None: fn("mgn_q8_pack_weight")(w, dt, K, 1, N, K, c, s, ct, st, None)  # noqa: E731
     for kw in (dict(w=None), dict(N=0), dict(K=0), dict(c=None), dict(s=None), dict(c=None, s=None), dict(ct=BUF), dict(st=BUF), dict(dt=3)):
         assert weight(**kw) == -22, kw
-    mm = lambda a=BUF, sa=BUF, M=4, b=BUF, sb=BUF, N=4, K=4, act=0, out=BUF, f32=0, ldo=4: fn("mgn_q8_matmul")(a, sa, M, b, sb, N, K, None, act, 0.0, out, f32, ldo, None)  # noqa: E731
+    mm = lambda a=BUF, sa=BUF, M=4, b=BUF, sb=BUF, N=4, K=4, act=0, slope=0.0, out=BUF, f32=0, ldo=4: fn("mgn_q8_matmul")(a, sa, M, b, sb, N, K, None, act, slope, out, f32, ldo, None)  # noqa: E731
     assert mm(M=0) == 0
-    for kw in (dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(out=None), dict(N=0), dict(K=0), dict(act=3), dict(ldo=3), dict(a=BUF + 8), dict(out=BUF + 1), dict(M=-1)):
+    for kw in (dict(a=None), dict(sa=None), dict(b=None), dict(sb=None), dict(out=None), dict(N=0), dict(K=0), dict(act=3), dict(act=2, slope=1.5), dict(act=2, slope=-0.1), dict(ldo=3), dict(a=BUF + 8), dict(out=BUF + 1), dict(M=-1)):
         assert mm(**kw) == -22, kw
     wg = lambda dy=BUF, ldy=8, M=4, N=8, c=BUF, s=BUF, K=8, dw=BUF, ws=BUF, nb=1 << 30: fn("mgn_q8_wgrad")(dy, ldy, M, N, c, s, K, dw, None, ws, nb, None)  # noqa: E731
     for kw in (dict(dy=None), dict(c=None), dict(dw=None), dict(ws=None), dict(ldy=7), dict(ldy=12), dict(M=0), dict(N=0), dict(K=70000), dict(dy=BUF + 2)):

@@ -558,6 +558,7 @@ def test_refusals_on_the_gpu():
                 lambda: o.conv1x1_q8(x, w[:, :8]), lambda: o.conv1x1_q8(x, torch.zeros((8, 16, 3, 3), device="cuda")), lambda: o.conv1x1_q8(x, w, torch.zeros(7, device="cuda")),
                 lambda: o.conv1x1_q8(x, w.cpu()), lambda: o.q8_matmul(o.q8_pack(x), o.q8_pack(torch.zeros((8, 24), device="cuda"), tile=True)),
                 lambda: o.q8_matmul(o.q8_pack(x), w), lambda: o.q8_matmul(o.q8_pack(x), o.q8_pack(w.view(8, 16), tile=True), act="gelu"),
+                lambda: o.q8_matmul(o.q8_pack(x), o.q8_pack(w.view(8, 16), tile=True), act="leaky_relu", slope=2.0),
                 lambda: o.q8_matmul(o.q8_pack(x), o.q8_pack(w.view(8, 16), tile=True), bias=torch.zeros(9, device="cuda")),
                 lambda: o.q8_matmul(o.q8_pack(x), o.q8_pack(w.view(8, 16), tile=True), out_dtype=torch.float64), lambda: o.q8_pack(x).unpack(torch.int8)):
         with pytest.raises(ValueError):
