@@ -19,6 +19,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "h16.h"
 #include "mgnet_hip.h"
 
@@ -896,50 +898,60 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
     const bool with_db = tk == 0 && wn == 0;
 
     // In flight at the top of step ks: the loads of steps ks and ks + 1, 4 LDS-DMA and 4 register loads each, in this order.
+    // The 16 rows of the next MFMAs are read while the current ones run; `db` (with the ones column) is a type, so that no branch parts the step.
     // (restrict pointers, waits outside: see q8_mm_body)
-    auto multiply = [&](int ks, const unsigned char* __restrict__ sa, const unsigned char* __restrict__ sb, unsigned char* __restrict__ next, Fetched& f) {
+    auto multiply = [&](auto db, int ks, const unsigned char* __restrict__ sa, const unsigned char* __restrict__ sb, unsigned char* __restrict__ next, Fetched& f) {
+        h16x8 a[2][2], b[2][2];
+        auto read = [&](int kk) {         // the swizzle depends on row bits 0..1: unchanged by + 16 rows
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[kk & 1][i] = frag(sa + fa[i] + kk * 16 * 256);
+                b[kk & 1][i] = frag(sb + fb[i] + kk * 16 * 256);
+            }
+        };
+        read(0);
         issue(ks + 2, next);              // (rows behind the range load nothing)
         f = fetch(ks + 2);
 #pragma unroll
-        for (int kk = 0; kk < WG_ROWS / 16; ++kk) {   // the swizzle depends on row bits 0..1: unchanged by + 16 rows
-            h16x8 a[2], b[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i] = frag(sa + fa[i] + kk * 16 * 256);
-                b[i] = frag(sb + fb[i] + kk * 16 * 256);
-            }
+        for (int kk = 0; kk < WG_ROWS / 16; ++kk) {
+            if (kk + 1 < WG_ROWS / 16) read(kk + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = MGN_MFMA_32x32x16(a[i], b[j], acc[i][j]);
-            if (with_db) {
-                accb[0] = MGN_MFMA_32x32x16(a[0], ones, accb[0]);
-                accb[1] = MGN_MFMA_32x32x16(a[1], ones, accb[1]);
+                for (int j = 0; j < 2; ++j) acc[i][j] = MGN_MFMA_32x32x16(a[kk & 1][i], b[kk & 1][j], acc[i][j]);
+            if constexpr (decltype(db)::value) {
+                accb[0] = MGN_MFMA_32x32x16(a[kk & 1][0], ones, accb[0]);
+                accb[1] = MGN_MFMA_32x32x16(a[kk & 1][1], ones, accb[1]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto step = [&](int ks, int a_buf, Fetched& f) {
-        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // step ks has landed
-        unsigned char* xb = q8_sm + (3 + (ks & 1)) * WG_TILE;
-        spread(f, xb);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();     // ... for everyone; step ks - 1 has been read
-        multiply(ks, q8_sm + a_buf * WG_TILE, xb, q8_sm + (a_buf == 0 ? 2 : a_buf - 1) * WG_TILE, f);
+    auto run = [&](auto db) {
+        auto step = [&](int ks, int a_buf, Fetched& f) {
+            asm volatile("s_waitcnt vmcnt(8)" ::: "memory");   // step ks has landed
+            unsigned char* xb = q8_sm + (3 + (ks & 1)) * WG_TILE;
+            spread(f, xb);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();     // ... for everyone; step ks - 1 has been read
+            multiply(db, ks, q8_sm + a_buf * WG_TILE, xb, q8_sm + (a_buf == 0 ? 2 : a_buf - 1) * WG_TILE, f);
+        };
+        issue(0, q8_sm);
+        Fetched f0 = fetch(0);
+        __builtin_amdgcn_sched_barrier(0);    // (in this order: the loop's waits count on it)
+        issue(1, q8_sm + WG_TILE);
+        __builtin_amdgcn_sched_barrier(0);
+        Fetched f1 = fetch(1);
+        __builtin_amdgcn_sched_barrier(0);
+        int a_buf = 0;
+        for (int ks = 0; ks < steps; ks += 2) {   // (an odd last step multiplies rows of zeros)
+            step(ks, a_buf, f0);
+            a_buf = a_buf == 2 ? 0 : a_buf + 1;
+            step(ks + 1, a_buf, f1);
+            a_buf = a_buf == 2 ? 0 : a_buf + 1;
+        }
     };
-    issue(0, q8_sm);
-    Fetched f0 = fetch(0);
-    __builtin_amdgcn_sched_barrier(0);    // (in this order: the loop's waits count on it)
-    issue(1, q8_sm + WG_TILE);
-    __builtin_amdgcn_sched_barrier(0);
-    Fetched f1 = fetch(1);
-    __builtin_amdgcn_sched_barrier(0);
-    int a_buf = 0;
-    for (int ks = 0; ks < steps; ks += 2) {   // (an odd last step multiplies rows of zeros)
-        step(ks, a_buf, f0);
-        a_buf = a_buf == 2 ? 0 : a_buf + 1;
-        step(ks + 1, a_buf, f1);
-        a_buf = a_buf == 2 ? 0 : a_buf + 1;
-    }
+    if (with_db) run(std::true_type{}); else run(std::false_type{});
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no LDS-DMA outlives the block
     const long wsize = ((long)p.N * p.K + p.N + 3) & ~3L;
     float* out = p.part + (long)z * wsize;
