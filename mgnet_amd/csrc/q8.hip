@@ -367,11 +367,14 @@ struct MmParams {
     int M, N, K, nb, ld;                  // ld: bytes per code row (both operands)
     long lda_s, ldb_s, ldo;               // scale rows; elements per row of out
     Act act;
-    int out32, vec;                       // vec: rows of out are 4-element aligned
-    int mt, nt, group;
+    int out32;
+    int mt, nt;
 };
 MGN_PLAN_RO(MmParams, MGN_RO(a) MGN_RO(sa) MGN_RO(b) MGN_RO(sb) MGN_RO(bias))
 
+// 16 and 8 bytes at any address that suits an element: global stores need no more
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 // four consecutive n of row m
 template <typename P>
@@ -384,41 +387,100 @@ __device__ __forceinline__ void mm_emit(const P& p, long m, int n, const float (
     }
     if (p.out32) {
         float* o = (float*)p.out + m * p.ldo + n;
-        if (p.vec && n + 3 < p.N) { *reinterpret_cast<float4*>(o) = make_float4(r[0], r[1], r[2], r[3]); return; }
+        if (n + 3 < p.N) { *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4_any, make_float4(r[0], r[1], r[2], r[3])); return; }
 #pragma unroll
         for (int e = 0; e < 4; ++e) if (n + e < p.N) o[e] = r[e];
     } else {
         uint16_t* o = (uint16_t*)p.out + m * p.ldo + n;
         const uint2 w = make_uint2(mgn_pack2(r[0], r[1]), mgn_pack2(r[2], r[3]));
-        if (p.vec && n + 3 < p.N) { *reinterpret_cast<uint2*>(o) = w; return; }
+        if (n + 3 < p.N) { *reinterpret_cast<u32x2_any*>(o) = u32x2_any{w.x, w.y}; return; }
 #pragma unroll
         for (int e = 0; e < 4; ++e) if (n + e < p.N) o[e] = (uint16_t)((e < 2 ? w.x : w.y) >> (16 * (e & 1)));
     }
 }
 
-template <int BM, int BN, int WVM, int WVN>
+template <int BM, int BN, int WVM, int WVN, int ST>
 struct MmTile {
     static constexpr int NW = WVM * WVN, TM = BM / WVM / 32, TN = BN / WVN / 32;
     static constexpr int ABYTES = BM * BLK, STAGE = (BM + BN) * BLK, SCALES = 512;   // [256 rows of A][256 rows of B]
     static constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;                           // 1-KB pieces (8 rows) per wave and stage
-    static constexpr int LDS = 2 * (STAGE + SCALES);
-    static_assert(PA * NW * 8 == BM && (PB * NW * 8 == BN) && BM <= 256 && BN <= 256 && NW % 2 == 0, "tile shape");
+    static constexpr int LDS = ST * (STAGE + SCALES), OUT = 32 * (TN * 32 * 4 + 16);     // OUT: a wave's share on the way out
+    static_assert(NW * OUT <= LDS && PA * NW * 8 == BM && (PB * NW * 8 == BN) && BM <= 256 && BN <= 256 && NW % 2 == 0, "tile shape");
 };
+
+// the accumulators of TM x TN 32 x 32 tiles (channels by 4 in a lane, rows over lanes) as rows of out from (m0, n0); `sm`: the wave's own LDS
+template <int TM, int TN, typename T>
+__device__ __forceinline__ void mm_store(const MmParams& p, const f32x16 (&acc)[TN][TM], unsigned char* sm, long m0, int n0, int lane) {
+    constexpr int E = 16 / sizeof(T), PITCH = TN * 32 * sizeof(T) + 16, CHUNKS = TN * 32 / E, ROWS = 64 / CHUNKS;
+    const int lr = lane & 31, hi = lane >> 5, row = lane / CHUNKS, n = n0 + lane % CHUNKS * E;
+    float bias[TN][16];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int c = n0 + i * 32 + 8 * (e >> 2) + 4 * hi + (e & 3);
+            bias[i][e] = (p.bias && c < p.N) ? p.bias[c] : 0.f;
+        }
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float r[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] = activate(acc[i][j][4 * q + e] + bias[i][4 * q + e], p.act);
+                unsigned char* d = sm + lr * PITCH + (i * 32 + 8 * q + 4 * hi) * sizeof(T);
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(d) = make_float4(r[0], r[1], r[2], r[3]);
+                else *reinterpret_cast<uint2*>(d) = make_uint2(mgn_pack2(r[0], r[1]), mgn_pack2(r[2], r[3]));
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (LDS keeps a wave's order: the next 32 rows need no wait)
+#pragma unroll
+        for (int it = 0; it < 32 / ROWS; ++it) {
+            const long m = m0 + j * 32 + it * ROWS + row;
+            const uint4 w = *reinterpret_cast<const uint4*>(sm + (it * ROWS + row) * PITCH + lane % CHUNKS * 16);
+            if (m >= p.M || n >= p.N) continue;
+            T* o = (T*)p.out + m * p.ldo + n;
+            if (n + E <= p.N) {
+                *reinterpret_cast<u32x4_any*>(o) = u32x4_any{w.x, w.y, w.z, w.w};
+            } else {
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (n + e < p.N) {
+                        if constexpr (sizeof(T) == 4) o[e] = __builtin_bit_cast(float, u[e]);
+                        else o[e] = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+                    }
+            }
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+// The tile of this block.  Tiles are counted through groups of 4 row tiles, in a group column by column; XCD x (= blockIdx % 8) takes the
+// x-th eighth of that sequence, so that the XCDs have equal shares and the tiles in flight on one share rows and columns in its L2.
+__device__ __forceinline__ bool mm_tile(const MmParams& p, int& mtile, int& ntile) {
+    constexpr int G = 4;
+    const long total = (long)p.mt * p.nt;
+    const int x = blockIdx.x & 7, first = (int)(total * x >> 3), t = first + (int)(blockIdx.x >> 3);
+    if (t >= (int)(total * (x + 1) >> 3)) return false;
+    const int g = t / (G * p.nt), in = t - g * G * p.nt, rows = p.mt - g * G < G ? p.mt - g * G : G;
+    ntile = in / rows, mtile = g * G + in - ntile * rows;
+    return true;
+}
+
+constexpr int loads_left(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0070; }   // s_waitcnt vmcnt(n) lgkmcnt(0)
 
 // A block computes a BM x BN tile; a step covers one block of 128 k.  Rows travel HBM/L2 -> LDS by LDS-DMA (16 bytes a lane, 8 rows a
 // piece), two stages; 16-byte chunk c of row r lies at position c ^ ((r >> 1) & 7), so that the 16-byte fragment reads of 16 neighbouring
 // rows cover every bank once.
-template <int BM, int BN, int WVM, int WVN>
+template <int BM, int BN, int WVM, int WVN, int ST>
 __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
-    using Tl = MmTile<BM, BN, WVM, WVN>;
+    using Tl = MmTile<BM, BN, WVM, WVN, ST>;
     extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // XCD x (= blockIdx % 8) owns the row tiles t with (t / group) % 8 == x, in groups of `group` row tiles that run through all column
-    // tiles together: a row tile is read from HBM by one XCD, and the tiles in flight on it share rows and columns
-    const int local = blockIdx.x >> 3, per = p.group * p.nt;
-    const int sg = local / per, in = local - sg * per;
-    const int mtile = (sg * 8 + (blockIdx.x & 7)) * p.group + in % p.group, ntile = in / p.group;
-    if (mtile >= p.mt) return;
+    int mtile, ntile;
+    if (!mm_tile(p, mtile, ntile)) return;
     const long m0 = (long)mtile * BM;
     const int n0 = ntile * BN;
     const int rowsA = (int)(p.M - m0 < BM ? p.M - m0 : BM), rowsB = p.N - n0 < BN ? p.N - n0 : BN;
@@ -441,7 +503,7 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
     }
     auto issue = [&](int kb, unsigned char* st) {
         const int k0 = kb * BLK;
-        const bool in = k0 + col < p.ld;   // (OOB + k0 stays beyond every descriptor)
+        const bool in = k0 + col < p.ld;   // (OOB + k0 stays beyond every descriptor; steps behind the last one load nothing)
 #pragma unroll
         for (int q = 0; q < Tl::PA; ++q)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_ptr)(st + (wave + Tl::NW * q) * 1024), 16, in ? offA[q] + k0 : OOB, 0, 0, 0);
@@ -450,7 +512,7 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_ptr)(st + Tl::ABYTES + (wave + Tl::NW * q) * 1024), 16, in ? offB[q] + k0 : OOB, 0, 0, 0);
         if (wave < 2) {                   // wave 0: A's scales, wave 1: B's
             const unsigned char* s = wave == 0 ? p.sa + (long)kb * p.lda_s + m0 : p.sb + (long)kb * p.ldb_s + n0;
-            const int words = wave == 0 ? sra : srb;
+            const int words = kb < p.nb ? (wave == 0 ? sra : srb) : 0;
             const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(s), 0, (uint32_t)(words * 4), 0x00020000);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(st + Tl::STAGE + wave * 256), 4, lane < words ? lane * 4 : OOB, 0, 0, 0);
         }
@@ -470,7 +532,7 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
     // otherwise takes every LDS read after an LDS-DMA for a read of its target and puts a full s_waitcnt vmcnt(0) between the two, which
     // makes the two stages one: measured 1.9x on a large product.
     auto step = [&](int kb, const unsigned char* __restrict__ st, unsigned char* __restrict__ next) {
-        if (kb + 1 < p.nb) issue(kb + 1, next);
+        issue(kb + ST - 1, next);
         int xs[Tl::TM], ws[Tl::TN];
 #pragma unroll
         for (int j = 0; j < Tl::TM; ++j) xs[j] = st[Tl::STAGE + (wm * Tl::TM + j) * 32 + lr];
@@ -499,31 +561,172 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
                     acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], x[j], acc[i][j], 0, 0, 0, ws[i], 0, xs[j]);
         }
     };
-    issue(0, q8_sm);
+    // `ahead` stages' loads are in flight behind the one that is waited for: PA + PB each, one more in the two waves of the scales.  (This
+    // wave's reads of the step before are through as well: their stage is the next to be loaded.)
+    auto landed = [&]() {
+        constexpr int ahead = ST - 2;
+        if (wave < 2) __builtin_amdgcn_s_waitcnt(loads_left(ahead * (Tl::PA + Tl::PB + 1)));
+        else __builtin_amdgcn_s_waitcnt(loads_left(ahead * (Tl::PA + Tl::PB)));
+        asm volatile("" ::: "memory");
+    };
+#pragma unroll
+    for (int k = 0; k < ST - 1; ++k) issue(k, q8_sm + k * (Tl::STAGE + Tl::SCALES));
+    int cur = 0;
     for (int kb = 0; kb < p.nb; ++kb) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        landed();
         __builtin_amdgcn_s_barrier();     // everyone's rows of step kb have landed, and step kb - 1 has been read
-        step(kb, q8_sm + (kb & 1) * (Tl::STAGE + Tl::SCALES), q8_sm + (~kb & 1) * (Tl::STAGE + Tl::SCALES));
+        const int nxt = cur == 0 ? ST - 1 : cur - 1;
+        step(kb, q8_sm + cur * (Tl::STAGE + Tl::SCALES), q8_sm + nxt * (Tl::STAGE + Tl::SCALES));
+        cur = cur == ST - 1 ? 0 : cur + 1;
     }
-#pragma unroll
-    for (int j = 0; j < Tl::TM; ++j) {
-        const long m = m0 + (wm * Tl::TM + j) * 32 + lr;
-        if (m >= p.M) continue;
-#pragma unroll
-        for (int i = 0; i < Tl::TN; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + (wn * Tl::TN + i) * 32 + 8 * q + 4 * hi;
-                if (n >= p.N) continue;
-                const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                mm_emit(p, m, n, v);
-            }
-    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (empty loads behind the last step write their stages as well)
+    // A wave's 32 rows of 32 TN channels go through LDS, so that they leave as whole row segments, 16 bytes a lane: with 8-byte stores of
+    // each lane's own 4 channels (16 bytes of a row side by side) the write-back of short products is bound by the number of requests.
+    // Rows of out need no alignment beyond their element's (global stores take any address).
+    __syncthreads();                      // the last stage has been read
+    if (p.out32) mm_store<Tl::TM, Tl::TN, float>(p, acc, q8_sm + wave * Tl::OUT, m0 + wm * Tl::TM * 32, n0 + wn * Tl::TN * 32, lane);
+    else mm_store<Tl::TM, Tl::TN, uint16_t>(p, acc, q8_sm + wave * Tl::OUT, m0 + wm * Tl::TM * 32, n0 + wn * Tl::TN * 32, lane);
 }
 
-__global__ __launch_bounds__(512, 1) void q8_mm_256x256(MmParams p) { q8_mm_body<256, 256, 2, 4>(p); }
-__global__ __launch_bounds__(256, 2) void q8_mm_128x128(MmParams p) { q8_mm_body<128, 128, 2, 2>(p); }
-__global__ __launch_bounds__(256, 2) void q8_mm_128x32(MmParams p) { q8_mm_body<128, 32, 4, 1>(p); }
+// Large products: 256 x 256 outputs by eight waves (each 128 x 64: 4 x 2 MFMA tiles), 64 k at a time through a ring of four LDS stages.
+// The waves work in two groups, one slot apart: while one group multiplies (8 MFMAs), the other one reads its next 64 k from LDS and starts
+// the loads of three stages later, so that matrix cores, LDS and loads run together.  Group 0 reads stage h in slot 2h and multiplies in
+// slot 2h + 1, group 1 a slot later; a barrier ends each slot.  Stage h + 3 takes the place of stage h - 1, which group 1 read in slot 2h - 1;
+// every wave has waited for its part of stage h + 1 when slot 2h + 1 ends.
+struct Mm256 {
+    static constexpr int ABYTES = 256 * 64, STAGE = 2 * ABYTES + 512, ST = 4, TM = 4, TN = 2, OUT = 32 * (TN * 32 * 4 + 16);
+    static constexpr int LDS = ST * STAGE;
+    static_assert(8 * OUT <= LDS, "the way out");
+};
+__global__ __launch_bounds__(512, 1) void q8_mm_256x256(MmParams p) {
+    using Tl = Mm256;
+    constexpr int TM = Tl::TM, TN = Tl::TN;
+    extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, hi = lane >> 5;
+    int mtile, ntile;
+    if (!mm_tile(p, mtile, ntile)) return;
+    const long m0 = (long)mtile * 256;
+    const int n0 = ntile * 256;
+    const int rowsA = (int)(p.M - m0 < 256 ? p.M - m0 : 256), rowsB = p.N - n0 < 256 ? p.N - n0 : 256;
+    const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a + m0 * p.ld), 0, (uint32_t)(rowsA * p.ld), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsB = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b + (long)n0 * p.ld), 0, (uint32_t)(rowsB * p.ld), 0x00020000);
+    const int nh = (p.ld + 63) >> 6;
+    // 16-byte chunk c of row r at c ^ ((r >> 2) & 3): 16 neighbouring rows cover every bank once
+    const int col = ((lane & 3) ^ ((lane >> 4) & 3)) << 4;
+    int offA[2], offB[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int r = (wave + 8 * q) * 16 + (lane >> 2);
+        offA[q] = r < rowsA ? r * p.ld + col : OOB;
+        offB[q] = r < rowsB ? r * p.ld + col : OOB;
+    }
+    auto issue = [&](int h, unsigned char* st) {
+        // (offsets with the top bit set stay beyond every descriptor; stages behind the last one load nothing)
+        const int k0 = h * 64, out = k0 + col < p.ld ? 0 : OOB;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_ptr)(st + (wave + 8 * q) * 1024), 16, (offA[q] | out) + k0, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_ptr)(st + Tl::ABYTES + (wave + 8 * q) * 1024), 16, (offB[q] | out) + k0, 0, 0, 0);
+        }
+    };
+    // scales, in even stages: wave 0 A's, wave 1 B's
+    const unsigned char* const sbase = wave == 0 ? p.sa + m0 : p.sb + n0;
+    const long spitch = wave == 0 ? p.lda_s : p.ldb_s;
+    const uint32_t sbytes = (uint32_t)(((wave == 0 ? rowsA : rowsB) + 3) & ~3);
+    auto issue_scales = [&](int h, unsigned char* st) {
+        if (wave < 2) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(sbase + (long)(h >> 1) * spitch), 0, h < nh ? sbytes : 0u, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr)(st + 2 * Tl::ABYTES + wave * 256), 4, lane * 4, 0, 0, 0);
+        }
+    };
+    const int wm = wave >> 2, wn = wave & 3, group = wave >> 2, sw = (lr >> 2) & 3;
+    const int c0 = ((hi * 2) ^ sw) << 4, c1 = ((hi * 2 + 1) ^ sw) << 4;
+    f32x16 acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    i32x8 x[TM], w[TN];
+    int xs[TM], ws[TN];
+    auto meet = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // the two stages behind the next one may be in flight: 4 loads each, and the scales of the even one in their two waves
+    auto landed = [&]() {
+        if (wave < 2) __builtin_amdgcn_s_waitcnt(loads_left(9));
+        else __builtin_amdgcn_s_waitcnt(loads_left(8));
+        asm volatile("" ::: "memory");
+    };
+    auto fetch = [&](auto even, int h, const unsigned char* __restrict__ st, unsigned char* __restrict__ next) {
+        if constexpr (decltype(even)::value) {
+#pragma unroll
+            for (int j = 0; j < TM; ++j) xs[j] = st[2 * Tl::ABYTES + (wm * TM + j) * 32 + lr];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) ws[i] = st[2 * Tl::ABYTES + 256 + (wn * TN + i) * 32 + lr];
+        }
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const unsigned char* row = st + ((wm * TM + j) * 32 + lr) * 64;
+            const int4 u = *reinterpret_cast<const int4*>(row + c0), v = *reinterpret_cast<const int4*>(row + c1);
+            x[j] = i32x8{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        }
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            const unsigned char* row = st + Tl::ABYTES + ((wn * TN + i) * 32 + lr) * 64;
+            const int4 u = *reinterpret_cast<const int4*>(row + c0), v = *reinterpret_cast<const int4*>(row + c1);
+            w[i] = i32x8{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        }
+        issue(h + 3, next);
+        if constexpr (!decltype(even)::value) issue_scales(h + 3, next);
+    };
+    auto half = [&](auto grp, auto even, int h) {
+        fetch(even, h, q8_sm + (h & 3) * Tl::STAGE, q8_sm + ((h + 3) & 3) * Tl::STAGE);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (decltype(grp)::value) landed();
+        meet();
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[i], x[j], acc[i][j], 0, 0, 0, ws[i], 0, xs[j]);
+        __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) asm volatile("" : "+v"(acc[i][j]));   // (here, not behind the next branch)
+        if constexpr (!decltype(grp)::value) landed();
+        meet();
+    };
+    auto run = [&](auto grp) {
+        for (int h = 0; h < nh; h += 2) {
+            half(grp, std::true_type{}, h);
+            if (h + 1 < nh) half(grp, std::false_type{}, h + 1);
+        }
+    };
+    issue(0, q8_sm), issue_scales(0, q8_sm);
+    issue(1, q8_sm + Tl::STAGE);
+    issue(2, q8_sm + 2 * Tl::STAGE), issue_scales(2, q8_sm + 2 * Tl::STAGE);
+    landed();
+    meet();
+    if (group) {
+        meet();
+        run(std::true_type{});
+    } else {
+        run(std::false_type{});
+        meet();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (empty loads behind the last stage write LDS as well)
+    __syncthreads();
+    if (p.out32) mm_store<TM, TN, float>(p, acc, q8_sm + wave * Tl::OUT, m0 + wm * TM * 32, n0 + wn * TN * 32, lane);
+    else mm_store<TM, TN, uint16_t>(p, acc, q8_sm + wave * Tl::OUT, m0 + wm * TM * 32, n0 + wn * TN * 32, lane);
+}
+__global__ __launch_bounds__(256, 2) void q8_mm_128x128(MmParams p) { q8_mm_body<128, 128, 2, 2, 2>(p); }
+__global__ __launch_bounds__(256, 2) void q8_mm_128x32(MmParams p) { q8_mm_body<128, 32, 4, 1, 3>(p); }
 
 // The product for short k (K <= 512) and many rows -- every 1x1 convolution of the network: bound by HBM (256 -> 256 at 1/8 resolution: 201 MB
 // for 34 GFLOP), so rows are streamed once through persistent blocks that keep their weights in REGISTERS.
@@ -744,35 +947,71 @@ Q8_STREAM(1_128, 1, 1, 4, true) Q8_STREAM(2_128, 2, 1, 4, true) Q8_STREAM(4_128,
 Q8_STREAM(1_256, 1, 2, 4, true) Q8_STREAM(2_256, 2, 2, 4, true) Q8_STREAM(4_256, 4, 1, 8, true)         // (<4, 2, 4>: 128 registers for the weights alone, spills)
 #undef Q8_STREAM
 
-// Few tiles: a block per 32 x 32 outputs, the blocks of k dealt to its four waves, operands straight from memory into registers, the four
-// partial tiles added through LDS in wave order.
+// Few tiles: a block per 32 x 32 outputs, the blocks of k dealt to its four waves, each with LDS stages of its own (rows travel by LDS-DMA,
+// the next block's while one is multiplied; no barrier), the four partial tiles added through LDS in wave order.
+constexpr int SMALL_STAGE = 64 * BLK;     // 32 rows of A, 32 of B
 __global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
-    __shared__ float part[4][32][33];
+    extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];   // [stages][4 waves][SMALL_STAGE], later [4][32][33] floats
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 31, hi = lane >> 5;
     const int n0 = blockIdx.x * 32;
     const long m0 = (long)blockIdx.y * 32;
-    const bool am = m0 + lr < p.M, bn = n0 + lr < p.N;
-    const unsigned char* arow = p.a + (am ? m0 + lr : 0) * p.ld;
-    const unsigned char* brow = p.b + (long)(bn ? n0 + lr : 0) * p.ld;
+    const int rowsA = (int)(p.M - m0 < 32 ? p.M - m0 : 32), rowsB = p.N - n0 < 32 ? p.N - n0 : 32;
+    const __amdgpu_buffer_rsrc_t rsA = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.a + m0 * p.ld), 0, (uint32_t)(rowsA * p.ld), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rsB = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p.b + (long)n0 * p.ld), 0, (uint32_t)(rowsB * p.ld), 0x00020000);
+    int off[4], col[2];                   // 16-byte chunk c of row r at c ^ ((r >> 1) & 7); a piece has 8 rows
+#pragma unroll
+    for (int q = 0; q < 4; ++q) off[q] = (q * 8 + (lane >> 3)) * p.ld;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) col[q] = ((lane & 7) ^ ((q * 4 + (lane >> 4)) & 7)) << 4;
+    // rows behind the last one lie behind the descriptor; columns behind the row's end are sent there
+    auto issue = [&](int kb, unsigned char* st) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int c = kb * BLK + col[q & 1], at = c < p.ld ? off[q] + c : OOB;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, (lds_ptr)(st + q * 1024), 16, at, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_ptr)(st + (4 + q) * 1024), 16, at, 0, 0, 0);
+        }
+    };
+    const bool am = lr < rowsA, bn = lr < rowsB;
+    const unsigned char *as = p.sa + m0 + (am ? lr : 0), *bs = p.sb + n0 + (bn ? lr : 0);
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-    for (int kb = wave; kb < p.nb; kb += 4) {
-        const int xs = am ? p.sa[(long)kb * p.lda_s + m0 + lr] : 0, ws = bn ? p.sb[(long)kb * p.ldb_s + n0 + lr] : 0;
-        int4 u[4], v[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int c = kb * BLK + (q >> 1) * 64 + hi * 32 + (q & 1) * 16;
-            u[q] = (am && c < p.ld) ? *reinterpret_cast<const int4*>(arow + c) : make_int4(0, 0, 0, 0);
-            v[q] = (bn && c < p.ld) ? *reinterpret_cast<const int4*>(brow + c) : make_int4(0, 0, 0, 0);
-        }
+    const int sw = (lr >> 1) & 7;
+    auto multiply = [&](const unsigned char* __restrict__ st, int xs, int ws) {
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            const i32x8 x = {u[2 * kk].x, u[2 * kk].y, u[2 * kk].z, u[2 * kk].w, u[2 * kk + 1].x, u[2 * kk + 1].y, u[2 * kk + 1].z, u[2 * kk + 1].w};
-            const i32x8 w = {v[2 * kk].x, v[2 * kk].y, v[2 * kk].z, v[2 * kk].w, v[2 * kk + 1].x, v[2 * kk + 1].y, v[2 * kk + 1].z, v[2 * kk + 1].w};
-            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, acc, 0, 0, 0, ws, 0, xs);
+            const int c0 = ((kk * 4 + hi * 2) ^ sw) << 4, c1 = ((kk * 4 + hi * 2 + 1) ^ sw) << 4;
+            const int4 u = *reinterpret_cast<const int4*>(st + lr * BLK + c0), v = *reinterpret_cast<const int4*>(st + lr * BLK + c1);
+            const int4 g = *reinterpret_cast<const int4*>(st + (32 + lr) * BLK + c0), h = *reinterpret_cast<const int4*>(st + (32 + lr) * BLK + c1);
+            acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(i32x8{g.x, g.y, g.z, g.w, h.x, h.y, h.z, h.w}, i32x8{u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w},
+                                                                  acc, 0, 0, 0, ws, 0, xs);
         }
+    };
+    unsigned char* const mine = q8_sm + wave * SMALL_STAGE;
+    int at = 0, xs = 0, ws = 0;
+    if (wave < p.nb) {
+        xs = as[(long)wave * p.lda_s], ws = bs[(long)wave * p.ldb_s];
+        issue(wave, mine);
     }
+    for (int kb = wave; kb < p.nb; kb += 4) {
+        const unsigned char* st = mine + at * 4 * SMALL_STAGE;
+        int xn = 0, wn = 0;
+        if (kb + 4 < p.nb) {
+            at ^= 1;
+            xn = as[(long)(kb + 4) * p.lda_s], wn = bs[(long)(kb + 4) * p.ldb_s];
+            __builtin_amdgcn_sched_barrier(0);
+            issue(kb + 4, mine + at * 4 * SMALL_STAGE);
+            asm volatile("s_waitcnt vmcnt(10)" ::: "memory");   // (10: what was issued just now)
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        multiply(st, am ? xs : 0, bn ? ws : 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // read: the stage may be loaded again
+        xs = xn, ws = wn;
+    }
+    __syncthreads();
+    float(*part)[32][33] = reinterpret_cast<float(*)[32][33]>(q8_sm);
 #pragma unroll
     for (int e = 0; e < 16; ++e) part[wave][lr][8 * (e >> 2) + 4 * hi + (e & 3)] = acc[e];
     __syncthreads();
@@ -1259,8 +1498,8 @@ inline int done() { return hipGetLastError() == hipSuccess ? MGN_OK : MGN_ELAUNC
 constexpr long MAX_ROWS = 0x7fffff00L;    // rows are counted in 32 bits (padded to 16), offsets in 64
 constexpr int MAX_COLS = 1 << 20;
 
-// The streaming product; MGN_ENOTSUP where another kernel is meant.  src_kind as SRC.
-int launch_stream(StreamParams p, int src_kind, hipStream_t s) {
+// The streaming product; MGN_ENOTSUP where another kernel is meant.  src_kind as SRC; `least` tiles for each block, or that other kernel.
+int launch_stream(StreamParams p, int src_kind, int least, hipStream_t s) {
     if (p.K > 512 || p.lds * 4 > 0x7fffffffL) return MGN_ENOTSUP;
     const bool vec = !p.out32 && p.N % 8 == 0 && p.ldo % 8 == 0 && p.ldo <= MAX_COLS && aligned(p.out, 16);
     if (!vec && p.N > 32) return MGN_ENOTSUP;
@@ -1269,7 +1508,7 @@ int launch_stream(StreamParams p, int src_kind, hipStream_t s) {
     const int th = KB == 4 && shape == 3 ? 512 : 256, BM = 128 / KB * (src_kind == 0 ? 2 : 1) * (th / 256), groups = (p.N + chans - 1) / chans;
     p.ntiles = (int)(((long)p.M + BM - 1) / BM);
     int gx = (512 * 256 / th) / groups & ~7;   // two blocks a CU (one of 512 threads)
-    if (gx < 8) return MGN_ENOTSUP;
+    if (gx < 8 || p.ntiles < least * gx) return MGN_ENOTSUP;
     gx = p.ntiles < gx ? p.ntiles : gx;
     const int lds = 2 * (BM * KB * BLK + KB * BM) + 1024;
     typedef void (*K)(StreamParams);
@@ -1293,24 +1532,22 @@ int launch_stream(StreamParams p, int src_kind, hipStream_t s) {
     return done();
 }
 
-template <int BM, int BN, int WVM, int WVN>
+template <int BM, int BN, int LDS, int TH>
 int launch_mm(void (*kernel)(MmParams), MmParams p, hipStream_t s) {
-    using Tl = MmTile<BM, BN, WVM, WVN>;
     p.mt = (int)(((long)p.M + BM - 1) / BM);
     p.nt = (p.N + BN - 1) / BN;
-    p.group = p.mt < 16 ? 1 : (p.mt >= 32 ? 4 : p.mt / 8);
-    const long blocks = ((long)p.mt + 8 * p.group - 1) / (8 * p.group) * p.group * p.nt * 8;
+    const long blocks = ((long)p.mt * p.nt + 7) / 8 * 8;
     if (blocks > 0x7fffffffL) return MGN_EINVAL;
-    if (Tl::LDS > 65536) {
+    if (LDS > 65536) {
         static bool ready[64] = {};
         int dev = 0;
         if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return MGN_ELAUNCH;
         if (!ready[dev]) {
-            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, Tl::LDS) != hipSuccess) return MGN_ELAUNCH;
+            if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return MGN_ELAUNCH;
             ready[dev] = true;
         }
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * WVM * WVN), Tl::LDS, s, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(TH), LDS, s, p);
     return done();
 }
 
@@ -1389,27 +1626,30 @@ int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const vo
     if (!a || !a_scales || !b || !b_scales || !out || !aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 16) || !aligned(b_scales, 16) ||
         !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;
     MmParams p = {(const unsigned char*)a, (const unsigned char*)a_scales, (const unsigned char*)b, (const unsigned char*)b_scales, bias, out,
-                  (int)M, N, K, nblocks(K), code_ld(K), scale_ld(M), scale_ld(N), ldo, make_act(act, slope), out_f32, 0, 0, 0, 1};
-    p.vec = ldo % 4 == 0 && aligned(out, out_f32 ? 16 : 8);
+                  (int)M, N, K, nblocks(K), code_ld(K), scale_ld(M), scale_ld(N), ldo, make_act(act, slope), out_f32, 0, 0};
     hipStream_t s = (hipStream_t)stream_;
     auto tiles = [&](int BM, int BN) { return ((M + BM - 1) / BM) * ((N + BN - 1) / BN); };
-    if (M <= 64 || tiles(128, 128) < 64) {
-        const long gy = (M + 31) / 32;
-        if (gy > 65535) return MGN_EINVAL;
-        hipLaunchKernelGGL(q8_mm_small, dim3((unsigned)((N + 31) / 32), (unsigned)gy), dim3(TPB), 0, s, p);
+    // Up to some 1400 tiles of 32 x 32 the chip is better filled by those, k split over their waves, than by larger ones: 256 x 4096 x 4096
+    // (1024 tiles) 15.2 us against 21.9 with 128 x 128, 459 x 2932 x 3872 (1380) 22.9 against 22.6, 1500^3 (2209) 16.3 against 12.8
+    const long gy = (M + 31) / 32;
+    if ((M <= 64 || tiles(32, 32) <= 1400) && gy <= 65535) {
+        const int lds = p.nb > 4 ? 8 * SMALL_STAGE : 4 * SMALL_STAGE;   // (a wave with one block of k needs one stage)
+        hipLaunchKernelGGL(q8_mm_small, dim3((unsigned)((N + 31) / 32), (unsigned)gy), dim3(TPB), lds, s, p);
         return done();
     }
     if (K <= 512) {
+        // more than 128 channels: only with two tiles or more for each persistent block (16000 x 512 x 512, one tile a block: 13.5 us against
+        // 10.9 with 128 x 128 tiles; 256000 x 512 x 512: 106 against 133)
         StreamParams q = {p.a, p.sa, nullptr, nullptr, p.b, p.sb, bias, out, (int)M, K, N, p.ld, p.ld, p.ld, 0, p.lda_s, p.ldb_s, ldo, make_act(act, slope), out_f32};
-        const int rc = launch_stream(q, 0, s);
+        const int rc = launch_stream(q, 0, N > 128 ? 2 : 0, s);
         if (rc != MGN_ENOTSUP) return rc;
     }
-    if (N <= 32) return launch_mm<128, 32, 4, 1>(q8_mm_128x32, p, s);
-    // 256 x 256 tiles run at 2.4 PFLOP/s and 128 x 128 tiles at 1.8 where they fill the chip (256 and 512 blocks at a time): the better of the
-    // two rates after the share of idle slots in the last round
-    auto share = [](long t, long slots) { return (double)t / (double)((t + slots - 1) / slots * slots); };
-    if (N > 128 && share(tiles(256, 256), 256) >= 0.75 * share(tiles(128, 128), 512)) return launch_mm<256, 256, 2, 4>(q8_mm_256x256, p, s);
-    return launch_mm<128, 128, 2, 2>(q8_mm_128x128, p, s);
+    if (N <= 32) return launch_mm<128, 32, MmTile<128, 32, 4, 1, 3>::LDS, 256>(q8_mm_128x32, p, s);
+    // 256 blocks of 256 x 256 fill the chip, 512 of 128 x 128, the former 1.16 times as fast (8192^3: 421 us against 490): the better of the two
+    // by the share of a whole number of rounds that is used
+    auto used = [&](int B, long slots) { const long t = tiles(B, B); return (double)M * N / ((double)((t + slots - 1) / slots * slots) * B * B); };
+    if (N > 128 && 1.16 * used(256, 256) >= used(128, 512)) return launch_mm<256, 256, Mm256::LDS, 512>(q8_mm_256x256, p, s);
+    return launch_mm<128, 128, MmTile<128, 128, 2, 2, 2>::LDS, 256>(q8_mm_128x128, p, s);
 }
 
 int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* codes, void* scales, const void* b, const void* b_scales, int N,
@@ -1421,7 +1661,7 @@ int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* co
     if (K > 512 || K % 8 != 0 || ldx % 8 != 0 || !aligned(x, 16)) return MGN_ENOTSUP;
     StreamParams p = {(const unsigned char*)x, nullptr, (unsigned char*)codes, (unsigned char*)scales, (const unsigned char*)b, (const unsigned char*)b_scales, bias, out,
                       (int)M, K, N, (int)ldx, code_ld(K), code_ld(K), 0, scale_ld(M), scale_ld(N), ldo, make_act(act, slope), out_f32};
-    return launch_stream(p, codes ? 2 : 1, (hipStream_t)stream_);
+    return launch_stream(p, codes ? 2 : 1, 0, (hipStream_t)stream_);
 }
 
 #ifndef MGN_F16
