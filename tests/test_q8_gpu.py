@@ -217,6 +217,36 @@ def test_product(M, N, K, dtype):
     check_product(a, b, bias, "leaky_relu" if N % 2 else "relu", 0.01, F32 if M % 2 else dtype)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 19, 3000), (33, 1000, 4096), (100, 77, 1400), (1000, 40, 513), (2300, 1030, 1000), (4097, 515, 530), (16380, 1021, 130),
+                                   (16380, 1021, 700), (8190, 2045, 64), (60000, 21, 530), (50000, 32, 1100), (16000, 512, 512), (3001, 517, 257)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_product_of_every_tile(M, N, K, dtype):
+    """sizes that leave tiles, half steps of k and rows of the result ragged, for each of the product's kernels"""
+    a, b = rand((M, K), dtype, M + N), rand((N, K), F32, N + K, 0.3) / math.sqrt(K)
+    check_product(a, b, rand((N,), F32, 2, 0.0), "leaky_relu", 0.25, dtype)
+    check_product(a, b, None, "none", 0.01, F32)
+
+
+@pytest.mark.parametrize("M,N,K,ldo,at", [(40, 37, 300, 41, 3), (70, 33, 2000, 33, 1), (2300, 1030, 700, 1035, 5), (16380, 1021, 130, 1021, 7), (60000, 21, 530, 24, 1),
+                                          (60000, 21, 200, 23, 9), (50000, 40, 256, 48, 8), (50000, 200, 256, 208, 8), (50000, 200, 256, 201, 1)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_product_leaves_what_lies_around_it(M, N, K, ldo, at, dtype):
+    """rows of any pitch from any element on: nothing before, between or behind them is written"""
+    from mgnet_amd import _C
+    o = ops()
+    qa, qb = o.q8_pack(rand((M, K), BF, 1)), o.q8_pack(rand((N, K), F32, 2, 0.0), tile=True)
+    whole = torch.full((at + M * ldo + 32,), 7.0, dtype=dtype, device="cuda")
+    out = whole[at:at + M * ldo].view(M, ldo)
+    pa, pb = qa.buf.data_ptr(), qb.buf.data_ptr()
+    _C.check(_C._fn("mgn_q8_matmul", out)(pa, pa + _C.q8_code_bytes(M, K), M, pb, pb + _C.q8_code_bytes(N, K), N, K, None, 0, 0.0, out.data_ptr(),
+                                          int(dtype == F32), ldo, _C._stream()), "mgn_q8_matmul")
+    ref = o.q8_matmul(qa, qb, out_dtype=dtype)
+    close = (out[:, :N].double() - ref.double()).abs() <= 2.0 ** -7 * ref.double().abs() + K * 2.0 ** -12 * float(ref.abs().max())   # (another kernel's order)
+    assert bool(close.all())
+    out[:, :N] = 7.0
+    assert bool((whole == 7.0).all())
+
+
 def test_product_scales_over_the_whole_range():
     """blocks whose exponents differ by hundreds of binades, and NaN that stay in their rows"""
     o = ops()
