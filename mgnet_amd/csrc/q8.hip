@@ -161,27 +161,49 @@ __device__ __forceinline__ long row_offset(const RowMap& m, int r) {
     return (long)n * m.sn + (long)h * m.sh + (long)w * m.sw;
 }
 
+// 16, 8 and 4 bytes at any address that suits an element: global loads and stores need no more, so that rows of any pitch move alike
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32_any __attribute__((aligned(2)));
+
 template <typename T> struct Src;
 template <> struct Src<float> {
-    struct Raw { float4 a, b; };
+    struct Raw { u32x4_any a, b; };
     static constexpr float TOP = TOP32;
-    __device__ static Raw zero() { return Raw{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)}; }
-    __device__ static Raw load(const float* p) { return Raw{reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]}; }
+    __device__ static Raw zero() { return Raw{}; }
     __device__ static float one(const float* p) { return *p; }
+    __device__ static Raw load(const float* p) { return Raw{*reinterpret_cast<const u32x4_any*>(p), *reinterpret_cast<const u32x4_any*>(p + 4)}; }
+    __device__ static Raw tail(const float* p, int t) {   // t < 8 values, zeros behind them
+        Raw r{};
+        u32x4_any v = {0, 0, 0, 0};
+        if (t & 4) { r.a = *reinterpret_cast<const u32x4_any*>(p); p += 4; }
+        if (t & 2) { const u32x2_any w = *reinterpret_cast<const u32x2_any*>(p); v.x = w.x; v.y = w.y; p += 2; }
+        if (t & 1) { if (t & 2) v.z = __float_as_uint(*p); else v.x = __float_as_uint(*p); }
+        if (t & 4) r.b = v; else r.a = v;
+        return r;
+    }
     __device__ static void get(const Raw& r, float (&v)[8]) {
-        v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; v[4] = r.b.x; v[5] = r.b.y; v[6] = r.b.z; v[7] = r.b.w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { v[k] = __uint_as_float(r.a[k]); v[k + 4] = __uint_as_float(r.b[k]); }
     }
 };
 template <> struct Src<uint16_t> {
     struct Raw { uint4 a; };
     static constexpr float TOP = TOP16;
     __device__ static Raw zero() { return Raw{make_uint4(0, 0, 0, 0)}; }
-    __device__ static Raw load(const uint16_t* p) { return Raw{*reinterpret_cast<const uint4*>(p)}; }
     __device__ static float one(const uint16_t* p) { return mgn_h2f(*p); }
-    __device__ static void get(const Raw& r, float (&v)[8]) { unpack8(r.a, v); }
+    __device__ static Raw load(const uint16_t* p) { const u32x4_any v = *reinterpret_cast<const u32x4_any*>(p); return Raw{make_uint4(v.x, v.y, v.z, v.w)}; }
+    __device__ static Raw tail(const uint16_t* p, int t) {
+        u32x2_any lo = {0, 0};
+        uint32_t x = 0, y = 0;
+        if (t & 4) { lo = *reinterpret_cast<const u32x2_any*>(p); p += 4; }
+        if (t & 2) { x = *reinterpret_cast<const u32_any*>(p); p += 2; }
+        if (t & 1) { if (t & 2) y = *p; else x = *p; }
+        return (t & 4) ? Raw{make_uint4(lo.x, lo.y, x, y)} : Raw{make_uint4(x, y, 0, 0)};
+    }
 };
 
-template <typename T, int LPB, bool VEC>
+template <typename T, int LPB>
 __global__ __launch_bounds__(TPB) void q8_pack(const T* __restrict__ x, RowMap map, int M, int C, int nb, int ldc, long lds,
                                                unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
     const long gid = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
@@ -191,35 +213,26 @@ __global__ __launch_bounds__(TPB) void q8_pack(const T* __restrict__ x, RowMap m
     if (r0l >= M) return;                 // (whole groups leave together: the DPP steps below stay inside one group)
     const int r0 = (int)r0l, c0 = kb * BLK + l * 8;
     uint32_t sb[RPG];
-    auto finish = [&](int j, const float (&f)[8]) {
-        const uint32_t s = scale_of(group_max<LPB>(amax8(f, Src<T>::TOP)));
-        sb[j] = s;
-        if (r0 + j < M && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = encode8(f, inv_scale(s), Src<T>::TOP);
-    };
-    if (VEC) {                            // C % 8 == 0 and 16-byte aligned rows
-        typename Src<T>::Raw q[RPG];
+    typename Src<T>::Raw q[RPG];
+    if (c0 + 8 <= C || c0 >= C) {
 #pragma unroll
         for (int j = 0; j < RPG; ++j) q[j] = (r0 + j < M && c0 < C) ? Src<T>::load(x + row_offset(map, r0 + j) + c0) : Src<T>::zero();
-#pragma unroll
-        for (int j = 0; j < RPG; ++j) {
-            if constexpr (sizeof(T) == 2) {
-                const uint2 e = quantize8<LPB>(q[j].a, sb[j]);
-                if (r0 + j < M && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = e;
-            } else {
-                float f[8];
-                Src<T>::get(q[j], f);
-                finish(j, f);
-            }
-        }
     } else {
 #pragma unroll
-        for (int j = 0; j < RPG; ++j) {
-            float f[8];
-            const T* p = x + (r0 + j < M ? row_offset(map, r0 + j) : 0) + c0;
+        for (int j = 0; j < RPG; ++j) q[j] = r0 + j < M ? Src<T>::tail(x + row_offset(map, r0 + j) + c0, C - c0) : Src<T>::zero();
+    }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = (r0 + j < M && c0 + k < C) ? Src<T>::one(p + k) : 0.f;
-            finish(j, f);
+    for (int j = 0; j < RPG; ++j) {
+        uint2 e;
+        if constexpr (sizeof(T) == 2) {
+            e = quantize8<LPB>(q[j].a, sb[j]);
+        } else {
+            float f[8];
+            Src<T>::get(q[j], f);
+            sb[j] = scale_of(group_max<LPB>(amax8(f, Src<T>::TOP)));
+            e = encode8(f, inv_scale(sb[j]), Src<T>::TOP);
         }
+        if (r0 + j < M && c0 < ldc) *reinterpret_cast<uint2*>(codes + (long)(r0 + j) * ldc + c0) = e;
     }
     if (l == 0) {                         // lds is a multiple of 16: eight bytes from a row that is a multiple of 8 stay inside it
         const uint2 w = make_uint2(sb[0] | (sb[1] << 8) | (sb[2] << 16) | (sb[3] << 24), sb[4] | (sb[5] << 8) | (sb[6] << 16) | (sb[7] << 24));
@@ -227,8 +240,10 @@ __global__ __launch_bounds__(TPB) void q8_pack(const T* __restrict__ x, RowMap m
     }
 }
 
-// codes, scales -> x^ [M][C] (rows of C contiguous values); the mirror image of q8_pack
-template <typename T, int LPB, bool VEC>
+// codes, scales -> x^ [M][C] (rows of C contiguous values); the mirror image of q8_pack.  A lane writes 16 bytes at a time, neighbours side by
+// side: of 16-bit values its 8 channels, of 32-bit ones 4 channels in either half of the block (60M values: 62 us against 75
+// with 8 in a row, whose two stores lie 32 bytes apart)
+template <typename T, int LPB>
 __global__ __launch_bounds__(TPB) void q8_unpack(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, int M, int C,
                                                  int nb, int ldc, long lds, T* __restrict__ y) {
     const long gid = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
@@ -236,33 +251,46 @@ __global__ __launch_bounds__(TPB) void q8_unpack(const unsigned char* __restrict
     const int kb = (int)(gid % nb);
     const long r0l = gid / nb * RPG;
     if (r0l >= M) return;
-    const int r0 = (int)r0l, c0 = kb * BLK + l * 8;
+    constexpr bool HALF = sizeof(T) == 2;
+    const int r0 = (int)r0l, c0 = kb * BLK + l * (HALF ? 8 : 4), c1 = c0 + (HALF ? 4 : 4 * LPB);   // two runs of 4 channels
     if (c0 >= C) return;
     const uint2 w = *reinterpret_cast<const uint2*>(scales + kb * lds + r0);
     uint2 q[RPG];
 #pragma unroll
-    for (int j = 0; j < RPG; ++j) q[j] = r0 + j < M ? *reinterpret_cast<const uint2*>(codes + (long)(r0 + j) * ldc + c0) : make_uint2(0, 0);
+    for (int j = 0; j < RPG; ++j) {
+        const unsigned char* p = codes + (long)(r0 + j) * ldc;
+        if (r0 + j >= M) q[j] = make_uint2(0, 0);
+        else if (HALF) q[j] = *reinterpret_cast<const uint2*>(p + c0);
+        else q[j] = make_uint2(*reinterpret_cast<const uint32_t*>(p + c0), c1 < C ? *reinterpret_cast<const uint32_t*>(p + c1) : 0);
+    }
 #pragma unroll
     for (int j = 0; j < RPG; ++j) {
         if (r0 + j >= M) break;
         float v[8];
         decode8(q[j], pow2(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), v);
-        T* p = y + (long)(r0 + j) * C + c0;
-        if constexpr (sizeof(T) == 2) {
+        T* row = y + (long)(r0 + j) * C;
+        if constexpr (HALF) {
             const uint4 o = pack8(v);
-            if (VEC) *reinterpret_cast<uint4*>(p) = o;
-            else {
-                const uint32_t u[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-                for (int k = 0; k < 8; ++k) if (c0 + k < C) p[k] = (T)(u[k >> 1] >> (16 * (k & 1)));
+            T* p = row + c0;
+            if (c0 + 8 <= C) {
+                *reinterpret_cast<u32x4_any*>(p) = u32x4_any{o.x, o.y, o.z, o.w};
+            } else {
+                const int t = C - c0;
+                uint32_t a = o.x, b = o.y;
+                if (t & 4) { *reinterpret_cast<u32x2_any*>(p) = u32x2_any{a, b}; a = o.z; b = o.w; p += 4; }
+                if (t & 2) { *reinterpret_cast<u32_any*>(p) = a; a = b; p += 2; }
+                if (t & 1) *p = (T)a;
             }
         } else {
-            if (VEC) {
-                reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) if (c0 + k < C) p[k] = v[k];
+            for (int h = 0; h < 2; ++h) {
+                const int c = h ? c1 : c0;
+                if (c + 4 <= C) {
+                    *reinterpret_cast<u32x4_any*>(row + c) = u32x4_any{__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])};
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) if (c + k < C) row[c + k] = v[4 * h + k];
+                }
             }
         }
     }
@@ -371,10 +399,6 @@ struct MmParams {
     int mt, nt;
 };
 MGN_PLAN_RO(MmParams, MGN_RO(a) MGN_RO(sa) MGN_RO(b) MGN_RO(sb) MGN_RO(bias))
-
-// 16 and 8 bytes at any address that suits an element: global stores need no more
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 // four consecutive n of row m
 template <typename P>
@@ -1576,15 +1600,12 @@ int MGN_SYM(mgn_q8_pack)(const void* x, int dtype, long M, int C, long sn, long 
     RowMap map = {sn, sh, sw, H, W, 0};
     map.flat = (H == 1 || sh == (long)W * sw) && (images == 1 || sn == (long)H * W * sw);
     const int nb = nblocks(C), ldc = code_ld(C), lpb = lanes_for(C);
-    const int el = dtype ? 8 : 4;         // elements in 16 bytes
-    const bool vec = C % 8 == 0 && aligned(x, 16) && sw % el == 0 && (map.flat || (sh % el == 0 && sn % el == 0));
     const long groups = (M + RPG - 1) / RPG * nb, blocks = (groups * lpb + TPB - 1) / TPB;
     if (blocks > 0x7fffffffL) return MGN_EINVAL;
     hipStream_t s = (hipStream_t)stream_;
-#define Q8_PACK(T, V) Q8_LANES(C, (hipLaunchKernelGGL((q8_pack<T, LPB, V>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const T*)x, map, (int)M, C, nb, ldc, \
-                                                      scale_ld(M), (unsigned char*)codes, (unsigned char*)scales)))
-    if (dtype) { if (vec) Q8_PACK(uint16_t, true); else Q8_PACK(uint16_t, false); }
-    else { if (vec) Q8_PACK(float, true); else Q8_PACK(float, false); }
+#define Q8_PACK(T) Q8_LANES(C, (hipLaunchKernelGGL((q8_pack<T, LPB>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const T*)x, map, (int)M, C, nb, ldc, \
+                                                   scale_ld(M), (unsigned char*)codes, (unsigned char*)scales)))
+    if (dtype) Q8_PACK(uint16_t); else Q8_PACK(float);
 #undef Q8_PACK
     return done();
 }
@@ -1594,14 +1615,12 @@ int MGN_SYM(mgn_q8_unpack)(const void* codes, const void* scales, long M, int C,
     if (M == 0) return MGN_OK;
     if (!codes || !scales || !y || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(y, dtype ? 2 : 4)) return MGN_EINVAL;
     const int nb = nblocks(C), ldc = code_ld(C), lpb = lanes_for(C);
-    const bool vec = C % 8 == 0 && aligned(y, 16);
     const long groups = (M + RPG - 1) / RPG * nb, blocks = (groups * lpb + TPB - 1) / TPB;
     if (blocks > 0x7fffffffL) return MGN_EINVAL;
     hipStream_t s = (hipStream_t)stream_;
-#define Q8_UNPACK(T, V) Q8_LANES(C, (hipLaunchKernelGGL((q8_unpack<T, LPB, V>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const unsigned char*)codes, \
-                                                        (const unsigned char*)scales, (int)M, C, nb, ldc, scale_ld(M), (T*)y)))
-    if (dtype) { if (vec) Q8_UNPACK(uint16_t, true); else Q8_UNPACK(uint16_t, false); }
-    else { if (vec) Q8_UNPACK(float, true); else Q8_UNPACK(float, false); }
+#define Q8_UNPACK(T) Q8_LANES(C, (hipLaunchKernelGGL((q8_unpack<T, LPB>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const unsigned char*)codes, \
+                                                     (const unsigned char*)scales, (int)M, C, nb, ldc, scale_ld(M), (T*)y)))
+    if (dtype) Q8_UNPACK(uint16_t); else Q8_UNPACK(float);
 #undef Q8_UNPACK
     return done();
 }
