@@ -1686,12 +1686,16 @@ int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* co
 #ifndef MGN_F16
 static size_t wgrad_floats(int N, int K) { return ((size_t)N * K + N + 3) & ~(size_t)3; }
 // Row ranges: the power of two that minimises (steps a CU goes through) + (writing and reading the partial results), with the step at
-// 0.5 us and the traffic at 5 TB/s, both as measured.  262144 x 256 x 256: 128; 16384 x 256 x 512: 32.
+// 0.5 us and the traffic at 5 TB/s, both as measured, among those whose ranges a 32-bit buffer descriptor reaches (offsets run up to four
+// steps past the range); 0 if none does.  262144 x 256 x 256: 128; 16384 x 256 x 512: 32.
+static long wgrad_rows(long M, int splits) { return ((M + splits - 1) / splits + WG_ROWS - 1) / WG_ROWS * WG_ROWS; }
+static bool wgrad_reach(long rows, long ldy, int K) { return (rows + 4 * WG_ROWS) * (ldy * 2 > code_ld(K) ? ldy * 2 : code_ld(K)) <= 0x7fffffffL; }
 static int wgrad_splits(long M, int N, int K) {
     const double tiles = (double)nblocks(N) * nblocks(K), bytes = 8.0 * (double)wgrad_floats(N, K);
     double best = 1e300;
-    int z = 1;
+    int z = 0;
     for (int c = 1; c <= 512 && (c == 1 || (long)c * WG_ROWS <= M * 2); c *= 2) {
+        if (!wgrad_reach(wgrad_rows(M, c), (N + 7) & ~7, K)) continue;
         const double steps = (double)((M + (long)c * WG_ROWS - 1) / ((long)c * WG_ROWS)), rounds = (double)((long)((tiles * c + 511) / 512));
         const double t = steps * rounds * 0.5 + c * bytes / 5e6;
         if (t < best) { best = t; z = c; }
@@ -1700,7 +1704,9 @@ static int wgrad_splits(long M, int N, int K) {
 }
 int mgn_q8_wgrad_workspace_bytes(long M, int N, int K, size_t* bytes) {
     if (M < 1 || M > MAX_ROWS || N < 1 || K < 1 || N > 65536 || K > 65536 || !bytes) return MGN_EINVAL;
-    *bytes = sizeof(float) * (size_t)wgrad_splits(M, N, K) * wgrad_floats(N, K);
+    const int splits = wgrad_splits(M, N, K);
+    if (splits == 0) return MGN_EINVAL;
+    *bytes = sizeof(float) * (size_t)splits * wgrad_floats(N, K);
     return MGN_OK;
 }
 #endif
@@ -1713,9 +1719,8 @@ int MGN_SYM(mgn_q8_wgrad)(const void* dy, long ldy, long M, int N, const void* c
     if (!dy || !codes || !scales || !dw || !ws || !aligned(dy, 16) || !aligned(codes, 16) || ldy < N || ldy % 8 != 0 || ldy > 65536) return MGN_EINVAL;
     if (ws_bytes < need) return MGN_ENOSPC;
     const int zmax = (int)(need / (sizeof(float) * (((size_t)N * K + N + 3) & ~(size_t)3)));
-    // rows per split: whole steps, and a range whose bytes stay inside a 32-bit buffer descriptor
-    long rows = ((M + zmax - 1) / zmax + WG_ROWS - 1) / WG_ROWS * WG_ROWS;
-    if ((rows + 4 * WG_ROWS) * (ldy * 2 > code_ld(K) ? ldy * 2 : code_ld(K)) > 0x7fffffffL) return MGN_EINVAL;   // (offsets run up to four steps past the range)
+    const long rows = ((M + zmax - 1) / zmax + WG_ROWS - 1) / WG_ROWS * WG_ROWS;   // whole steps
+    if ((rows + 4 * WG_ROWS) * (ldy * 2 > code_ld(K) ? ldy * 2 : code_ld(K)) > 0x7fffffffL) return MGN_EINVAL;   // (a row pitch beyond wgrad_splits' own)
     WgradParams8 p = {(const uint16_t*)dy, (const unsigned char*)codes, (const unsigned char*)scales, (float*)ws, (int)M, N, K, (int)ldy, code_ld(K),
                       scale_ld(M), (int)rows, (int)((M + rows - 1) / rows), nblocks(N), nblocks(K)};
     const long blocks = (long)((p.splits + 7) / 8) * 8 * p.ntn * p.ntk;

@@ -71,3 +71,17 @@ def test_python_refuses_cpu_tensors_and_wrong_shapes():
     for f in (lambda: ops.q8_pack(x[0]), lambda: ops.q8_pack([1.0]), lambda: ops.q8_matmul(x, x)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_weight_gradient_ranges():
+    """row ranges stay within 32-bit offsets, or the sizes are refused before anything is computed"""
+    L = lib()
+    a, b = ctypes.c_size_t(), ctypes.c_size_t()
+    for M, N, K in ((66000, 16384, 512), (262144, 4096, 4096), (0x7fffff00, 64, 64), (1 << 27, 19, 320)):
+        assert L.mgn_q8_wgrad_workspace_bytes(M, N, K, ctypes.byref(a)) == 0
+        per = 4 * ((N * K + N + 3) // 4 * 4)
+        assert a.value % per == 0
+        rows = -(-(-(-M // (a.value // per))) // 64) * 64
+        assert (rows + 256) * max(2 * ((N + 7) // 8 * 8), (K + 15) // 16 * 16) <= 0x7fffffff, (M, N, K)
+    assert L.mgn_q8_wgrad_workspace_bytes(0x7fffff00, 65536, 8, ctypes.byref(a)) == -22
+    assert L.mgn_q8_conv1x1_bytes(0x7fffff00, 8, 65536, ctypes.byref(a), ctypes.byref(b)) == -22

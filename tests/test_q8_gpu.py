@@ -353,6 +353,28 @@ def test_conv1x1_partial_gradients_and_empty():
     assert y.shape == (0, 24, 6, 10) and ge.shape == e.shape and not bool(gw.any()) and not bool(gb.any())
 
 
+def test_conv1x1_of_rows_past_32_bits():
+    """2.16 GB of result and of its gradient: a sample of each output against 64 bits"""
+    o = ops()
+    M, C, N = 66000, 512, 16384
+    x, w = rand((1, 1, M, C), BF, 1, 0.3).permute(0, 3, 1, 2).requires_grad_(), (rand((N, C), F32, 2, 0.2) / math.sqrt(C)).view(N, C, 1, 1).requires_grad_()
+    dy = rand((1, 1, M, N), BF, 3, 0.0).permute(0, 3, 1, 2)
+    y = o.conv1x1_q8(x, w, None)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    r = torch.tensor([0, 1, 777, 40000, M - 300, M - 2, M - 1], device="cuda")
+    n = torch.tensor([0, 5, 127, 128, 9000, N - 1], device="cuda")
+    w8, x8 = q8_ref(w.detach().view(N, C), True)[0], q8_ref(rows(x.detach()))[0]
+    ref, S = x8[r] @ w8.t(), x8[r].abs() @ w8.abs().t()
+    got = rows(y.detach())[r].double()
+    assert bool(((got - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * ((C + 2) * 2.0 ** -23 * S + group_tol(x8[r], w8))).all())
+    g = rows(dy)
+    g8 = q8_ref(g[r])[0]
+    ref, S = g8 @ w8, g8.abs() @ w8.abs()
+    assert bool(((rows(dx)[r].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * ((N + 2) * 2.0 ** -23 * S + group_tol(g8, w8.t()))).all())
+    gn = g[:, n].double()
+    assert bool(((dw.view(N, C)[n].double() - gn.t() @ x8).abs() <= (M + 2) * 2.0 ** -23 * (gn.abs().t() @ x8.abs())).all())
+
+
 def test_conv1x1_gradient_against_differences():
     """<dW, V>, <db, v> and <dx, U> against differences of the unquantised convolution in 64 bits: q(.) is off by at most 2^-4 of a value
     (2^-10 * 2^e next to a block's largest, itself under 2^-4 of the term's share here)"""
@@ -465,6 +487,57 @@ def test_block_tail_one_row_and_inference():
     assert bool(((y.float() - ref).abs() <= 2.0 ** -11 * ref + 2.0 ** -20 * (z.abs() + s.float().abs() + 1)).all())
     with pytest.raises(NotImplementedError):
         torch.autograd.grad(o.abn_add_relu_q8(x, norm, s), (x,), g)
+
+
+def test_block_tail_of_two_ranks(monkeypatch):
+    """the exchange of a process group of two, played by one process: each half of the batch sees the whole batch's statistics and sums"""
+    from mgnet_amd import _C
+    from mgnet_amd.modeling import ops as o, q8
+    from mgnet_amd.modeling.layers import InPlaceABNSync
+    n, c, h, w = 4, 72, 9, 7
+    x, s, dy = (rand_map(n, c, h, w, BF, k, 0.3) for k in (1, 2, 3))
+
+    def norm():
+        torch.manual_seed(5)
+        m = InPlaceABNSync(c, momentum=0.01, activation="identity").cuda()
+        with torch.no_grad():
+            m.weight.uniform_(0.5, 1.5)
+            m.bias.uniform_(-0.5, 0.5)
+        return m
+
+    def run(x, s, dy, m):
+        x, s = x.clone(memory_format=torch.channels_last).requires_grad_(), s.clone(memory_format=torch.channels_last).requires_grad_()
+        y = o.abn_add_relu_q8(x, m, s)
+        return (y.detach(),) + torch.autograd.grad(y, (x, s, m.weight, m.bias), dy)
+
+    whole = norm()
+    ref = run(x, s, dy, whole)
+    halves = [tuple(t[k:k + 2] for t in (x, s, dy)) for k in (0, 2)]
+    M = 2 * h * w
+    stats = []
+    for xs, _, _ in halves:
+        part, shift = _C.q8_tail_stats(rows(xs).contiguous(), M, c)
+        stats.append(_C.iabn_from_partials(part, c, M, shift, stats_only=True))
+    monkeypatch.setattr(q8, "_dist_active", lambda group: True)
+    monkeypatch.setattr(q8.dist, "get_world_size", lambda group=None: 2)
+    monkeypatch.setattr(o, "_gather_stats", lambda own, world, group: torch.stack([t.view_as(own) for t in stats]))
+    own = []
+    monkeypatch.setattr(q8, "_allreduce_sums", lambda t, group: own.append(t.clone()) or t)
+    for half in halves:
+        run(*half, norm())
+    monkeypatch.setattr(q8, "_allreduce_sums", lambda t, group: own[0] + own[1])
+    ms = [norm(), norm()]
+    got = [run(*half, m) for half, m in zip(halves, ms)]
+    # fp32 sums in another order (2^-20 of their terms covers 126 of them), then one rounding on either side
+    for k in range(3):
+        a, b = torch.cat([g[k] for g in got]).double(), ref[k].double()
+        assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() + 2.0 ** -16 * (1 + b.abs().max())).all()), k
+    for k in (3, 4):       # of the whole batch's gradient each rank has its share
+        a, b = got[0][k].double() + got[1][k].double(), ref[k].double()
+        assert bool(((a - b).abs() <= 2.0 ** -16 * (1 + b.abs().max())).all()), k
+    for m in ms:
+        for t, r in ((m.running_mean, whole.running_mean), (m.running_var, whole.running_var)):
+            assert bool(((t - r).abs() <= 2.0 ** -18 * (1 + r.abs())).all())
 
 
 def test_nan_and_infinities_reach_the_result():
