@@ -148,7 +148,7 @@ __device__ __forceinline__ uint2 quantize8(const uint4& q, uint32_t& s) {
 // ------------------------------------------------------------------------------------------------------
 // x -> codes, scales.  One pass: a group of LPB lanes owns one block of 8 consecutive rows (8 channels a lane), so a block's maximum is
 // four DPP steps and its eight scales leave in one store; the 8 rows are 8 independent 16-byte loads per lane.  Bound by HBM (3 bytes per
-// 16-bit value).
+// 16-bit value): 262144 x 256 bf16 in 39.6 us, 5.1 TB/s, the rate of a large copy (5.12); back in 30.2 us, the codes still in the last cache.
 // ------------------------------------------------------------------------------------------------------
 struct RowMap {                           // row r of the matrix = pixel (n, h, w) of a map with these strides (elements)
     long sn, sh, sw;
@@ -299,7 +299,8 @@ __global__ __launch_bounds__(TPB) void q8_unpack(const unsigned char* __restrict
 // ------------------------------------------------------------------------------------------------------
 // a weight matrix W [N][K] (any strides) -> codes [N][ldc(K)] + scales [ceil(K/128)][lds(N)], and the same values transposed: codes
 // [K][ldc(N)] + scales [ceil(N/128)][lds(K)] (what the data gradient multiplies by).  A block per 128 x 128 tile; the tile goes through
-// LDS once so that both outputs leave in 16-byte stores.
+// LDS once so that both outputs leave in 16-byte stores.  A layer has few tiles: 256 x 256 fp32 takes 8 us, the latency of one block's load,
+// maximum, conversion and two stores; 8192 x 8192 takes 87 us, 3.8 TB/s.
 // ------------------------------------------------------------------------------------------------------
 constexpr int TILE_TPB = 1024;             // (16 values a thread: with 64 the few blocks of a layer took 11 us, all of it their own latency)
 template <typename T>
@@ -375,6 +376,8 @@ __global__ __launch_bounds__(TILE_TPB) void q8_pack_tile(const T* __restrict__ w
 //   Precision, measured on the instruction: it adds the products of 8 neighbouring k before they join the fp32 accumulator, each cut
 //   towards zero to a multiple of 2^-13 of the largest one's binade.  1.3e-5 of a result (2-norm, Gaussian operands): far below the
 //   rounding to 16 bits (1.7e-3 / 2.1e-4) and the operands' own (2.6e-2); a 32-bit result carries it.
+//   Kernels, by size (the rules stand in mgn_q8_matmul): q8_mm_small for few tiles, q8_stream_* for K <= 512 and many rows, q8_mm_128x32 for
+//   N <= 32, q8_mm_128x128 and q8_mm_256x256.
 // ------------------------------------------------------------------------------------------------------
 // act(v) without a branch: ReLU is lo = 0, neg = 1; leaky ReLU lo = -inf, neg = slope (0 < slope <= 1); none lo = -inf, neg = 1.  `maximum`
 // passes a NaN on.
@@ -496,8 +499,10 @@ __device__ __forceinline__ bool mm_tile(const MmParams& p, int& mtile, int& ntil
 constexpr int loads_left(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0070; }   // s_waitcnt vmcnt(n) lgkmcnt(0)
 
 // A block computes a BM x BN tile; a step covers one block of 128 k.  Rows travel HBM/L2 -> LDS by LDS-DMA (16 bytes a lane, 8 rows a
-// piece), two stages; 16-byte chunk c of row r lies at position c ^ ((r >> 1) & 7), so that the 16-byte fragment reads of 16 neighbouring
-// rows cover every bank once.
+// piece), ST stages; 16-byte chunk c of row r lies at position c ^ ((r >> 1) & 7), so that the 16-byte fragment reads of 16 neighbouring
+// rows cover every bank once.  128 x 128: two stages leave room for two blocks a CU, whose matrix and load phases fill each other's gaps
+// (four stages and one block: 8192^3 631 us against 490); 2048^3 15.3 us, 1.1 PFLOP/s, 256 blocks, one a CU and its step's latency.
+// 128 x 32: bound by reading A, three stages (100000 x 8 x 4096: 90 us against 106 with two; its 410 MB take 80 at the rate of a copy).
 template <int BM, int BN, int WVM, int WVN, int ST>
 __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
     using Tl = MmTile<BM, BN, WVM, WVN, ST>;
@@ -617,6 +622,9 @@ __device__ __forceinline__ void q8_mm_body(const MmParams& p) {
 // the loads of three stages later, so that matrix cores, LDS and loads run together.  Group 0 reads stage h in slot 2h and multiplies in
 // slot 2h + 1, group 1 a slot later; a barrier ends each slot.  Stage h + 3 takes the place of stage h - 1, which group 1 read in slot 2h - 1;
 // every wave has waited for its part of stage h + 1 when slot 2h + 1 ends.
+// 8192^3: 421-455 us, 2.4-2.6 PFLOP/s (the library's product with one scale per tensor 2.6).  The matrix cores are busy in 70 % of the
+// cycles, and the clock is down to 1.7-2.0 GHz: what is left is bound by power.  (One slot for all waves, two stages of 128 k: 10 % more
+// cycles; without any loads of the next stage 330 us, without LDS reads 370, without MFMAs 308.)
 struct Mm256 {
     static constexpr int ABYTES = 256 * 64, STAGE = 2 * ABYTES + 512, ST = 4, TM = 4, TN = 2, OUT = 32 * (TN * 32 * 4 + 16);
     static constexpr int LDS = ST * STAGE;
@@ -762,6 +770,8 @@ __global__ __launch_bounds__(256, 2) void q8_mm_128x32(MmParams p) { q8_mm_body<
 //   * 16-byte chunk c of LDS row r at c ^ (r & 15) (KB = 1: c ^ ((r >> 1) & 7)): fragment reads of 16 neighbouring rows cover each bank once;
 //   * a lane ends up with 4 + 4 consecutive channels of a pixel; v_permlane32_swap joins them to 16-byte stores.
 // grid (row blocks, N / (32 NT WN)); the blocks of one row range sit on one XCD (grid.x % 8 == 0) and share its rows through L2.
+// 262144 x 256 x 256: packed source 45-50 us (201 MB, 39 at the rate of a copy), 16-bit source 60-63 (269 MB, 52), with codes kept 64-69
+// (336 MB, 65).
 struct StreamParams {
     const unsigned char* src;             // codes, or 16-bit rows of `ld` elements
     const unsigned char* src_scales;
@@ -972,7 +982,9 @@ Q8_STREAM(1_256, 1, 2, 4, true) Q8_STREAM(2_256, 2, 2, 4, true) Q8_STREAM(4_256,
 #undef Q8_STREAM
 
 // Few tiles: a block per 32 x 32 outputs, the blocks of k dealt to its four waves, each with LDS stages of its own (rows travel by LDS-DMA,
-// the next block's while one is multiplied; no barrier), the four partial tiles added through LDS in wave order.
+// the next block's while one is multiplied; no barrier), the four partial tiles added through LDS in wave order.  1 x 4096 x 4096: 5.7 us
+// (16.8 MB of weights, 3.3 at the rate of a copy), 128 x 4096 x 4096 9.2.  Rows loaded straight into registers as the MFMA wants them, 16
+// bytes of another row in every lane, cost the address unit a cycle a lane: 8.6 and 19 us.  More waves for k do not help (8: 7.6 and 20).
 constexpr int SMALL_STAGE = 64 * BLK;     // 32 rows of A, 32 of B
 __global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
     extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];   // [stages][4 waves][SMALL_STAGE], later [4][32][33] floats
@@ -1052,7 +1064,10 @@ __global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
 // dW[n][k] = sum_m dy[m][n] x^[m][k], db[n] = sum_m dy[m][n]: dy in 16 bits, x^ from its codes.
 //   A block computes a 128 x 128 tile over one of `splits` row ranges.  dy rows go to LDS by LDS-DMA (three stages), codes through
 //   registers, where a value and its scale become the exact 16-bit x^ (one instruction for two); both tiles are read back with the
-//   transposing LDS reads, since the summed index is the row.  Loads run two steps ahead (80 KB of LDS: two blocks a CU).  v_mfma_f32_32x32x16, fp32 accumulation; the splits' tiles are added by q8_wgrad_reduce in order.
+//   transposing LDS reads, since the summed index is the row.  Loads run two steps ahead (80 KB of LDS: two blocks a CU).
+//   v_mfma_f32_32x32x16, fp32 accumulation; the splits' tiles are added by q8_wgrad_reduce in order.
+//   262144 x 256 x 256: 53-59 us, 3.5 TB/s (201 MB, each byte read once: 39 us at the rate of a copy), and 9 us for the reduction of 128 partial
+//   results (34 MB).  Bound by the step: spreading codes to 16 bits, the barrier, transposing reads; a quarter of the LDS cycles are conflicts.
 //   db: the same dy fragments times a column of ones, in the blocks of the first k tile.
 // ------------------------------------------------------------------------------------------------------
 struct WgradParams8 {
@@ -1287,7 +1302,8 @@ __global__ __launch_bounds__(TPB) void q8_pad_rows(const uint16_t* __restrict__ 
 // ------------------------------------------------------------------------------------------------------
 // block tail y = relu(norm(x) + shortcut) whose backward pass reads x^ instead of x.  Thread mapping of the four kernels: blockIdx.y = a
 // block of 128 channels, LPB lanes (8 channels each) per row -- a thread's channels never change, so their coefficients stay in
-// registers.  All are bound by HBM.
+// registers.  All are bound by HBM: 1048576 x 64 bf16, 134 MB a tensor: statistics 33-36 us (134 MB), forward 80 (478 MB, 6.0 TB/s), backward
+// sums 63 (344 MB, 5.4 TB/s), dx 56 (336 MB, 6.0 TB/s); joining the partial sums 5 and 7 us, two launches of latency.
 // ------------------------------------------------------------------------------------------------------
 constexpr int TAIL_BLOCKS = 512;          // row blocks of the two reductions (= partial rows)
 

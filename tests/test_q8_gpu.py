@@ -611,6 +611,46 @@ def test_chain_is_reproducible_and_near_the_16_bit_chain(dtype):
         assert rel <= share + (flip if k in (1, 2, 3, 6) else 0.0), (k, rel)
 
 
+@pytest.mark.parametrize("what", ["tile256", "tile128", "tile32", "few", "stream", "conv", "tail", "pack"])
+def test_repeats_under_load_are_identical(what):
+    """the same call again and again while two other streams keep memory and matrix cores busy: a wait that is too short shows here"""
+    o = ops()
+    if what in ("conv", "tail"):
+        x, wt, b, dy = conv_case(8, 256, 128, 256, 256, BF) if what == "conv" else (None,) * 4
+        t = tail_case(8, 64, 256, 512, BF) if what == "tail" else None
+
+        def call():
+            if what == "conv":
+                y = o.conv1x1_q8(x, wt, b)
+                return (y.detach(),) + torch.autograd.grad(y, (x, wt, b), dy)
+            xs, norm, sc, g = t
+            y = o.abn_add_relu_q8(xs, norm, sc)
+            return (y.detach(),) + torch.autograd.grad(y, (xs, sc, norm.weight, norm.bias), g)
+    elif what == "pack":
+        x = rand((262144, 257), BF, 1)
+
+        def call():
+            q = o.q8_pack(x)
+            return q.buf, q.unpack()
+    else:
+        M, N, K = {"tile256": (8192, 8192, 1088), "tile128": (2048, 2048, 2048), "tile32": (60000, 24, 1100), "few": (256, 1024, 4096), "stream": (262144, 256, 256)}[what]
+        qa, qb = o.q8_pack(rand((M, K), BF, 1)), o.q8_pack(rand((N, K), F32, 2, 0.3), tile=True)
+
+        def call():
+            return (o.q8_matmul(qa, qb),)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    big, mm = torch.randn(32 << 20, device="cuda"), torch.randn(4096, 4096, device="cuda").to(BF)
+    want = call()
+    for r in range(10):
+        for st in side:
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                big.mul_(1.0001)
+                torch.mm(mm, mm)
+        assert all(torch.equal(p, q) for p, q in zip(call(), want)), r
+    torch.cuda.synchronize()
+
+
 def test_chain_on_another_stream():
     o = ops()
     a = chain(2)
