@@ -1008,8 +1008,8 @@ __global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, (lds_ptr)(st + (4 + q) * 1024), 16, at, 0, 0, 0);
         }
     };
-    const bool am = lr < rowsA, bn = lr < rowsB;
-    const unsigned char *as = p.sa + m0 + (am ? lr : 0), *bs = p.sb + n0 + (bn ? lr : 0);
+    // (rows that are not there take the first row's scale: their codes are zeros, and no select waits for a scale that is still on its way)
+    const unsigned char *as = p.sa + m0 + (lr < rowsA ? lr : 0), *bs = p.sb + n0 + (lr < rowsB ? lr : 0);
     f32x16 acc;
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -1042,7 +1042,7 @@ __global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
-        multiply(st, am ? xs : 0, bn ? ws : 0);
+        multiply(st, xs, ws);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // read: the stage may be loaded again
         xs = xn, ws = wn;
     }
