@@ -834,7 +834,7 @@ int mgn_q8_conv1x1_bwd(const void* dy, long M, int C, int N, const void* buffer,
                        void* stream);
 /* Block tail y = relu(norm(x) + shortcut) (res_net.py:62-79) that keeps x in 8 bits for its backward pass.  All maps [M, C] channels-last,
  * 16-bit, 16-byte aligned, C % 8 == 0, C <= 8192.
- *   stats      : partials[rows][C][2] (rows = mgn_q8_tail_partial_rows) of (x - shift), (x - shift)^2 and shift[C] = x's first row, the
+ *   stats      : partials[rows][C][2] (rows = mgn_q8_tail_partial_rows) of (x - shift), (x - shift)^2 and shift[C] = the mean of some 64 .. 256 rows, the
  *                input of mgn_iabn_coeffs_from_partials
  *   fwd        : y = relu(scale * x + offset + shortcut) (one rounding), x packed, relu_bits: one byte per 8 outputs, bit k = (y[k] > 0);
  *                codes, scales and relu_bits all NULL: y alone (inference)

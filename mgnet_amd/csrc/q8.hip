@@ -1304,7 +1304,7 @@ __global__ __launch_bounds__(TPB) void q8_pad_rows(const uint16_t* __restrict__ 
 // block of 128 channels, LPB lanes (8 channels each) per row -- a thread's channels never change, so their coefficients stay in
 // registers.  All are bound by HBM: 1048576 x 64 bf16, 134 MB a tensor: statistics 33-36 us (134 MB), forward 80 (478 MB, 6.0 TB/s), backward
 // sums 63 (344 MB, 5.4 TB/s), dx 56 (336 MB, 6.0 TB/s); joining the partial sums 5 and 5 us, two launches of latency.
-// Reading alone is slower than copying: a library sum reads 134 MB at 3.2 TB/s, 2 GB at 4.0; the statistics read at 4.0 with 512 row blocks, at
+// Reading alone is slower than copying: a library sum reads 134 MB at 3.2 TB/s, 2 GB at 4.0; the statistics read at 3.9 with 512 row blocks, at
 // 3.4 with 1024 or 2048.
 // ------------------------------------------------------------------------------------------------------
 constexpr int TAIL_BLOCKS = 512;          // row blocks of the two reductions (= partial rows)
@@ -1328,15 +1328,41 @@ __device__ __forceinline__ void tail_flush(const float (&a)[8], const float (&b)
     }
 }
 
-// sums of (x - x[0]) and their squares (around the first row: no cancellation for channels with a large mean); shift[C] = x[0]
+// sums of (x - shift) and their squares; shift = the mean of 4 TPB / LPB (64 .. 256) rows spread over the map, the same in every block.  The
+// variance is a difference of two sums, off by some 2^-24 (mean - shift)^2: the mean of a sample is near the mean, also where one row alone (the
+// first, say) would be an outlier, as in channels that are zero almost everywhere.
 template <int LPB>
 __global__ __launch_bounds__(TPB) void q8_tail_stats(const uint16_t* __restrict__ x, int M, int C, float* __restrict__ part, float* __restrict__ shift) {
-    const int l = threadIdx.x % LPB, c0 = blockIdx.y * BLK + l * 8;
+    constexpr int RPB = TPB / LPB, NS = 4 * RPB;
+    __shared__ float sample[RPB][LPB * 8 + 4];
+    const int l = threadIdx.x % LPB, ty = threadIdx.x / LPB, c0 = blockIdx.y * BLK + l * 8;
     const bool on = c0 < C;
     float s[8], a[8], b[8];
-    unpack8(on ? *reinterpret_cast<const uint4*>(x + c0) : make_uint4(0, 0, 0, 0), s);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = b[k] = 0.f;
+    for (int k = 0; k < 8; ++k) s[k] = a[k] = b[k] = 0.f;
+    if (on) {
+        uint4 q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const uint4*>(x + (long)(ty + j * RPB) * M / NS * C + c0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v[8];
+            unpack8(q[j], v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[k] = fmaf(v[k], 1.f / NS, s[k]);   // (scaled before it is added: no overflow)
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sample[ty][l * 8 + k] = s[k];
+    __syncthreads();
+    if (threadIdx.x < LPB * 8) {
+        float m = 0.f;
+        for (int y = 0; y < RPB; ++y) m += sample[y][threadIdx.x];
+        sample[0][threadIdx.x] = m;       // (its column is this thread's alone)
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] = sample[0][l * 8 + k];
     const int stride = gridDim.x * (TPB / LPB);
     auto add = [&](const uint4& q) {
         float v[8];

@@ -375,6 +375,47 @@ def test_conv1x1_of_rows_past_32_bits():
     assert bool(((dw.view(N, C)[n].double() - gn.t() @ x8).abs() <= (M + 2) * 2.0 ** -23 * (gn.abs().t() @ x8.abs())).all())
 
 
+def test_maps_past_32_bit_offsets():
+    """2.15e9 values: the streaming 1x1 convolution and the block tail, first and last rows against 64 bits"""
+    from mgnet_amd.modeling.layers import InPlaceABNSync
+    o = ops()
+    M, C = (1 << 23) + 133, 256
+    r = torch.cat([torch.arange(300), torch.arange(M - 300, M)]).cuda()
+    as_map = lambda t: t.view(1, M, 1, -1).permute(0, 3, 1, 2)  # noqa: E731
+    x2, g2 = torch.zeros((M, C), dtype=BF, device="cuda"), torch.zeros((M, C), dtype=BF, device="cuda")
+    x2[r], g2[r] = rand((600, C), BF, 1, 0.3), rand((600, C), BF, 2, 0.0)
+    x, w = as_map(x2).requires_grad_(), (rand((C, C), F32, 3, 0.2) / 16).view(C, C, 1, 1).requires_grad_()
+    y = o.conv1x1_q8(x, w, None)
+    dx, dw = torch.autograd.grad(y, (x, w), as_map(g2))
+    w8, x8, g8, gr = q8_ref(w.detach().view(C, C), True)[0], q8_ref(x2[r])[0], q8_ref(g2[r])[0], g2[r].double()
+    for got, a, b in ((rows(y.detach())[r], x8, w8.t()), (rows(dx)[r], g8, w8)):
+        ref = a @ b
+        assert bool(((got.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1.01 * ((C + 2) * 2.0 ** -23 * (a.abs() @ b.abs()) + group_tol(a, b.t()))).all())
+    assert bool(((dw.view(C, C).double() - gr.t() @ x8).abs() <= 602 * 2.0 ** -23 * (gr.abs().t() @ x8.abs())).all())   # (the other rows add zeros)
+    assert not bool(rows(y.detach())[300:M - 300].any()) and not bool(rows(dx)[300:M - 300].any())
+    del y, dx
+    norm = InPlaceABNSync(C, activation="identity").cuda()
+    s = as_map(torch.zeros((M, C), dtype=BF, device="cuda")).requires_grad_()
+    y = o.abn_add_relu_q8(x, norm, s)
+    dx, ds = torch.autograd.grad(y, (x, s), as_map(g2))
+    # Of M rows 600 are not zero: mean and variance from their sums; gain 1 + eps, offset 0.  The statistics are fp32 sums around the mean c of
+    # 64 rows of which the first is not zero, c = x[0] / 64: n terms of (x - c)^2 and of x - c in a row (M / (512 * 16) a thread, 16 threads)
+    # put the variance off by n 2^-24 (var + (mean - c)^2), the mean by n 2^-24 (|mean| + |c|), twice that with the difference of the two sums
+    xr = x2[r].double()
+    mean, var = xr.sum(0) / M, (xr * xr).sum(0) / M
+    var = var - mean ** 2
+    c, n = xr[0] / 64, M / (512 * 16) + 16
+    gain = (1 + norm.eps) / torch.sqrt(var + norm.eps)
+    lack = n * 2.0 ** -24 * (var + (mean - c) ** 2) / (var + norm.eps)         # of the gain: half the variance's relative share, twice
+    assert float(lack.max()) < 0.02
+    ref = torch.relu(gain * (xr - mean))
+    tol = 2.0 ** -8 * ref + 1.02 * (lack * gain * (xr - mean).abs() + gain * 2 * n * 2.0 ** -24 * (mean.abs() + c.abs())) + 2.0 ** -20 * gain * (xr.abs() + mean.abs())
+    assert bool(((rows(y.detach())[r].double() - ref).abs() <= tol).all())
+    kept = (rows(y.detach())[r] > 0).double()
+    assert equal(rows(ds)[r].double(), gr * kept)
+    assert bool(torch.isfinite(rows(dx)[r]).all()) and bool(torch.isfinite(rows(dx)[M // 2:M // 2 + 100]).all())
+
+
 def test_conv1x1_gradient_against_differences():
     """<dW, V>, <db, v> and <dx, U> against differences of the unquantised convolution in 64 bits: q(.) is off by at most 2^-4 of a value
     (2^-10 * 2^e next to a block's largest, itself under 2^-4 of the term's share here)"""
@@ -487,6 +528,27 @@ def test_block_tail_one_row_and_inference():
     assert bool(((y.float() - ref).abs() <= 2.0 ** -11 * ref + 2.0 ** -20 * (z.abs() + s.float().abs() + 1)).all())
     with pytest.raises(NotImplementedError):
         torch.autograd.grad(o.abn_add_relu_q8(x, norm, s), (x,), g)
+
+
+@pytest.mark.parametrize("C", [8, 40, 128, 200])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_block_tail_statistics_of_sparse_channels(C, dtype):
+    """channels that are zero almost everywhere, but not in the first row; and channels with a large mean"""
+    from mgnet_amd.modeling.layers import InPlaceABNSync
+    M = 300000
+    x2 = torch.zeros((M, C), dtype=dtype, device="cuda")
+    x2[0], x2[M // 3:M // 3 + 5] = 90.0, rand((5, C), dtype, 1, 0.0)
+    x2[:, C // 2:] += 100.0
+    norm = InPlaceABNSync(C, momentum=1.0, activation="identity").cuda()
+    x = x2.view(1, M, 1, C).permute(0, 3, 1, 2)
+    y = ops().abn_add_relu_q8(x.requires_grad_(), norm, torch.zeros_like(x))
+    xd = x2.double()
+    mean, var = xd.mean(0), xd.var(0, unbiased=True)
+    # fp32 sums around c, the mean of at least 64 rows, 90 / 64 from the mean at most: n terms a thread and 64 threads at most, n <= M / (512 * 16) + 64
+    n, far = M / (512 * 16) + 64, (90 / 64) ** 2
+    assert bool(((norm.running_mean.double() - mean).abs() <= 2.0 ** -23 * mean.abs() + 2 * n * 2.0 ** -24 * (90 / 64 + 1)).all())
+    assert bool(((norm.running_var.double() - var).abs() <= 2 * n * 2.0 ** -24 * (var + far) + 2.0 ** -22 * var).all())
+    assert bool(torch.isfinite(y.float()).all())
 
 
 def test_block_tail_of_two_ranks(monkeypatch):
