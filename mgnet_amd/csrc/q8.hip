@@ -192,6 +192,7 @@ template <> struct Src<uint16_t> {
     static constexpr float TOP = TOP16;
     __device__ static Raw zero() { return Raw{make_uint4(0, 0, 0, 0)}; }
     __device__ static float one(const uint16_t* p) { return mgn_h2f(*p); }
+    __device__ static void get(const Raw& r, float (&v)[8]) { unpack8(r.a, v); }
     __device__ static Raw load(const uint16_t* p) { const u32x4_any v = *reinterpret_cast<const u32x4_any*>(p); return Raw{make_uint4(v.x, v.y, v.z, v.w)}; }
     __device__ static Raw tail(const uint16_t* p, int t) {
         u32x2_any lo = {0, 0};
@@ -299,67 +300,61 @@ __global__ __launch_bounds__(TPB) void q8_unpack(const unsigned char* __restrict
 // ------------------------------------------------------------------------------------------------------
 // a weight matrix W [N][K] (any strides) -> codes [N][ldc(K)] + scales [ceil(K/128)][lds(N)], and the same values transposed: codes
 // [K][ldc(N)] + scales [ceil(N/128)][lds(K)] (what the data gradient multiplies by).  A block per 128 x 128 tile; the tile goes through
-// LDS once so that both outputs leave in 16-byte stores.  A layer has few tiles: 256 x 256 fp32 takes 8 us, the latency of one block's load,
-// maximum, conversion and two stores; 8192 x 8192 takes 87 us, 3.8 TB/s.
+// LDS once so that both outputs leave in 16-byte stores.  A layer has few tiles: 256 x 256 fp32 takes 5.5 us, the latency of one block's load,
+// maximum, conversion and two stores (8.2 with a scalar load and a byte store to LDS for each value); 8192 x 8192 takes 85 us, 3.9 TB/s.
 // ------------------------------------------------------------------------------------------------------
-constexpr int TILE_TPB = 1024;             // (16 values a thread: with 64 the few blocks of a layer took 11 us, all of it their own latency)
+constexpr int TILE_TPB = 1024;            // 16 values a thread (64: 11 us for the same layer)
 template <typename T>
 __global__ __launch_bounds__(TILE_TPB) void q8_pack_tile(const T* __restrict__ w, long sr, long sc, int N, int K, unsigned char* __restrict__ codes,
                                                     unsigned char* __restrict__ scales, unsigned char* __restrict__ codes_t,
                                                     unsigned char* __restrict__ scales_t) {
-    constexpr int PITCH = BLK + 16;       // (rows of 16-byte chunks; the transposing byte reads then spread over the banks)
-    __shared__ __attribute__((aligned(16))) unsigned char tile[BLK * PITCH];
+    constexpr int PITCH = BLK + 4;        // (33 words: the transposing byte reads spread over the banks)
+    __shared__ uint32_t tile[BLK * PITCH / 4];
     __shared__ uint32_t part[TILE_TPB / 64];
     const int n0 = blockIdx.x * BLK, k0 = blockIdx.y * BLK, tid = threadIdx.x;
     const int ldk = (K + 15) & ~15, ldn = (N + 15) & ~15;
-    float f[16];
-    uint32_t m = 0;
-    // (lanes run along whichever axis is contiguous)
-    const bool kfast = sc == 1;
+    // A thread has 16 neighbours along the fast axis, the contiguous one.  Along it the codes leave from registers; the transposed ones go
+    // through LDS.
+    const bool kfast = sc == 1 || sr != 1;
+    const int ns = kfast ? N : K, nf = kfast ? K : N, s0 = kfast ? n0 : k0, f0 = kfast ? k0 : n0, lds = kfast ? ldn : ldk, ldf = kfast ? ldk : ldn;
+    const long ss = kfast ? sr : sc, sf = kfast ? sc : sr;
+    unsigned char *const direct = kfast ? codes : codes_t, *const turned = kfast ? codes_t : codes;
+    const int row = tid >> 3, ch = (tid & 7) * 16;
+    const T* p = w + (long)(s0 + row) * ss + (long)(f0 + ch) * sf;
+    float f[2][8];
+    if (s0 + row < ns && sf == 1 && f0 + ch + 16 <= nf) {
+        const typename Src<T>::Raw a = Src<T>::load(p), b = Src<T>::load(p + 8);
+        Src<T>::get(a, f[0]);
+        Src<T>::get(b, f[1]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int fast = tid & 127, slow = i * 8 + (tid >> 7);
-        const int r = kfast ? slow : fast, c = kfast ? fast : slow;
-        f[i] = (n0 + r < N && k0 + c < K) ? Src<T>::one(w + (long)(n0 + r) * sr + (long)(k0 + c) * sc) : 0.f;
-        const uint32_t u = __float_as_uint(f[i]) & 0x7fffffffu, v = u < 0x7f800000u ? u : 0u;
-        m = m > v ? m : v;
+        for (int k = 0; k < 16; ++k) f[k >> 3][k & 7] = (s0 + row < ns && f0 + ch + k < nf) ? Src<T>::one(p + k * sf) : 0.f;
     }
+    uint32_t m = amax8(f[0], Src<T>::TOP);
+    const uint32_t m1 = amax8(f[1], Src<T>::TOP);
+    m = group_max<16>(m > m1 ? m : m1);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const uint32_t o = (uint32_t)__shfl_xor((int)m, d); m = m > o ? m : o; }
+    for (int d = 16; d < 64; d <<= 1) { const uint32_t o = (uint32_t)__shfl_xor((int)m, d); m = m > o ? m : o; }
     if ((tid & 63) == 0) part[tid >> 6] = m;
     __syncthreads();
     m = part[0];
 #pragma unroll
     for (int k = 1; k < TILE_TPB / 64; ++k) m = m > part[k] ? m : part[k];
-    const uint32_t top = __float_as_uint(Src<T>::TOP);
-    const uint32_t s = scale_of(m < top ? m : top);
+    const uint32_t s = scale_of(m);
     const float inv = inv_scale(s);
-#pragma unroll
-    for (int i = 0; i < 16; i += 8) {
-        float g[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) g[k] = f[i + k];
-        const uint2 e = encode8(g, inv, Src<T>::TOP);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int fast = tid & 127, slow = (i + k) * 8 + (tid >> 7);
-            const int r = kfast ? slow : fast, c = kfast ? fast : slow;
-            tile[r * PITCH + c] = (unsigned char)((k < 4 ? e.x : e.y) >> (8 * (k & 3)));
-        }
-    }
-    __syncthreads();
-    for (int p = tid; p < BLK * (BLK / 16); p += TILE_TPB) {
-        const int r = p >> 3, ch = (p & 7) * 16;
-        if (codes && n0 + r < N && k0 + ch < ldk)
-            *reinterpret_cast<uint4*>(codes + (long)(n0 + r) * ldk + k0 + ch) = *reinterpret_cast<const uint4*>(tile + r * PITCH + ch);
-        if (codes_t && k0 + r < K && n0 + ch < ldn) {
+    const uint2 e0 = encode8(f[0], inv, Src<T>::TOP), e1 = encode8(f[1], inv, Src<T>::TOP);
+    if (direct && s0 + row < ns && f0 + ch < ldf) *reinterpret_cast<uint4*>(direct + (long)(s0 + row) * ldf + f0 + ch) = make_uint4(e0.x, e0.y, e1.x, e1.y);
+    if (turned) {
+        uint32_t* d = tile + (row * PITCH + ch) / 4;
+        d[0] = e0.x, d[1] = e0.y, d[2] = e1.x, d[3] = e1.y;
+        __syncthreads();
+        if (f0 + row < nf && s0 + ch < lds) {
+            const unsigned char* t = reinterpret_cast<const unsigned char*>(tile) + ch * PITCH + row;
             uint32_t o[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const unsigned char* t = tile + (ch + 4 * q) * PITCH + r;
+            for (int q = 0; q < 4; ++q, t += 4 * PITCH)
                 o[q] = (uint32_t)t[0] | ((uint32_t)t[PITCH] << 8) | ((uint32_t)t[2 * PITCH] << 16) | ((uint32_t)t[3 * PITCH] << 24);
-            }
-            *reinterpret_cast<uint4*>(codes_t + (long)(k0 + r) * ldn + n0 + ch) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(turned + (long)(f0 + row) * lds + s0 + ch) = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
     if (tid < BLK) {
