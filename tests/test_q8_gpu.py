@@ -470,7 +470,8 @@ def check_tail(x, norm, s, g):
     dev = (X - X[0]).abs().mean(0) + (X - mean).abs().mean(0)
     rstd, w = (var + norm.eps) ** -0.5, norm.weight.detach().double()
     gain = w.abs() + norm.eps
-    # variance around the first row: relative to the second moment there
+    # the variance comes from sums around the mean of a sample of rows: second moment there, for which the one around the first row stands (at
+    # least the variance itself)
     rv_err = u * ((X - X[0]) ** 2).mean(0) / (var + norm.eps)
     xh = (X - mean) * rstd
     ref = (gain * xh + norm.bias.detach().double() + S)
