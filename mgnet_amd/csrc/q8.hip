@@ -43,6 +43,18 @@ constexpr float TOP16 = 1.875f * 1.7014118346046923e38f;
 #endif
 constexpr float TOP32 = 1.875f * 1.7014118346046923e38f;
 
+// This block's number among those of flat_grid() below.  One dimension of a launch holds less than 2^32 work items: what is beyond that is
+// dropped without an error.
+constexpr int GRID_X_LOG2 = 20;
+__device__ __forceinline__ long block_id() { return ((long)blockIdx.y << GRID_X_LOG2) | blockIdx.x; }
+// blocks from the number that was asked for up to the grid's own have nothing to do and say so themselves
+inline bool flat_grid(long blocks, int threads, dim3* grid) {
+    if (blocks * threads <= 0xffffffffL) { *grid = dim3((unsigned)blocks); return true; }
+    const long rows = (blocks + (1L << GRID_X_LOG2) - 1) >> GRID_X_LOG2;
+    *grid = dim3(1u << GRID_X_LOG2, (unsigned)rows);
+    return rows <= 65535;
+}
+
 __device__ __forceinline__ float pow2(uint32_t biased) { return __uint_as_float(biased << 23); }
 // biased exponent of the scale: a <= 1.75 * 2^E  <=>  the mantissa bits of a do not exceed 0x600000
 __device__ __forceinline__ uint32_t scale_of(uint32_t amax_bits) {
@@ -207,7 +219,7 @@ template <> struct Src<uint16_t> {
 template <typename T, int LPB>
 __global__ __launch_bounds__(TPB) void q8_pack(const T* __restrict__ x, RowMap map, int M, int C, int nb, int ldc, long lds,
                                                unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
-    const long gid = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
+    const long gid = block_id() * (TPB / LPB) + threadIdx.x / LPB;
     const int l = threadIdx.x % LPB;
     const int kb = (int)(gid % nb);
     const long r0l = gid / nb * RPG;
@@ -247,7 +259,7 @@ __global__ __launch_bounds__(TPB) void q8_pack(const T* __restrict__ x, RowMap m
 template <typename T, int LPB>
 __global__ __launch_bounds__(TPB) void q8_unpack(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales, int M, int C,
                                                  int nb, int ldc, long lds, T* __restrict__ y) {
-    const long gid = (long)blockIdx.x * (TPB / LPB) + threadIdx.x / LPB;
+    const long gid = block_id() * (TPB / LPB) + threadIdx.x / LPB;
     const int l = threadIdx.x % LPB;
     const int kb = (int)(gid % nb);
     const long r0l = gid / nb * RPG;
@@ -483,9 +495,11 @@ __device__ __forceinline__ void mm_store(const MmParams& p, const f32x16 (&acc)[
 // x-th eighth of that sequence, so that the XCDs have equal shares and the tiles in flight on one share rows and columns in its L2.
 __device__ __forceinline__ bool mm_tile(const MmParams& p, int& mtile, int& ntile) {
     constexpr int G = 4;
-    const long total = (long)p.mt * p.nt;
-    const int x = blockIdx.x & 7, first = (int)(total * x >> 3), t = first + (int)(blockIdx.x >> 3);
-    if (t >= (int)(total * (x + 1) >> 3)) return false;
+    const long total = (long)p.mt * p.nt, id = block_id();
+    const int x = (int)id & 7;
+    const long first = total * x >> 3;
+    if (first + (id >> 3) >= total * (x + 1) >> 3) return false;
+    const int t = (int)(first + (id >> 3));
     const int g = t / (G * p.nt), in = t - g * G * p.nt, rows = p.mt - g * G < G ? p.mt - g * G : G;
     ntile = in / rows, mtile = g * G + in - ntile * rows;
     return true;
@@ -1093,8 +1107,8 @@ __global__ __launch_bounds__(TPB, 2) void q8_wgrad(WgradParams8 p) {
     extern __shared__ __attribute__((aligned(16))) unsigned char q8_sm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
     // the tiles of one row range share an XCD (its rows are then read from HBM once)
-    const int tiles = p.ntn * p.ntk, local = blockIdx.x >> 3;
-    const int z = (local / tiles) * 8 + (blockIdx.x & 7), t = local % tiles;
+    const int tiles = p.ntn * p.ntk, id = (int)block_id(), local = id >> 3;
+    const int z = (local / tiles) * 8 + (id & 7), t = local % tiles;
     if (z >= p.splits) return;
     const int tn = t % p.ntn, tk = t / p.ntn;
     const long mb = (long)z * p.rows_per_split;
@@ -1249,7 +1263,7 @@ __global__ __launch_bounds__(1024) void q8_wgrad_reduce(const float* __restrict_
                                                         float* __restrict__ db) {
     __shared__ float4 sh[16][64];
     const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const long stride = (total + 3) & ~3L, i = ((long)blockIdx.x * 64 + lane) * 4;
+    const long stride = (total + 3) & ~3L, i = (block_id() * 64 + lane) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < stride) {
         const float* src = part + i;
@@ -1281,7 +1295,7 @@ __global__ __launch_bounds__(1024) void q8_wgrad_reduce(const float* __restrict_
 // dy rows of N 16-bit values -> rows of ld (a multiple of 8) with zeros behind: what the 16-byte loads of the two gradients want
 __global__ __launch_bounds__(TPB) void q8_pad_rows(const uint16_t* __restrict__ src, long M, int N, int ld, uint4* __restrict__ dst) {
     const int per = ld / 8;
-    const long i = (long)blockIdx.x * TPB + threadIdx.x;
+    const long i = block_id() * TPB + threadIdx.x;
     if (i >= M * per) return;
     const long r = i / per;
     const int c = (int)(i - r * per) * 8;
@@ -1609,7 +1623,8 @@ int launch_mm(void (*kernel)(MmParams), MmParams p, hipStream_t s) {
     p.mt = (int)(((long)p.M + BM - 1) / BM);
     p.nt = (p.N + BN - 1) / BN;
     const long blocks = ((long)p.mt * p.nt + 7) / 8 * 8;
-    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    dim3 grid;
+    if (blocks > 0x7fffffffL || !flat_grid(blocks, TH, &grid)) return MGN_EINVAL;
     if (LDS > 65536) {
         static bool ready[64] = {};
         int dev = 0;
@@ -1619,7 +1634,7 @@ int launch_mm(void (*kernel)(MmParams), MmParams p, hipStream_t s) {
             ready[dev] = true;
         }
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(TH), LDS, s, p);
+    hipLaunchKernelGGL(kernel, grid, dim3(TH), LDS, s, p);
     return done();
 }
 
@@ -1648,10 +1663,11 @@ int MGN_SYM(mgn_q8_pack)(const void* x, int dtype, long M, int C, long sn, long 
     RowMap map = {sn, sh, sw, H, W, 0};
     map.flat = (H == 1 || sh == (long)W * sw) && (images == 1 || sn == (long)H * W * sw);
     const int nb = nblocks(C), ldc = code_ld(C), lpb = lanes_for(C);
-    const long groups = (M + RPG - 1) / RPG * nb, blocks = (groups * lpb + TPB - 1) / TPB;
-    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    const long groups = (M + RPG - 1) / RPG * nb;
+    dim3 grid;
+    if (!flat_grid((groups * lpb + TPB - 1) / TPB, TPB, &grid)) return MGN_EINVAL;
     hipStream_t s = (hipStream_t)stream_;
-#define Q8_PACK(T) Q8_LANES(C, (hipLaunchKernelGGL((q8_pack<T, LPB>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const T*)x, map, (int)M, C, nb, ldc, \
+#define Q8_PACK(T) Q8_LANES(C, (hipLaunchKernelGGL((q8_pack<T, LPB>), grid, dim3(TPB), 0, s, (const T*)x, map, (int)M, C, nb, ldc, \
                                                    scale_ld(M), (unsigned char*)codes, (unsigned char*)scales)))
     if (dtype) Q8_PACK(uint16_t); else Q8_PACK(float);
 #undef Q8_PACK
@@ -1663,10 +1679,11 @@ int MGN_SYM(mgn_q8_unpack)(const void* codes, const void* scales, long M, int C,
     if (M == 0) return MGN_OK;
     if (!codes || !scales || !y || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(y, dtype ? 2 : 4)) return MGN_EINVAL;
     const int nb = nblocks(C), ldc = code_ld(C), lpb = lanes_for(C);
-    const long groups = (M + RPG - 1) / RPG * nb, blocks = (groups * lpb + TPB - 1) / TPB;
-    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    const long groups = (M + RPG - 1) / RPG * nb;
+    dim3 grid;
+    if (!flat_grid((groups * lpb + TPB - 1) / TPB, TPB, &grid)) return MGN_EINVAL;
     hipStream_t s = (hipStream_t)stream_;
-#define Q8_UNPACK(T) Q8_LANES(C, (hipLaunchKernelGGL((q8_unpack<T, LPB>), dim3((unsigned)blocks), dim3(TPB), 0, s, (const unsigned char*)codes, \
+#define Q8_UNPACK(T) Q8_LANES(C, (hipLaunchKernelGGL((q8_unpack<T, LPB>), grid, dim3(TPB), 0, s, (const unsigned char*)codes, \
                                                      (const unsigned char*)scales, (int)M, C, nb, ldc, scale_ld(M), (T*)y)))
     if (dtype) Q8_UNPACK(uint16_t); else Q8_UNPACK(float);
 #undef Q8_UNPACK
@@ -1772,7 +1789,9 @@ int MGN_SYM(mgn_q8_wgrad)(const void* dy, long ldy, long M, int N, const void* c
     WgradParams8 p = {(const uint16_t*)dy, (const unsigned char*)codes, (const unsigned char*)scales, (float*)ws, (int)M, N, K, (int)ldy, code_ld(K),
                       scale_ld(M), (int)rows, (int)((M + rows - 1) / rows), nblocks(N), nblocks(K)};
     const long blocks = (long)((p.splits + 7) / 8) * 8 * p.ntn * p.ntk;
-    if (blocks > 0x7fffffffL) return MGN_EINVAL;
+    const long nk = (long)N * K, total = nk + N;
+    dim3 grid, rgrid;
+    if (blocks > 0x7fffffffL || !flat_grid(blocks, TPB, &grid) || !flat_grid((total + 255) / 256, 1024, &rgrid)) return MGN_EINVAL;
     hipStream_t s = (hipStream_t)stream_;
     static bool ready[64] = {};
     int dev = 0;
@@ -1781,9 +1800,8 @@ int MGN_SYM(mgn_q8_wgrad)(const void* dy, long ldy, long M, int N, const void* c
         if (hipFuncSetAttribute(reinterpret_cast<const void*>(q8_wgrad), hipFuncAttributeMaxDynamicSharedMemorySize, WG_LDS) != hipSuccess) return MGN_ELAUNCH;
         ready[dev] = true;
     }
-    hipLaunchKernelGGL(q8_wgrad, dim3((unsigned)blocks), dim3(TPB), WG_LDS, s, p);
-    const long nk = (long)N * K, total = nk + N;
-    hipLaunchKernelGGL(q8_wgrad_reduce, dim3((unsigned)((total + 255) / 256)), dim3(1024), 0, s, (const float*)ws, p.splits, total, nk, dw, db);
+    hipLaunchKernelGGL(q8_wgrad, grid, dim3(TPB), WG_LDS, s, p);
+    hipLaunchKernelGGL(q8_wgrad_reduce, rgrid, dim3(1024), 0, s, (const float*)ws, p.splits, total, nk, dw, db);
     return done();
 }
 
@@ -1858,9 +1876,9 @@ int MGN_SYM(mgn_q8_conv1x1_bwd)(const void* dy, long M, int C, int N, const void
     unsigned char* s = (unsigned char*)scratch;
     const int ldy = pad8(N);
     if (N % 8) {
-        const long blocks = (M * (ldy / 8) + TPB - 1) / TPB;
-        if (blocks > 0x7fffffffL) return MGN_EINVAL;
-        hipLaunchKernelGGL(q8_pad_rows, dim3((unsigned)blocks), dim3(TPB), 0, (hipStream_t)stream_, (const uint16_t*)dy, M, N, ldy, (uint4*)(s + t.pad));
+        dim3 grid;
+        if (!flat_grid((M * (ldy / 8) + TPB - 1) / TPB, TPB, &grid)) return MGN_EINVAL;
+        hipLaunchKernelGGL(q8_pad_rows, grid, dim3(TPB), 0, (hipStream_t)stream_, (const uint16_t*)dy, M, N, ldy, (uint4*)(s + t.pad));
         dy = s + t.pad;
     }
     if (dx) {   // (K = N padded: the columns behind N are zeros on both sides)

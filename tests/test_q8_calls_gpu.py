@@ -1,0 +1,25 @@
+"""8-bit operators at the sizes and in the calls where launches, masks and memory go wrong; tolerances as in test_q8_gpu.py."""
+import pytest
+import torch
+
+from test_q8_gpu import BF, ops, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def test_weight_gradient_of_more_than_2_32_work_items():
+    """32768 x 32768 weights: the sums of the partial gradients are 4194432 blocks of 1024 threads, more than one launch dimension holds.  dy and
+    x are small whole numbers, so the sums are exact in fp32"""
+    M, N = 64, 32768
+    g = torch.Generator(device="cuda").manual_seed(3)
+    whole = lambda: torch.randint(-7, 8, (1, 1, M, N), generator=g, device="cuda").to(BF).permute(0, 3, 1, 2)  # noqa: E731
+    x, dy = whole().requires_grad_(), whole()
+    w = torch.zeros((N, N, 1, 1), dtype=BF, device="cuda", requires_grad=True)
+    b = torch.zeros(N, device="cuda", requires_grad=True)
+    dw, db = torch.autograd.grad(ops().conv1x1_q8(x, w, b), (w, b), dy)
+    G, X = rows(dy).float(), rows(x.detach()).float()
+    assert torch.equal(db, G.sum(0))
+    for r in (0, 1, 8191, 16384, N - 4096, N - 1):
+        k = slice(r, min(r + 64, N))
+        assert torch.equal(dw[k, :, 0, 0].float(), (G[:, k].t().double() @ X.double()).float().to(BF).float()), r
+    assert torch.equal(dw.view(-1)[-N:].float(), (G[:, -1].double() @ X.double()).float().to(BF).float())
