@@ -183,7 +183,8 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
             return dx, torch.zeros(wshape, dtype=wdtype, device=dev) if want_dw else None, torch.zeros(Cout, dtype=bdtype, device=dev) if want_db else None, None
         dy = _rows16(dy, dtype)
         if y is not None:
-            dy = _C.relu_mask_bwd(dy, y) if _C.elt_supported(y) and _C.elt_supported(dy) else _rows16(dy * (y > 0), dtype)
+            # (a select either way: what is masked may be infinite)
+            dy = _C.relu_mask_bwd(dy, y) if _C.elt_supported(y) and _C.elt_supported(dy) else _rows16(dy.masked_fill(~(y > 0), 0.0), dtype)
         dw = torch.empty((Cout, C, 1, 1), dtype=torch.float32, device=dev) if want_dw or want_db else None
         db = torch.empty(Cout, dtype=torch.float32, device=dev) if want_db else None
         _C.q8_conv1x1_bwd(dy, M, C, Cout, buf, dx, dw, db)

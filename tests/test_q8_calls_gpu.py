@@ -1,8 +1,10 @@
 """8-bit operators at the sizes and in the calls where launches, masks and memory go wrong; tolerances as in test_q8_gpu.py."""
+import math
+
 import pytest
 import torch
 
-from test_q8_gpu import BF, ops, rows
+from test_q8_gpu import BF, conv_case, HF, ops, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +25,17 @@ def test_weight_gradient_of_more_than_2_32_work_items():
         k = slice(r, min(r + 64, N))
         assert torch.equal(dw[k, :, 0, 0].float(), (G[:, k].t().double() @ X.double()).float().to(BF).float()), r
     assert torch.equal(dw.view(-1)[-N:].float(), (G[:, -1].double() @ X.double()).float().to(BF).float())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("cout", [20, 24, 64])     # (64: the mask's kernel; 20 and 24: no kernel has their width)
+def test_relu_mask_takes_what_is_not_finite(cout, dtype):
+    """gradients that are infinite or NaN where the output is zero do not reach anything"""
+    x, wt, b, dy = conv_case(2, 40, 9, 7, cout, dtype)
+    y = ops().conv1x1_q8(x, wt, b, relu=True)
+    off = y.detach() == 0
+    assert 0.1 < float(off.float().mean()) < 0.9
+    want = torch.autograd.grad(y, (x, wt, b), dy.masked_fill(off, 0.0), retain_graph=True)
+    for v in (math.inf, -math.inf, math.nan):
+        got = torch.autograd.grad(y, (x, wt, b), dy.masked_fill(off, v), retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), v
