@@ -156,13 +156,14 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
     bits with the exact 16-bit value of the codes."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, relu):
+    def forward(ctx, x, weight, bias, relu, grad):
+        # grad: torch.is_grad_enabled() at the call (needs_input_grad goes by the inputs alone, and in here gradients are off)
         N, C, H, W = x.shape
         Cout = weight.shape[0]
         y = torch.empty((N, Cout, H, W), dtype=x.dtype, device=x.device, memory_format=_CL)
         rows, geometry = _geometry(x)
         w = weight.view(Cout, C) if weight.dtype in (torch.float32, x.dtype) and weight.is_contiguous() else weight.detach().float().reshape(Cout, C)
-        need = ctx.needs_input_grad
+        need = [grad and n for n in ctx.needs_input_grad]
         buf = _C.q8_conv1x1_fwd(rows, *geometry, w, Cout, None if bias is None else _f32(bias), int(relu), y, int(need[1] or need[2]))
         if need[0] or need[1] or need[2]:
             ctx.save_for_backward(buf, y if relu else None)
@@ -180,7 +181,7 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
         want_db = want_db and bdtype is not None
         dx = torch.empty(xshape, dtype=dtype, device=dev, memory_format=_CL) if want_dx else None
         if M == 0:
-            return dx, torch.zeros(wshape, dtype=wdtype, device=dev) if want_dw else None, torch.zeros(Cout, dtype=bdtype, device=dev) if want_db else None, None
+            return dx, torch.zeros(wshape, dtype=wdtype, device=dev) if want_dw else None, torch.zeros(Cout, dtype=bdtype, device=dev) if want_db else None, None, None
         dy = _rows16(dy, dtype)
         if y is not None:
             # (a select either way: what is masked may be infinite)
@@ -190,7 +191,7 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
         _C.q8_conv1x1_bwd(dy, M, C, Cout, buf, dx, dw, db)
         if want_db and bdtype != torch.float32:
             db = db.to(bdtype)
-        return dx, (dw if wdtype == torch.float32 else dw.to(wdtype)) if want_dw else None, db, None
+        return dx, (dw if wdtype == torch.float32 else dw.to(wdtype)) if want_dw else None, db, None, None
 
 
 def conv1x1_q8(x, weight, bias=None, relu=False):
@@ -210,8 +211,8 @@ def conv1x1_q8(x, weight, bias=None, relu=False):
         raise ValueError("conv1x1_q8: operands on different devices")
     if _elsewhere(x):
         with torch.cuda.device(x.device):
-            return _Conv1x1Q8Fn.apply(x, weight, bias, relu)
-    return _Conv1x1Q8Fn.apply(x, weight, bias, relu)
+            return _Conv1x1Q8Fn.apply(x, weight, bias, relu, torch.is_grad_enabled())
+    return _Conv1x1Q8Fn.apply(x, weight, bias, relu, torch.is_grad_enabled())
 
 
 def conv1x1_q8_supported(x, conv):
@@ -235,13 +236,13 @@ class _AbnAddReluQ8Fn(torch.autograd.Function):
     (the norm's x_hat is recomputed from there) and the ReLU mask in one bit a value; y is not kept."""
 
     @staticmethod
-    def forward(ctx, x, shortcut, weight, bias, running_mean, running_var, training, momentum, eps, group, pstats):
+    def forward(ctx, x, shortcut, weight, bias, running_mean, running_var, training, momentum, eps, group, pstats, grad):
         N, C, H, W = x.shape
         M = N * H * W
         x, shortcut = _rows16(x, x.dtype), _rows16(shortcut, x.dtype)
         w32, b32 = _f32(weight), _f32(bias)
         need = ctx.needs_input_grad
-        buf = _C.q8_tail_buffer(M, C, x.device) if training and (need[0] or need[1] or need[2] or need[3]) else None
+        buf = _C.q8_tail_buffer(M, C, x.device) if training and grad and (need[0] or need[1] or need[2] or need[3]) else None   # (grad: as above)
         y = torch.empty((N, C, H, W), dtype=x.dtype, device=x.device, memory_format=_CL)
         world = dist.get_world_size(group) if _dist_active(group) else 1
         if training and world == 1 and pstats is None:
@@ -278,7 +279,7 @@ class _AbnAddReluQ8Fn(torch.autograd.Function):
         dw, db = out[2], out[3]
         if wdtype != torch.float32:
             dw, db = dw.to(wdtype), db.to(wdtype)
-        return dx, dz, dw, db, None, None, None, None, None, None, None
+        return dx, dz, dw, db, None, None, None, None, None, None, None, None
 
 
 def abn_add_relu_q8(x, norm, shortcut):
@@ -295,7 +296,7 @@ def abn_add_relu_q8(x, norm, shortcut):
     if norm.activation != "identity" or norm.num_features != C or w.device != x.device or norm.running_mean.dtype != torch.float32:
         raise ValueError(f"abn_add_relu_q8: an identity-activation norm of {C} channels on {x.device} with float32 statistics, got {norm.activation}, "
                          f"{norm.num_features}, {w.device}, {norm.running_mean.dtype}")
-    args = (x, shortcut, w, norm.bias, norm.running_mean, norm.running_var, norm.training, norm.momentum, norm.eps, norm.group, _pstats(x))
+    args = (x, shortcut, w, norm.bias, norm.running_mean, norm.running_var, norm.training, norm.momentum, norm.eps, norm.group, _pstats(x), torch.is_grad_enabled())
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return _AbnAddReluQ8Fn.apply(*args)

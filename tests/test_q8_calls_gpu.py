@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_q8_gpu import BF, conv_case, HF, ops, rows
+from test_q8_gpu import BF, conv_case, HF, ops, rows, tail_case
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,30 @@ def test_relu_mask_takes_what_is_not_finite(cout, dtype):
     for v in (math.inf, -math.inf, math.nan):
         got = torch.autograd.grad(y, (x, wt, b), dy.masked_fill(off, v), retain_graph=True)
         assert all(torch.equal(p, q) for p, q in zip(got, want)), v
+
+
+def test_block_tail_without_gradients_keeps_nothing(monkeypatch):
+    import copy
+
+    from mgnet_amd import _C
+    o = ops()
+    x, norm, s, _ = tail_case(2, 64, 33, 20, BF, 4)
+    other = copy.deepcopy(norm)
+    want = o.abn_add_relu_q8(x, norm, s).detach()
+    monkeypatch.setattr(_C, "q8_tail_buffer", None)        # (not asked for)
+    with torch.no_grad():
+        y = o.abn_add_relu_q8(x, other, s)
+    assert torch.equal(y, want) and torch.equal(norm.running_mean, other.running_mean) and torch.equal(norm.running_var, other.running_var)
+
+
+def test_conv1x1_without_gradients_writes_no_codes(monkeypatch):
+    from mgnet_amd import _C
+    o = ops()
+    x, wt, b, _ = conv_case(2, 64, 33, 20, 24, BF)
+    keep = []
+    fwd = _C.q8_conv1x1_fwd
+    monkeypatch.setattr(_C, "q8_conv1x1_fwd", lambda *a: keep.append(int(a[-1])) or fwd(*a))
+    want = o.conv1x1_q8(x, wt, b)
+    with torch.no_grad():
+        assert torch.equal(o.conv1x1_q8(x, wt, b), want)
+    assert keep == [1, 0]
