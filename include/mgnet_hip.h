@@ -825,9 +825,15 @@ int mgn_q8_wgrad_workspace_bytes(long M, int N, int K, size_t* bytes);
 int mgn_q8_wgrad(const void* dy, long ldy, long M, int N, const void* codes, const void* scales, int K, float* dw, float* db, void* workspace,
                  size_t workspace_bytes, void* stream);
 /* The trained 1x1 convolution in one call each way.  x: as mgn_q8_pack (16-bit); w [N][C] with strides w_sr, w_sc (dtype as there); y, dy, dx:
- * contiguous rows, 16-byte aligned.  `buffer` (mgn_q8_conv1x1_bytes, 16-byte aligned) holds the packed x (unless keep = 0), the packed
- * weights and their transpose; the backward call reads it.  dx, dw [N][C], db [N] may be NULL (db only with dw). */
+ * contiguous rows, 16-byte aligned.  `buffer` (16-byte aligned) holds the packed weights' transpose, the packed weights and the packed x; the
+ * backward call reads it.  keep = 0: no weight gradient will be asked for, and of the buffer only its first part is read again.
+ * mgn_q8_conv1x1_bytes     : sizes that are enough for every call of M, C, N
+ * mgn_q8_conv1x1_fwd_bytes : what this forward call needs (x, strides, y and keep as there), and how many of the buffer's first bytes the
+ *                            backward call reads
+ * dx, dw [N][C], db [N] may be NULL (db only with dw; dw only after keep = 1). */
 int mgn_q8_conv1x1_bytes(long M, int C, int N, size_t* buffer, size_t* scratch);
+int mgn_q8_conv1x1_fwd_bytes(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, int N, const void* y, int keep, size_t* buffer,
+                             size_t* kept);
 int mgn_q8_conv1x1_fwd(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, const void* w, int w_dtype, long w_sr, long w_sc, int N,
                        const float* bias, int relu, void* y, int keep, void* buffer, size_t buffer_bytes, void* stream);
 int mgn_q8_conv1x1_bwd(const void* dy, long M, int C, int N, const void* buffer, void* dx, float* dw, float* db, void* scratch, size_t scratch_bytes,

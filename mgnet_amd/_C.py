@@ -33,7 +33,7 @@ SYMBOLS = ["mgn_version", "mgn_reproj_workspace_bytes", "mgn_reproj_loss_fwd", "
            "mgn_plan_trace", "mgn_plan_trace_read", "mgn_plan_set_skip", "mgn_plan_node_ro", "mgn_plan_node_ro_family", "mgn_plan_set_jitter", "mgn_plan_probe",
            "mgn_abn_apply_pool", "mgn_att_abn_bwd_stats", "mgn_att_abn_bwd_sums", "mgn_att_abn_bwd_apply",
            "mgn_q8_bytes", "mgn_q8_pack", "mgn_q8_unpack", "mgn_q8_pack_weight", "mgn_q8_matmul", "mgn_q8_pack_matmul", "mgn_q8_wgrad_workspace_bytes", "mgn_q8_wgrad", "mgn_q8_tail_partial_rows", "mgn_q8_tail_stats", "mgn_q8_tail_fwd", "mgn_q8_tail_bwd_reduce", "mgn_q8_tail_sums", "mgn_q8_tail_bwd_apply",
-           "mgn_q8_conv1x1_bytes", "mgn_q8_conv1x1_fwd", "mgn_q8_conv1x1_bwd", "mgn_q8_tail_workspace_bytes", "mgn_q8_tail_train_fwd", "mgn_q8_tail_train_bwd"]
+           "mgn_q8_conv1x1_bytes", "mgn_q8_conv1x1_fwd_bytes", "mgn_q8_conv1x1_fwd", "mgn_q8_conv1x1_bwd", "mgn_q8_tail_workspace_bytes", "mgn_q8_tail_train_fwd", "mgn_q8_tail_train_bwd"]
 SYMBOLS_F16 = [n + "_f16" for n in ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_pack_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply', 'mgn_q8_conv1x1_fwd', 'mgn_q8_conv1x1_bwd', 'mgn_q8_tail_train_fwd', 'mgn_q8_tail_train_bwd']]
 DEPTH_MAX_FILTER_IDS = 16
 MGN_MAX_TASKS = 8   # include/mgnet_hip.h
@@ -254,6 +254,7 @@ def lib():
         L.mgn_q8_tail_sums.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
         L.mgn_q8_tail_bwd_apply.argtypes = [vp, vp, vp, vp, vp, vp, vp, cf, cf, cl, ci, vp, vp]
         L.mgn_q8_conv1x1_bytes.argtypes = [cl, ci, ci, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        L.mgn_q8_conv1x1_fwd_bytes.argtypes = [vp, cl, ci, cl, cl, cl, ci, ci, ci, vp, ci, ctypes.POINTER(sz), ctypes.POINTER(sz)]
         L.mgn_q8_conv1x1_fwd.argtypes = [vp, cl, ci, cl, cl, cl, ci, ci, vp, ci, cl, cl, ci, vp, ci, vp, ci, vp, sz, vp]
         L.mgn_q8_conv1x1_bwd.argtypes = [vp, cl, ci, ci, vp, vp, vp, vp, vp, sz, vp]
         L.mgn_q8_tail_workspace_bytes.argtypes = [cl, ci, ctypes.POINTER(sz)]
@@ -1688,12 +1689,17 @@ def _q8_conv_sizes(M, C, N):
 
 
 def q8_conv1x1_fwd(x, M, C, sn, sh, sw, H, W, w, N, bias, relu, y, keep):
-    """y [M, N] = q(x) q(w)^T + bias [-> ReLU] -> the buffer q8_conv1x1_bwd reads"""
-    nb = _q8_conv_sizes(M, C, N)[0]
+    """y [M, N] = q(x) q(w)^T + bias [-> ReLU] -> (buffer, how many of its first bytes q8_conv1x1_bwd reads); keep = 0: without the packed x, for no
+    weight gradient"""
+    nb = kept = _q8_conv_sizes(M, C, N)[0]
+    if not keep:                # (by the call: whether x is packed on the way goes by its strides and alignment)
+        a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        check(lib().mgn_q8_conv1x1_fwd_bytes(x.data_ptr(), M, C, sn, sh, sw, H, W, N, y.data_ptr(), 0, ctypes.byref(a), ctypes.byref(b)), "mgn_q8_conv1x1_fwd_bytes")
+        nb, kept = a.value, b.value
     buf = torch.empty(nb, dtype=torch.uint8, device=x.device)
     check(_fn("mgn_q8_conv1x1_fwd", x)(x.data_ptr(), M, C, sn, sh, sw, H, W, w.data_ptr(), _act_dtype(w), w.stride(0), w.stride(1), N,
                                        None if bias is None else bias.data_ptr(), relu, y.data_ptr(), keep, buf.data_ptr(), nb, _stream()), "mgn_q8_conv1x1_fwd")
-    return buf
+    return buf, kept
 
 
 def q8_conv1x1_bwd(dy, M, C, N, buf, dx, dw, db):

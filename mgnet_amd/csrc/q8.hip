@@ -1584,19 +1584,32 @@ inline int done() { return hipGetLastError() == hipSuccess ? MGN_OK : MGN_ELAUNC
 constexpr long MAX_ROWS = 0x7fffff00L;    // rows are counted in 32 bits (padded to 16), offsets in 64
 constexpr int MAX_COLS = 1 << 20;
 
-// The streaming product; MGN_ENOTSUP where another kernel is meant.  src_kind as SRC; `least` tiles for each block, or that other kernel.
+// The streaming product's form for these sizes; false where another kernel is meant.  src_kind as SRC; `least` tiles for each block, or that
+// other kernel; vec: 16-bit results in rows of 16-byte pieces.
+struct StreamForm { int ki, shape, th, BM, groups, gx, ntiles; };
+bool stream_form(long M, int K, int N, bool vec, int src_kind, int least, StreamForm* f) {
+    if (K > 512 || scale_ld(M) * 4 > 0x7fffffffL || (!vec && N > 32)) return false;
+    f->ki = K <= 128 ? 0 : (K <= 256 ? 1 : 2);
+    const int KB = 1 << f->ki;
+    f->shape = !vec ? 0 : (N <= 32 ? 1 : (N <= 128 ? 2 : 3));
+    const int chans = f->shape <= 1 ? 32 : (f->shape == 2 ? 128 : 256);
+    f->th = KB == 4 && f->shape == 3 ? 512 : 256;
+    f->BM = 128 / KB * (src_kind == 0 ? 2 : 1) * (f->th / 256);
+    f->groups = (N + chans - 1) / chans;
+    f->ntiles = (int)((M + f->BM - 1) / f->BM);
+    f->gx = (512 * 256 / f->th) / f->groups & ~7;   // two blocks a CU (one of 512 threads)
+    if (f->gx < 8 || f->ntiles < least * f->gx) return false;
+    f->gx = f->ntiles < f->gx ? f->ntiles : f->gx;
+    return true;
+}
+bool stream_vec(int N, const void* out, int out32, long ldo) { return !out32 && N % 8 == 0 && ldo % 8 == 0 && ldo <= MAX_COLS && aligned(out, 16); }
+
+// The streaming product; MGN_ENOTSUP where another kernel is meant.
 int launch_stream(StreamParams p, int src_kind, int least, hipStream_t s) {
-    if (p.K > 512 || p.lds * 4 > 0x7fffffffL) return MGN_ENOTSUP;
-    const bool vec = !p.out32 && p.N % 8 == 0 && p.ldo % 8 == 0 && p.ldo <= MAX_COLS && aligned(p.out, 16);
-    if (!vec && p.N > 32) return MGN_ENOTSUP;
-    const int ki = p.K <= 128 ? 0 : (p.K <= 256 ? 1 : 2), KB = 1 << ki;
-    const int shape = !vec ? 0 : (p.N <= 32 ? 1 : (p.N <= 128 ? 2 : 3)), chans = shape <= 1 ? 32 : (shape == 2 ? 128 : 256);
-    const int th = KB == 4 && shape == 3 ? 512 : 256, BM = 128 / KB * (src_kind == 0 ? 2 : 1) * (th / 256), groups = (p.N + chans - 1) / chans;
-    p.ntiles = (int)(((long)p.M + BM - 1) / BM);
-    int gx = (512 * 256 / th) / groups & ~7;   // two blocks a CU (one of 512 threads)
-    if (gx < 8 || p.ntiles < least * gx) return MGN_ENOTSUP;
-    gx = p.ntiles < gx ? p.ntiles : gx;
-    const int lds = 2 * (BM * KB * BLK + KB * BM) + 1024;
+    StreamForm f;
+    if (!stream_form(p.M, p.K, p.N, stream_vec(p.N, p.out, p.out32, p.ldo), src_kind, least, &f)) return MGN_ENOTSUP;
+    p.ntiles = f.ntiles;
+    const int ki = f.ki, shape = f.shape, KB = 1 << ki, lds = 2 * (f.BM * KB * BLK + KB * f.BM) + 1024;
     typedef void (*K)(StreamParams);
 #define Q8_SRC(N) {q8_stream_##N##_packed, q8_stream_##N##_h16, q8_stream_##N##_keep}
     static const K table[3][4][3] = {{Q8_SRC(1_any), Q8_SRC(1_32), Q8_SRC(1_128), Q8_SRC(1_256)},
@@ -1614,7 +1627,7 @@ int launch_stream(StreamParams p, int src_kind, int least, hipStream_t s) {
             r = true;
         }
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)gx, (unsigned)groups), dim3(th), lds, s, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)f.gx, (unsigned)f.groups), dim3(f.th), lds, s, p);
     return done();
 }
 
@@ -1736,13 +1749,19 @@ int MGN_SYM(mgn_q8_matmul)(const void* a, const void* a_scales, long M, const vo
     return launch_mm<128, 128, MmTile<128, 128, 2, 2, 2>::LDS, 256>(q8_mm_128x128, p, s);
 }
 
+// whether mgn_q8_pack_matmul packs on the way
+static bool stream_packs(const void* x, long M, int K, long ldx, int N, const void* out, int out_f32, long ldo, int src_kind) {
+    StreamForm f;
+    return K % 8 == 0 && ldx % 8 == 0 && aligned(x, 16) && stream_form(M, K, N, stream_vec(N, out, out_f32, ldo), src_kind, 0, &f);
+}
+
 int MGN_SYM(mgn_q8_pack_matmul)(const void* x, long M, int K, long ldx, void* codes, void* scales, const void* b, const void* b_scales, int N,
                                 const float* bias, int act, float slope, void* out, int out_f32, long ldo, void* stream_) {
     if (M < 0 || M > MAX_ROWS || N < 1 || N > MAX_COLS || K < 1 || K > MAX_COLS || !act_ok(act, slope) || ldo < N || ldx < K || ldx > MAX_COLS) return MGN_EINVAL;
     if (M == 0) return MGN_OK;
     if (!x || !b || !b_scales || !out || !codes != !scales || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(b, 16) || !aligned(x, 2) ||
         !aligned(out, out_f32 ? 4 : 2)) return MGN_EINVAL;
-    if (K > 512 || K % 8 != 0 || ldx % 8 != 0 || !aligned(x, 16)) return MGN_ENOTSUP;
+    if (!stream_packs(x, M, K, ldx, N, out, out_f32, ldo, codes ? 2 : 1)) return MGN_ENOTSUP;
     StreamParams p = {(const unsigned char*)x, nullptr, (unsigned char*)codes, (unsigned char*)scales, (const unsigned char*)b, (const unsigned char*)b_scales, bias, out,
                       (int)M, K, N, (int)ldx, code_ld(K), code_ld(K), 0, scale_ld(M), scale_ld(N), ldo, make_act(act, slope), out_f32};
     return launch_stream(p, codes ? 2 : 1, 0, (hipStream_t)stream_);
@@ -1806,16 +1825,18 @@ int MGN_SYM(mgn_q8_wgrad)(const void* dy, long ldy, long M, int N, const void* c
 }
 
 /* ---- the trained 1x1 convolution in two calls ---- */
-struct ConvBuffer { size_t codes, scales, tcodes, tscales, wcodes, wscales, total; };   // offsets; every piece is a multiple of 16 bytes
+// [transposed weights][weights][packed x], offsets, every piece a multiple of 16 bytes: what the data gradient reads comes first, what only the
+// weight gradient reads comes last
+struct ConvBuffer { size_t tcodes, tscales, wcodes, wscales, codes, scales, total; };
 static ConvBuffer conv_buffer(long M, int C, int N) {
     ConvBuffer b;
-    b.codes = 0;
-    b.scales = b.codes + (size_t)M * code_ld(C);
-    b.tcodes = b.scales + (size_t)nblocks(C) * scale_ld(M);
+    b.tcodes = 0;
     b.tscales = b.tcodes + (size_t)C * code_ld(N);
     b.wcodes = b.tscales + (size_t)nblocks(N) * scale_ld(C);
     b.wscales = b.wcodes + (size_t)N * code_ld(C);
-    b.total = b.wscales + (size_t)nblocks(C) * scale_ld(N);
+    b.codes = b.wscales + (size_t)nblocks(C) * scale_ld(N);
+    b.scales = b.codes + (size_t)M * code_ld(C);
+    b.total = b.scales + (size_t)nblocks(C) * scale_ld(M);
     return b;
 }
 static bool conv_shape(long M, int C, int N) { return M >= 0 && M <= MAX_ROWS && C >= 1 && C <= 65536 && N >= 1 && N <= 65536; }
@@ -1843,18 +1864,37 @@ int mgn_q8_conv1x1_bytes(long M, int C, int N, size_t* buffer, size_t* scratch) 
 }
 #endif
 
+// rows of C 16-bit values one behind the other
+static bool conv_flat(long M, int C, long sn, long sh, long sw, int H, int W) {
+    const long images = H < 1 || W < 1 ? 0 : M / ((long)H * W);
+    return (W == 1 || sw == C) && (H == 1 || sh == (long)W * C) && (images == 1 || sn == (long)H * W * C);
+}
+// x goes into the product without a packed form in memory
+static bool conv_unkept(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, int N, const void* y, int keep) {
+    return M == 0 || (!keep && conv_flat(M, C, sn, sh, sw, H, W) && stream_packs(x, M, C, C, N, y, 0, N, 1));
+}
+
+#ifndef MGN_F16
+int mgn_q8_conv1x1_fwd_bytes(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, int N, const void* y, int keep, size_t* buffer,
+                             size_t* kept) {
+    if (!conv_shape(M, C, N) || !buffer || !kept) return MGN_EINVAL;
+    const ConvBuffer b = conv_buffer(M, C, N);
+    *buffer = conv_unkept(x, M, C, sn, sh, sw, H, W, N, y, keep) ? b.codes : b.total;
+    *kept = keep ? b.total : b.wcodes;
+    return MGN_OK;
+}
+#endif
+
 int MGN_SYM(mgn_q8_conv1x1_fwd)(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, const void* w, int w_dtype, long w_sr, long w_sc,
                                 int N, const float* bias, int relu, void* y, int keep, void* buffer, size_t buffer_bytes, void* stream_) {
     if (!conv_shape(M, C, N) || !w || (!y && M > 0) || !buffer || !aligned(buffer, 16)) return MGN_EINVAL;
     const ConvBuffer b = conv_buffer(M, C, N);
-    if (buffer_bytes < b.total) return MGN_ENOSPC;
+    if (buffer_bytes < (conv_unkept(x, M, C, sn, sh, sw, H, W, N, y, keep) ? b.codes : b.total)) return MGN_ENOSPC;
     unsigned char* p = (unsigned char*)buffer;
     int rc = MGN_SYM(mgn_q8_pack_weight)(w, w_dtype, w_sr, w_sc, N, C, p + b.wcodes, p + b.wscales, p + b.tcodes, p + b.tscales, stream_);
     if (rc != MGN_OK || M == 0) return rc;
-    const long images = H < 1 || W < 1 ? 0 : M / ((long)H * W);
-    const bool flat = (W == 1 || sw == C) && (H == 1 || sh == (long)W * C) && (images == 1 || sn == (long)H * W * C);
     rc = MGN_ENOTSUP;
-    if (flat) rc = MGN_SYM(mgn_q8_pack_matmul)(x, M, C, C, keep ? p + b.codes : nullptr, keep ? p + b.scales : nullptr, p + b.wcodes, p + b.wscales, N, bias,
+    if (conv_flat(M, C, sn, sh, sw, H, W)) rc = MGN_SYM(mgn_q8_pack_matmul)(x, M, C, C, keep ? p + b.codes : nullptr, keep ? p + b.scales : nullptr, p + b.wcodes, p + b.wscales, N, bias,
                                                relu ? 1 : 0, 0.f, y, 0, N, stream_);
     if (rc != MGN_ENOTSUP) return rc;
     rc = MGN_SYM(mgn_q8_pack)(x, 1, M, C, sn, sh, sw, H, W, p + b.codes, p + b.scales, stream_);

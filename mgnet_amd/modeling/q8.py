@@ -164,8 +164,10 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
         rows, geometry = _geometry(x)
         w = weight.view(Cout, C) if weight.dtype in (torch.float32, x.dtype) and weight.is_contiguous() else weight.detach().float().reshape(Cout, C)
         need = [grad and n for n in ctx.needs_input_grad]
-        buf = _C.q8_conv1x1_fwd(rows, *geometry, w, Cout, None if bias is None else _f32(bias), int(relu), y, int(need[1] or need[2]))
+        buf, kept = _C.q8_conv1x1_fwd(rows, *geometry, w, Cout, None if bias is None else _f32(bias), int(relu), y, int(need[1] or need[2]))
         if need[0] or need[1] or need[2]:
+            if buf.numel() - kept > N * H * W * C:      # (x was packed in a pass of its own, for this call alone: its codes do not wait)
+                buf = buf[:kept].clone()
             ctx.save_for_backward(buf, y if relu else None)
             ctx.cfg = (x.shape, x.dtype, weight.dtype, weight.shape, None if bias is None else bias.dtype)
         return y

@@ -1,0 +1,145 @@
+"""8-bit operators at the sizes and in the calls where launches, masks and memory go wrong; tolerances as in test_q8_gpu.py."""
+import math
+
+import pytest
+import torch
+
+from test_q8_gpu import BF, conv_case, F32, HF, ops, rand, rows, tail_case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _give_the_memory_back():
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_weight_gradient_of_more_than_2_32_work_items():
+    """32768 x 32768 weights: the sums of the partial gradients are 4194432 blocks of 1024 threads, more than one launch dimension holds.  dy and
+    x are small whole numbers, so the sums are exact in fp32"""
+    M, N = 64, 32768
+    g = torch.Generator(device="cuda").manual_seed(3)
+    whole = lambda: torch.randint(-7, 8, (1, 1, M, N), generator=g, device="cuda").to(BF).permute(0, 3, 1, 2)  # noqa: E731
+    x, dy = whole().requires_grad_(), whole()
+    w = torch.zeros((N, N, 1, 1), dtype=BF, device="cuda", requires_grad=True)
+    b = torch.zeros(N, device="cuda", requires_grad=True)
+    dw, db = torch.autograd.grad(ops().conv1x1_q8(x, w, b), (w, b), dy)
+    G, X = rows(dy).float(), rows(x.detach()).float()
+    assert torch.equal(db, G.sum(0))
+    for r in (0, 1, 8191, 16384, N - 4096, N - 1):
+        k = slice(r, min(r + 64, N))
+        assert torch.equal(dw[k, :, 0, 0].float(), (G[:, k].t().double() @ X.double()).float().to(BF).float()), r
+    assert torch.equal(dw.view(-1)[-N:].float(), (G[:, -1].double() @ X.double()).float().to(BF).float())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("cout", [20, 24, 64])     # (64: the mask's kernel; 20 and 24: no kernel has their width)
+def test_relu_mask_takes_what_is_not_finite(cout, dtype):
+    """gradients that are infinite or NaN where the output is zero do not reach anything"""
+    x, wt, b, dy = conv_case(2, 40, 9, 7, cout, dtype)
+    y = ops().conv1x1_q8(x, wt, b, relu=True)
+    off = y.detach() == 0
+    assert 0.1 < float(off.float().mean()) < 0.9
+    want = torch.autograd.grad(y, (x, wt, b), dy.masked_fill(off, 0.0), retain_graph=True)
+    for v in (math.inf, -math.inf, math.nan):
+        got = torch.autograd.grad(y, (x, wt, b), dy.masked_fill(off, v), retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), v
+
+
+def test_block_tail_without_gradients_keeps_nothing(monkeypatch):
+    import copy
+
+    from mgnet_amd import _C
+    o = ops()
+    x, norm, s, _ = tail_case(2, 64, 33, 20, BF, 4)
+    other = copy.deepcopy(norm)
+    want = o.abn_add_relu_q8(x, norm, s).detach()
+    monkeypatch.setattr(_C, "q8_tail_buffer", None)        # (not asked for)
+    with torch.no_grad():
+        y = o.abn_add_relu_q8(x, other, s)
+    assert torch.equal(y, want) and torch.equal(norm.running_mean, other.running_mean) and torch.equal(norm.running_var, other.running_var)
+
+
+def test_conv1x1_without_gradients_writes_no_codes(monkeypatch):
+    from mgnet_amd import _C
+    o = ops()
+    x, wt, b, _ = conv_case(2, 64, 33, 20, 24, BF)
+    keep = []
+    fwd = _C.q8_conv1x1_fwd
+    monkeypatch.setattr(_C, "q8_conv1x1_fwd", lambda *a: keep.append(int(a[-1])) or fwd(*a))
+    want = o.conv1x1_q8(x, wt, b)
+    with torch.no_grad():
+        assert torch.equal(o.conv1x1_q8(x, wt, b), want)
+    assert keep == [1, 0]
+
+
+def held(fn):
+    """bytes that stay allocated, and the most that were, while fn() runs; its result"""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    out = fn()
+    torch.cuda.synchronize()
+    return torch.cuda.memory_allocated() - before, torch.cuda.max_memory_allocated() - before, out
+
+
+# (c, cout, map strides): packed on the way, packed in a pass of its own (K > 512; rows that are not contiguous)
+FORMS = [(256, 256, False), (640, 64, False), (256, 64, True)]
+
+
+@pytest.mark.parametrize("c,cout,strided", FORMS)
+def test_frozen_weights_leave_only_packed_weights_waiting(c, cout, strided):
+    """no weight gradient, so the packed input is not kept for the backward pass: what waits is the transposed weights"""
+    o = ops()
+    x, wt, b, dy = conv_case(2, c, 64, 128 if not strided else 256, cout, BF)
+    if strided:
+        x, dy = x.detach()[:, :, :, ::2].requires_grad_(), dy[:, :, :, ::2].contiguous(memory_format=torch.channels_last)
+    full = torch.autograd.grad(o.conv1x1_q8(x, wt, b), (x,), dy)[0]
+    M = x.shape[0] * x.shape[2] * x.shape[3]
+    n, _, y = held(lambda: o.conv1x1_q8(x, wt.detach(), b.detach()))
+    assert n - 2 * M * cout < M * c // 2, (n, M * c)
+    assert torch.equal(torch.autograd.grad(y, (x,), dy)[0], full)
+
+
+@pytest.mark.parametrize("c,cout,strided", FORMS)
+def test_no_gradient_keeps_and_writes_nothing(c, cout, strided):
+    o = ops()
+    x, wt, b, _ = conv_case(2, c, 64, 128 if not strided else 256, cout, BF)
+    if strided:
+        x = x.detach()[:, :, :, ::2].requires_grad_()
+    want = o.conv1x1_q8(x, wt, b).detach()
+    M = x.shape[0] * x.shape[2] * x.shape[3]
+
+    def call():
+        with torch.no_grad():
+            return o.conv1x1_q8(x, wt, b)
+    n, most, y = held(call)
+    assert torch.equal(y, want) and n - 2 * M * cout < 1 << 20
+    if c <= 512 and not strided:         # (packed on the way: no room for the codes is taken at all)
+        assert most - 2 * M * cout < M * c // 2, (most, M * c)
+
+
+def test_sizes_of_the_forward_call():
+    """what a call needs is what it takes: a byte less is refused, and the rest of a larger buffer stays as it was"""
+    import ctypes
+
+    from mgnet_amd import _C
+    M, C, N = 700, 64, 40
+    x, w = rand((M, C), BF, 1), rand((N, C), F32, 2)
+    y = torch.empty((M, N), dtype=BF, device="cuda")
+    need, kept = ctypes.c_size_t(), ctypes.c_size_t()
+    both = torch.full((1 << 20,), 77, dtype=torch.uint8, device="cuda")
+
+    def call(keep, sw, nbytes):
+        return _C.lib().mgn_q8_conv1x1_fwd(x.data_ptr(), M, C, M * sw, sw, 0, M, 1, w.data_ptr(), 0, C, 1, N, None, 0, y.data_ptr(), keep, both.data_ptr(), nbytes,
+                                           _C._stream())
+    first = {}
+    for keep, sw in ((0, C), (1, C), (0, C - 8), (1, C - 8)):       # (rows C - 8 apart overlap: packed in a pass of its own)
+        assert _C.lib().mgn_q8_conv1x1_fwd_bytes(x.data_ptr(), M, C, M * sw, sw, 0, M, 1, N, y.data_ptr(), keep, ctypes.byref(need), ctypes.byref(kept)) == 0
+        assert kept.value <= need.value and (keep or kept.value < 8192) and (need.value < M * C) == (keep == 0 and sw == C)
+        assert call(keep, sw, need.value - 1) == -28
+        both.fill_(77)
+        assert call(keep, sw, need.value) == 0
+        assert bool((both[need.value:] == 77).all())
+        assert torch.equal(y, first.setdefault(sw, y.clone()))
