@@ -830,10 +830,12 @@ int mgn_q8_wgrad(const void* dy, long ldy, long M, int N, const void* codes, con
  * mgn_q8_conv1x1_bytes     : sizes that are enough for every call of M, C, N
  * mgn_q8_conv1x1_fwd_bytes : what this forward call needs (x, strides, y and keep as there), and how many of the buffer's first bytes the
  *                            backward call reads
+ * mgn_q8_conv1x1_bwd_bytes : what the backward call needs for dx and / or dw (scratch may be NULL where that is nothing)
  * dx, dw [N][C], db [N] may be NULL (db only with dw; dw only after keep = 1). */
 int mgn_q8_conv1x1_bytes(long M, int C, int N, size_t* buffer, size_t* scratch);
 int mgn_q8_conv1x1_fwd_bytes(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, int N, const void* y, int keep, size_t* buffer,
                              size_t* kept);
+int mgn_q8_conv1x1_bwd_bytes(long M, int C, int N, int want_dx, int want_dw, size_t* scratch);
 int mgn_q8_conv1x1_fwd(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, const void* w, int w_dtype, long w_sr, long w_sc, int N,
                        const float* bias, int relu, void* y, int keep, void* buffer, size_t buffer_bytes, void* stream);
 int mgn_q8_conv1x1_bwd(const void* dy, long M, int C, int N, const void* buffer, void* dx, float* dw, float* db, void* scratch, size_t scratch_bytes,

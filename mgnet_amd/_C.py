@@ -33,7 +33,7 @@ SYMBOLS = ["mgn_version", "mgn_reproj_workspace_bytes", "mgn_reproj_loss_fwd", "
            "mgn_plan_trace", "mgn_plan_trace_read", "mgn_plan_set_skip", "mgn_plan_node_ro", "mgn_plan_node_ro_family", "mgn_plan_set_jitter", "mgn_plan_probe",
            "mgn_abn_apply_pool", "mgn_att_abn_bwd_stats", "mgn_att_abn_bwd_sums", "mgn_att_abn_bwd_apply",
            "mgn_q8_bytes", "mgn_q8_pack", "mgn_q8_unpack", "mgn_q8_pack_weight", "mgn_q8_matmul", "mgn_q8_pack_matmul", "mgn_q8_wgrad_workspace_bytes", "mgn_q8_wgrad", "mgn_q8_tail_partial_rows", "mgn_q8_tail_stats", "mgn_q8_tail_fwd", "mgn_q8_tail_bwd_reduce", "mgn_q8_tail_sums", "mgn_q8_tail_bwd_apply",
-           "mgn_q8_conv1x1_bytes", "mgn_q8_conv1x1_fwd_bytes", "mgn_q8_conv1x1_fwd", "mgn_q8_conv1x1_bwd", "mgn_q8_tail_workspace_bytes", "mgn_q8_tail_train_fwd", "mgn_q8_tail_train_bwd"]
+           "mgn_q8_conv1x1_bytes", "mgn_q8_conv1x1_fwd_bytes", "mgn_q8_conv1x1_bwd_bytes", "mgn_q8_conv1x1_fwd", "mgn_q8_conv1x1_bwd", "mgn_q8_tail_workspace_bytes", "mgn_q8_tail_train_fwd", "mgn_q8_tail_train_bwd"]
 SYMBOLS_F16 = [n + "_f16" for n in ['mgn_weight_layout', 'mgn_weight_layout_batch', 'mgn_conv_igemm', 'mgn_conv_igemm_stats', 'mgn_conv3x3_win', 'mgn_conv3x3_up2_win', 'mgn_conv_stem7', 'mgn_conv_wgrad', 'mgn_conv_wgrad_partial', 'mgn_conv1x1_cat', 'mgn_conv1x1_split', 'mgn_conv_wgrad_cat', 'mgn_conv3x3_win_act', 'mgn_conv_igemm_act', 'mgn_add_relu_fwd', 'mgn_sum3', 'mgn_abn_add_relu_fwd', 'mgn_relu_mask_bwd', 'mgn_colsum', 'mgn_bcast_rows', 'mgn_scale_channels', 'mgn_nearest_fwd', 'mgn_nearest_bwd', 'mgn_abn_maxpool_fwd', 'mgn_abn_maxpool_bwd', 'mgn_maxpool3x3s2_fwd', 'mgn_maxpool3x3s2_bwd', 'mgn_upce_fwd', 'mgn_upce_bwd', 'mgn_ins_loss_fwd', 'mgn_ins_loss_bwd', 'mgn_prep_input', 'mgn_iabn_stats', 'mgn_iabn_train_coeffs', 'mgn_iabn_apply', 'mgn_iabn_bwd_reduce', 'mgn_iabn_bwd_reduce_x', 'mgn_iabn_bwd_reduce_x_relu', 'mgn_iabn_bwd_apply', 'mgn_iabn_bwd_apply_x', 'mgn_abn_apply_pool', 'mgn_att_abn_bwd_stats', 'mgn_att_abn_bwd_apply', 'mgn_q8_pack', 'mgn_q8_unpack', 'mgn_q8_pack_weight', 'mgn_q8_matmul', 'mgn_q8_pack_matmul', 'mgn_q8_wgrad', 'mgn_q8_tail_stats', 'mgn_q8_tail_fwd', 'mgn_q8_tail_bwd_reduce', 'mgn_q8_tail_bwd_apply', 'mgn_q8_conv1x1_fwd', 'mgn_q8_conv1x1_bwd', 'mgn_q8_tail_train_fwd', 'mgn_q8_tail_train_bwd']]
 DEPTH_MAX_FILTER_IDS = 16
 MGN_MAX_TASKS = 8   # include/mgnet_hip.h
@@ -255,6 +255,7 @@ def lib():
         L.mgn_q8_tail_bwd_apply.argtypes = [vp, vp, vp, vp, vp, vp, vp, cf, cf, cl, ci, vp, vp]
         L.mgn_q8_conv1x1_bytes.argtypes = [cl, ci, ci, ctypes.POINTER(sz), ctypes.POINTER(sz)]
         L.mgn_q8_conv1x1_fwd_bytes.argtypes = [vp, cl, ci, cl, cl, cl, ci, ci, ci, vp, ci, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        L.mgn_q8_conv1x1_bwd_bytes.argtypes = [cl, ci, ci, ci, ci, ctypes.POINTER(sz)]
         L.mgn_q8_conv1x1_fwd.argtypes = [vp, cl, ci, cl, cl, cl, ci, ci, vp, ci, cl, cl, ci, vp, ci, vp, ci, vp, sz, vp]
         L.mgn_q8_conv1x1_bwd.argtypes = [vp, cl, ci, ci, vp, vp, vp, vp, vp, sz, vp]
         L.mgn_q8_tail_workspace_bytes.argtypes = [cl, ci, ctypes.POINTER(sz)]
@@ -1677,22 +1678,25 @@ def q8_matmul(a, M, b, N, K, bias, act, slope, out):
 _Q8_SIZES = {}
 
 
-def _q8_conv_sizes(M, C, N):
-    r = _Q8_SIZES.get((M, C, N))
+def _q8_size(*key):
+    """bytes of a call's buffer or scratch memory: (M, C, N) what a 1x1 convolution keeps, (M, C, N, dx, dw) its backward call, (M, C) the block tail"""
+    r = _Q8_SIZES.get(key)
     if r is None:
         a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
-        check(lib().mgn_q8_conv1x1_bytes(M, C, N, ctypes.byref(a), ctypes.byref(b)), "mgn_q8_conv1x1_bytes")
+        name = {2: "mgn_q8_tail_workspace_bytes", 3: "mgn_q8_conv1x1_bytes", 5: "mgn_q8_conv1x1_bwd_bytes"}[len(key)]
+        check(getattr(lib(), name)(*key, *(ctypes.byref(v) for v in ((a, b) if len(key) == 3 else (a,)))), name)
         if len(_Q8_SIZES) > 4096:
             _Q8_SIZES.clear()
-        r = _Q8_SIZES[(M, C, N)] = (a.value, b.value)
+        r = _Q8_SIZES[key] = a.value
     return r
 
 
 def q8_conv1x1_fwd(x, M, C, sn, sh, sw, H, W, w, N, bias, relu, y, keep):
     """y [M, N] = q(x) q(w)^T + bias [-> ReLU] -> (buffer, how many of its first bytes q8_conv1x1_bwd reads); keep = 0: without the packed x, for no
     weight gradient"""
-    nb = kept = _q8_conv_sizes(M, C, N)[0]
-    if not keep:                # (by the call: whether x is packed on the way goes by its strides and alignment)
+    if keep:
+        nb = kept = _q8_size(M, C, N)
+    else:                       # (by the call: whether x is packed on the way goes by its strides and alignment)
         a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
         check(lib().mgn_q8_conv1x1_fwd_bytes(x.data_ptr(), M, C, sn, sh, sw, H, W, N, y.data_ptr(), 0, ctypes.byref(a), ctypes.byref(b)), "mgn_q8_conv1x1_fwd_bytes")
         nb, kept = a.value, b.value
@@ -1703,19 +1707,14 @@ def q8_conv1x1_fwd(x, M, C, sn, sh, sw, H, W, w, N, bias, relu, y, keep):
 
 
 def q8_conv1x1_bwd(dy, M, C, N, buf, dx, dw, db):
-    nb = _q8_conv_sizes(M, C, N)[1]
+    nb = _q8_size(M, C, N, dx is not None, dw is not None)
     ws = torch.empty(nb, dtype=torch.uint8, device=dy.device)
     p = lambda t: None if t is None else t.data_ptr()
     check(_fn("mgn_q8_conv1x1_bwd", dy)(dy.data_ptr(), M, C, N, buf.data_ptr(), p(dx), p(dw), p(db), ws.data_ptr(), nb, _stream()), "mgn_q8_conv1x1_bwd")
 
 
 def _q8_tail_ws(M, C, device):
-    r = _Q8_SIZES.get((M, C))
-    if r is None:
-        a = ctypes.c_size_t(0)
-        check(lib().mgn_q8_tail_workspace_bytes(M, C, ctypes.byref(a)), "mgn_q8_tail_workspace_bytes")
-        r = _Q8_SIZES[(M, C)] = a.value
-    return torch.empty(r // 4, dtype=torch.float32, device=device)
+    return torch.empty(_q8_size(M, C) // 4, dtype=torch.float32, device=device)
 
 
 def q8_tail_stats(x, M, C):

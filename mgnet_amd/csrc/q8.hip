@@ -1841,17 +1841,19 @@ static ConvBuffer conv_buffer(long M, int C, int N) {
 }
 static bool conv_shape(long M, int C, int N) { return M >= 0 && M <= MAX_ROWS && C >= 1 && C <= 65536 && N >= 1 && N <= 65536; }
 static int pad8(int n) { return (n + 7) & ~7; }
-// what the backward call needs: [dy padded][dy packed, where the product does not pack it on the fly][partial weight gradients]
+// what the backward call needs: [dy padded][dy packed, if the data gradient's product does not pack it on the way][partial weight gradients]
 struct ConvScratch { size_t pad, codes, scales, part, total; };
-static ConvScratch conv_scratch(long M, int C, int N, size_t part_bytes) {
+static ConvScratch conv_scratch(long M, int N, bool pack, size_t part_bytes) {
     ConvScratch b;
     b.pad = 0;
     b.codes = N % 8 ? (size_t)M * pad8(N) * 2 : 0;
-    b.scales = b.codes + (size_t)M * code_ld(N);
-    b.part = b.scales + (size_t)nblocks(N) * scale_ld(M);
+    b.scales = b.codes + (pack ? (size_t)M * code_ld(N) : 0);
+    b.part = b.scales + (pack ? (size_t)nblocks(N) * scale_ld(M) : 0);
     b.total = b.part + part_bytes;
     return b;
 }
+// dy and dx are 16-byte aligned rows (`dy`: the padded rows are in the scratch memory, as well aligned)
+static bool conv_packs_dy(long M, int C, int N, const void* dx) { return !stream_packs(nullptr, M, pad8(N), pad8(N), C, dx, 0, C, 1); }
 
 #ifndef MGN_F16
 int mgn_q8_conv1x1_bytes(long M, int C, int N, size_t* buffer, size_t* scratch) {
@@ -1859,7 +1861,14 @@ int mgn_q8_conv1x1_bytes(long M, int C, int N, size_t* buffer, size_t* scratch) 
     *buffer = conv_buffer(M, C, N).total;
     size_t part = 0;
     if (M > 0) { const int rc = mgn_q8_wgrad_workspace_bytes(M, N, C, &part); if (rc != MGN_OK) return rc; }
-    *scratch = conv_scratch(M, C, N, part).total;
+    *scratch = conv_scratch(M, N, true, part).total;
+    return MGN_OK;
+}
+int mgn_q8_conv1x1_bwd_bytes(long M, int C, int N, int want_dx, int want_dw, size_t* scratch) {
+    if (!conv_shape(M, C, N) || !scratch) return MGN_EINVAL;
+    size_t part = 0;
+    if (M > 0 && want_dw) { const int rc = mgn_q8_wgrad_workspace_bytes(M, N, C, &part); if (rc != MGN_OK) return rc; }
+    *scratch = M > 0 ? conv_scratch(M, N, want_dx && conv_packs_dy(M, C, N, nullptr), part).total : 0;
     return MGN_OK;
 }
 #endif
@@ -1904,14 +1913,15 @@ int MGN_SYM(mgn_q8_conv1x1_fwd)(const void* x, long M, int C, long sn, long sh, 
 
 int MGN_SYM(mgn_q8_conv1x1_bwd)(const void* dy, long M, int C, int N, const void* buffer, void* dx, float* dw, float* db, void* scratch,
                                 size_t scratch_bytes, void* stream_) {
-    size_t need = 0, have = 0, part = 0;
-    int rc = mgn_q8_conv1x1_bytes(M, C, N, &have, &need);
+    if (!conv_shape(M, C, N)) return MGN_EINVAL;
+    size_t part = 0;
+    int rc = dw ? mgn_q8_wgrad_workspace_bytes(M, N, C, &part) : MGN_OK;
     if (rc != MGN_OK) return rc;
-    if (M < 1 || !dy || !buffer || !scratch || (!dx && !dw) || (db && !dw) || !aligned(dy, 16) || !aligned(buffer, 16) || !aligned(scratch, 16)) return MGN_EINVAL;
-    if (scratch_bytes < need) return MGN_ENOSPC;
-    mgn_q8_wgrad_workspace_bytes(M, N, C, &part);
+    if (M < 1 || !dy || !buffer || (!dx && !dw) || (db && !dw) || !aligned(dy, 16) || !aligned(buffer, 16) || !aligned(scratch, 16)) return MGN_EINVAL;
     const ConvBuffer b = conv_buffer(M, C, N);
-    const ConvScratch t = conv_scratch(M, C, N, part);
+    const ConvScratch t = conv_scratch(M, N, dx && conv_packs_dy(M, C, N, dx), part);
+    if (!scratch && t.total) return MGN_EINVAL;
+    if (scratch_bytes < t.total) return MGN_ENOSPC;
     const unsigned char* p = (const unsigned char*)buffer;
     unsigned char* s = (unsigned char*)scratch;
     const int ldy = pad8(N);

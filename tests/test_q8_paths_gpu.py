@@ -143,3 +143,47 @@ def test_sizes_of_the_forward_call():
         assert call(keep, sw, need.value) == 0
         assert bool((both[need.value:] == 77).all())
         assert torch.equal(y, first.setdefault(sw, y.clone()))
+
+
+def test_backward_takes_no_room_for_what_it_does_not_write():
+    """262144 x 256 -> 256: dy is packed on the way, and without a weight gradient there are no partial results"""
+    x, wt, b, dy = conv_case(8, 256, 128, 256, 256, BF)
+    M, o = 262144, ops()
+    y = o.conv1x1_q8(x, wt.detach(), b.detach())        # (autograd.grad for x alone would not tell: needs_input_grad goes by the inputs)
+    _, most, _ = held(lambda: torch.autograd.grad(y, (x,), dy))
+    assert most < 2 * M * 256 + (8 << 20), most
+    y = o.conv1x1_q8(x, wt, b)
+    _, most, _ = held(lambda: torch.autograd.grad(y, (x, wt, b), dy))
+    assert most < 2 * M * 256 + 512 * (4 * 256 * 257 + 4096), most      # (512 row ranges at most)
+
+
+@pytest.mark.parametrize("M,C,N", [(700, 64, 40), (700, 64, 19), (300, 640, 96), (300, 96, 640), (500, 24, 8)])
+def test_sizes_of_the_backward_call(M, C, N):
+    """each combination of gradients runs in the scratch memory that it asks for, not in a byte less, and writes nothing behind it"""
+    import ctypes
+
+    from mgnet_amd import _C
+    x, w, dy = rand((M, C), BF, 1), rand((N, C), F32, 2), rand((M, N), BF, 3)
+    y = torch.empty((M, N), dtype=BF, device="cuda")
+    buf, kept = _C.q8_conv1x1_fwd(x, M, C, M * C, C, 0, M, 1, w, N, None, 0, y, 1)
+    assert kept == buf.numel()
+    most = 0
+    ws, need = torch.empty(8 << 20, dtype=torch.uint8, device="cuda"), ctypes.c_size_t()
+    for want_dx, want_dw in ((1, 1), (1, 0), (0, 1)):
+        assert _C.lib().mgn_q8_conv1x1_bwd_bytes(M, C, N, want_dx, want_dw, ctypes.byref(need)) == 0
+        most = max(most, need.value)
+        dx, dw, db = torch.empty((M, C), dtype=BF, device="cuda"), torch.empty((N, C), device="cuda"), torch.empty(N, device="cuda")
+        p = lambda t, on: t.data_ptr() if on else None  # noqa: E731
+
+        def call(nbytes):
+            return _C.lib().mgn_q8_conv1x1_bwd(dy.data_ptr(), M, C, N, buf.data_ptr(), p(dx, want_dx), p(dw, want_dw), p(db, want_dw), ws.data_ptr(), nbytes, _C._stream())
+        if need.value:
+            assert call(need.value - 1) == -28
+        ws.fill_(77)
+        assert call(need.value) == 0
+        assert bool((ws[need.value:] == 77).all())
+        if want_dx and want_dw:
+            full = (dx, dw, db)
+        assert (not want_dx or torch.equal(dx, full[0])) and (not want_dw or (torch.equal(dw, full[1]) and torch.equal(db, full[2])))
+    a, b = ctypes.c_size_t(), ctypes.c_size_t()
+    assert _C.lib().mgn_q8_conv1x1_bytes(M, C, N, ctypes.byref(a), ctypes.byref(b)) == 0 and b.value >= most     # (enough for every call)
