@@ -1,6 +1,6 @@
 """Build libmgnet_hip.so (all csrc/*.hip, gfx950) in-tree with hipcc.  `python -m mgnet_amd.build [--force]`.
 
-Every source is compiled to its own object (in parallel, re-done only when the source or a header is newer) and the
+Every source is compiled to its own object (in parallel, re-done only when the source, a header or this file with its flags is newer) and the
 objects are linked into one shared library; the kernels of different files never reference each other."""
 import glob
 import os
@@ -8,7 +8,8 @@ import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
 
-HERE = os.path.dirname(os.path.abspath(__file__))
+SELF = os.path.abspath(__file__)   # (its flags are part of what an object is made from)
+HERE = os.path.dirname(SELF)
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "lib", "libmgnet_hip.so")
 OBJ = os.path.join(HERE, "lib", "obj")
@@ -36,14 +37,14 @@ def _stale(target, deps):
 
 
 def is_stale():
-    return _stale(LIB, sources() + headers())
+    return _stale(LIB, sources() + headers() + [SELF])
 
 
 def build(force=False, verbose=False):
     if not force and not is_stale():
         return LIB
     os.makedirs(OBJ, exist_ok=True)
-    hdr = headers()
+    hdr = headers() + [SELF]
     base = lambda s: [s[:-8] + ".hip"] if s.endswith("_f16.hip") else []   # x_f16.hip = `#define MGN_F16` + `#include "x.hip"`
     todo = [s for s in sources() if force or _stale(_obj(s), [s] + base(s) + hdr)]
 
