@@ -56,3 +56,13 @@ def test_forced(tree):
     run, _ = tree
     run()
     assert run(force=True) == ["a.hip", "a_f16.hip", "b.hip"]
+
+
+def test_the_entry_point_compiles_each_time(monkeypatch):
+    import __graft_entry__ as g
+    from mgnet_amd import build
+    calls = []
+    monkeypatch.setattr(build, "build", lambda **kw: calls.append(kw))
+    g.build()
+    g.build()
+    assert [kw.get("force") for kw in calls] == [True, True]
