@@ -1,4 +1,4 @@
-"""Build libmgnet_hip.so (all csrc/*.hip, gfx950) in-tree with hipcc.  `python -m mgnet_amd.build [--force]`.
+"""Build libmgnet_hip.so (all csrc/*.hip, gfx950) in-tree with hipcc.  `python -m mgnet_amd.build [--force | --flags]`.
 
 Every source is compiled to its own object (in parallel, re-done only when the source, a header or this file with its flags is newer) and the
 objects are linked into one shared library; the kernels of different files never reference each other."""
@@ -73,4 +73,7 @@ def build(force=False, verbose=False):
 
 
 if __name__ == "__main__":
+    if "--flags" in sys.argv:        # (for a build of single sources: tools/build_variant.sh)
+        print(" ".join(CFLAGS))
+        sys.exit(0)
     print(build(force="--force" in sys.argv, verbose=True))

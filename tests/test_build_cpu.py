@@ -66,3 +66,25 @@ def test_the_entry_point_compiles_each_time(monkeypatch):
     g.build()
     g.build()
     assert [kw.get("force") for kw in calls] == [True, True]
+
+
+def test_a_variant_is_built_with_the_librarys_flags(tmp_path):
+    """tools/build_variant.sh compiles one source by itself: with the flags that every object of the library has"""
+    import subprocess
+
+    from conftest import ROOT
+    from mgnet_amd import build
+    (tmp_path / "tools").mkdir()
+    (tmp_path / "tools" / "build_variant.sh").write_text(open(os.path.join(ROOT, "tools", "build_variant.sh")).read())
+    for name in ("mgnet_amd", "include"):
+        os.symlink(os.path.join(ROOT, name), tmp_path / name)
+    cc = tmp_path / "cc"
+    cc.write_text('#!/bin/sh\necho "$@" >> %s\n' % (tmp_path / "log"))
+    cc.chmod(cc.stat().st_mode | stat.S_IXUSR)
+    subprocess.run(["bash", str(tmp_path / "tools" / "build_variant.sh"), "x", "q8.hip", "-DX"], check=True, env=dict(os.environ, HIPCC=str(cc)), stdout=subprocess.DEVNULL)
+    lines = [line.split() for line in open(tmp_path / "log") if " -c " in line]
+    assert lines and all("-DX" in line for line in lines)
+    for line in lines:
+        k = line.index("-packed-fp32-ops")
+        assert line[k - 3:k + 1] == ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+        assert [f for f in build.CFLAGS if f.startswith("-O") or f.startswith("-std")] == [f for f in line if f.startswith("-O") or f.startswith("-std")]

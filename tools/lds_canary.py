@@ -33,7 +33,7 @@ d = tempfile.mkdtemp()
 open(os.path.join(d, "canary.hip"), "w").write(SRC)
 so = os.path.join(ROOT, "tools", "probe", "libcanary.so")
 if not os.path.exists(so) or os.environ.get("REBUILD"):
-    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O2", "-shared", "-fPIC", os.path.join(d, "canary.hip"), "-o", so], check=True)
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O2", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-shared", "-fPIC", os.path.join(d, "canary.hip"), "-o", so], check=True)
 if not torch.cuda.is_available():
     print("built", so); sys.exit(0)
 lib = ctypes.CDLL(so)
