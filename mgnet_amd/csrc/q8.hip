@@ -1896,7 +1896,8 @@ int mgn_q8_conv1x1_fwd_bytes(const void* x, long M, int C, long sn, long sh, lon
 
 int MGN_SYM(mgn_q8_conv1x1_fwd)(const void* x, long M, int C, long sn, long sh, long sw, int H, int W, const void* w, int w_dtype, long w_sr, long w_sc,
                                 int N, const float* bias, int relu, void* y, int keep, void* buffer, size_t buffer_bytes, void* stream_) {
-    if (!conv_shape(M, C, N) || !w || (!y && M > 0) || !buffer || !aligned(buffer, 16)) return MGN_EINVAL;
+    if (!conv_shape(M, C, N) || !w || !buffer || !aligned(buffer, 16)) return MGN_EINVAL;
+    if (M > 0 && (!x || !y || H < 1 || W < 1 || M % ((long)H * W) != 0 || sn < 0 || sh < 0 || sw < 0 || !aligned(x, 2) || !aligned(y, 2))) return MGN_EINVAL;
     const ConvBuffer b = conv_buffer(M, C, N);
     if (buffer_bytes < (conv_unkept(x, M, C, sn, sh, sw, H, W, N, y, keep) ? b.codes : b.total)) return MGN_ENOSPC;
     unsigned char* p = (unsigned char*)buffer;
