@@ -804,12 +804,15 @@ int mgn_project_bwd(const float* points, const float* A, const float* t, const f
  * mgn_q8_unpack     : the values, y [M][C] contiguous (dtype as above).
  * mgn_q8_pack_weight: w [N][K] with element strides sr, sc -> tile scales; codes/scales of [N][K] and / or codes_t/scales_t of its
  *                     transpose [K][N] (the same values).  A pair may be NULL.
- * mgn_q8_matmul     : out[m][n] = act( sum_k a[m][k] b[n][k] + bias[n] ), a [M][K], b [N][K] packed, fp32 accumulation, one rounding;
+ * mgn_q8_matmul     : out[m][n] = act( sum_k a[m][k] b[n][k] + bias[n] ), a [M][K], b [N][K] packed, one rounding to out.  The sum: the
+ *                     matrix instruction adds the products of 8 neighbouring k, each cut to a multiple of 2^-13 of the largest one's
+ *                     binade, and such sums are accumulated in fp32: off by some 1.3e-5 of a result, more than a sum in fp32 alone;
  *                     act 0 none | 1 ReLU | 2 leaky ReLU (0 <= slope <= 1); out fp32 or 16-bit, rows ldo elements
  *                     apart.
  * mgn_q8_pack_matmul: mgn_q8_pack of the 16-bit matrix x [M][K] (rows ldx elements apart) and mgn_q8_matmul of its packed form in one pass
  *                     over x; codes / scales: where the packed form is kept, or both NULL.  MGN_ENOTSUP (nothing done; pack first then):
- *                     K > 512, K % 8 or ldx % 8 != 0, x not 16-byte aligned; N > 32 with N % 8 or ldo % 8 != 0 or an fp32 result.  Same result as the two calls up to the order of the fp32 sums.
+ *                     K > 512, K % 8 or ldx % 8 != 0, x not 16-byte aligned; N > 32 with N % 8 or ldo % 8 != 0, an fp32 result or out not
+ *                     16-byte aligned; N > 8192 (16384 for K <= 256); M > 2^29.  Same result as the two calls up to the order of the sums.
  * mgn_q8_wgrad      : dw[n][k] = sum_m dy[m][n] x[m][k] with dy 16-bit (rows ldy elements apart, ldy % 8 == 0, 16-byte aligned; columns
  *                     N .. ldy are ignored) and x packed; db[n] = sum_m dy[m][n] (nullable).  Fixed summation order.
  * ---------------------------------------------------------------------------------------------- */

@@ -1075,8 +1075,9 @@ __global__ __launch_bounds__(TPB) void q8_mm_small(MmParams p) {
 //   registers, where a value and its scale become the exact 16-bit x^ (one instruction for two); both tiles are read back with the
 //   transposing LDS reads, since the summed index is the row.  Loads run two steps ahead (80 KB of LDS: two blocks a CU).
 //   v_mfma_f32_32x32x16, fp32 accumulation; the splits' tiles are added by q8_wgrad_reduce in order.
-//   262144 x 256 x 256: 54-59 us, 3.6 TB/s (201 MB, each byte read once: 39 us at the rate of a copy, 50 at the 4.0 TB/s that reading alone
-//   reaches here), and 9 us for the reduction of 128 partial results (34 MB).  Matrix cores 37 % busy, a quarter of the LDS cycles conflicts.
+//   262144 x 256 x 256: 54-59 us, 3.6 TB/s (201 MB, each byte read once: 39 us at the rate of a copy, 41 at the 4.9 TB/s that a pass of this
+//   library which only reads reaches on 537 MB), and 9 us for the reduction of 128 partial results (34 MB).  Neither memory nor matrix cores
+//   (37 % busy) are full; a quarter of the LDS cycles are conflicts.
 //   db: the same dy fragments times a column of ones, in the blocks of the first k tile.
 // ------------------------------------------------------------------------------------------------------
 struct WgradParams8 {
@@ -1313,8 +1314,8 @@ __global__ __launch_bounds__(TPB) void q8_pad_rows(const uint16_t* __restrict__ 
 // block of 128 channels, LPB lanes (8 channels each) per row -- a thread's channels never change, so their coefficients stay in
 // registers.  All are bound by HBM: 1048576 x 64 bf16, 134 MB a tensor: statistics 35 us (134 MB), forward 80 (478 MB, 6.0 TB/s), backward
 // sums 63 (344 MB, 5.4 TB/s), dx 56 (336 MB, 6.0 TB/s); joining the partial sums 5 and 5 us, two launches of latency.
-// Reading alone is slower than copying: a library sum reads 134 MB at 3.2 TB/s, 2 GB at 4.0; the statistics read at 3.9 with 512 row blocks, at
-// 3.4 with 1024 or 2048.
+// The statistics read 134 MB at 3.9 TB/s with 512 row blocks, at 3.4 with 1024 or 2048; iabn.hip's statistics pass reads 134 MB at 4.0 and 537 MB
+// at 4.9.
 // ------------------------------------------------------------------------------------------------------
 constexpr int TAIL_BLOCKS = 512;          // row blocks of the two reductions (= partial rows)
 

@@ -107,7 +107,8 @@ _ACT = {"none": 0, "relu": 1, "leaky_relu": 2}
 
 def q8_matmul(a, b, bias=None, act="none", slope=0.01, out_dtype=None):
     """act(a b^T + bias) of two packed matrices a [M, K] (or a map [N, K, H, W]: the result is the map [N, n, H, W]) and b [n, K]; products
-    of codes scaled in the matrix cores, fp32 accumulation, one rounding to out_dtype (default: a's source type).  act: none | relu |
+    of codes scaled in the matrix cores, one rounding to out_dtype (default: a's source type).  The matrix cores cut the products of 8
+    neighbouring k to 2^-13 of the largest one's binade before they join the fp32 sum: 1.3e-5 of a result, which a float32 one shows.  act: none | relu |
     leaky_relu (0 <= slope <= 1).  No gradient (conv1x1_q8 has one)."""
     if not (isinstance(a, Q8Map) and isinstance(b, Q8Map)):
         raise ValueError("q8_matmul: two Q8Map operands (ops.q8_pack)")
@@ -198,8 +199,8 @@ class _Conv1x1Q8Fn(torch.autograd.Function):
 
 def conv1x1_q8(x, weight, bias=None, relu=False):
     """A 1x1 convolution (stride 1) trained in 8 bits: y = q(x) q(W)^T + bias [-> ReLU], dx = q(dy) q(W), dW = dy^T q(x), db = sum dy, with
-    q(.) the block format of q8_pack (x and dy per 128 channels of a pixel, W per 128 x 128 tile), products accumulated in fp32.  Of the
-    input only its packed form is kept for the backward pass.
+    q(.) the block format of q8_pack (x and dy per 128 channels of a pixel, W per 128 x 128 tile), sums as in
+    q8_matmul (dW and db: fp32).  Of the input only its packed form is kept for the backward pass, and not that where no weight wants a gradient.
     x [N, C, H, W] bfloat16 / float16 (any strides; the result is channels-last), weight [Cout, C, 1, 1], bias [Cout] or None."""
     _check_source(x, "conv1x1_q8")
     C = x.shape[1]
