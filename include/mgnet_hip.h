@@ -847,9 +847,9 @@ int mgn_q8_conv1x1_bwd(const void* dy, long M, int C, int N, const void* buffer,
  * 16-bit, 16-byte aligned, C % 8 == 0, C <= 8192.
  *   stats      : partials[rows][C][2] (rows = mgn_q8_tail_partial_rows) of (x - shift), (x - shift)^2 and shift[C] = the mean of some 64 .. 256 rows, the
  *                input of mgn_iabn_coeffs_from_partials
- *   fwd        : y = relu(scale * x + offset + shortcut) (one rounding), x packed, relu_bits: one byte per 8 outputs, bit k = (y[k] > 0);
+ *   fwd        : y = relu(scale * x + offset + shortcut) (one rounding), x packed, relu_bits: one byte per 8 outputs, bit k = (y[k] > 0 or NaN);
  *                codes, scales and relu_bits all NULL: y alone (inference)
- *   bwd_reduce : dz = g * (y > 0) (the shortcut's gradient); sums[2][C] = { sum dz, sum dz * x_hat } with x_hat = (packed x - mean) * rstd;
+ *   bwd_reduce : dz = g where its bit is set, 0 elsewhere (the shortcut's gradient); sums[2][C] = { sum dz, sum dz * x_hat } with x_hat = (packed x - mean) * rstd;
  *                dwb[2][C] = { d weight, d bias } of this rank; partials as above (scratch)
  *   bwd_apply  : dx = (|weight| + eps) * rstd * (dz - sums[0] / n - x_hat * sums[1] / n), n = total_count (all ranks) */
 int mgn_q8_tail_partial_rows(long M, int C, int* rows);
