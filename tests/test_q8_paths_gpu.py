@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_q8_gpu import BF, conv_case, F32, HF, ops, rand, rows, tail_case
+from test_q8_gpu import BF, conv_case, F32, group_tol, HF, ops, q8_ref, rand, rand_map, rows, tail_case
 
 pytestmark = pytest.mark.gpu
 
@@ -187,3 +187,163 @@ def test_sizes_of_the_backward_call(M, C, N):
         assert (not want_dx or torch.equal(dx, full[0])) and (not want_dw or (torch.equal(dw, full[1]) and torch.equal(db, full[2])))
     a, b = ctypes.c_size_t(), ctypes.c_size_t()
     assert _C.lib().mgn_q8_conv1x1_bytes(M, C, N, ctypes.byref(a), ctypes.byref(b)) == 0 and b.value >= most     # (enough for every call)
+
+
+# ---- calls that the documentation allows -------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("case", ["both_axes", "rows_expanded", "columns_expanded", "transposed_view", "one_column", "one_row", "offset"])
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_weight_tiles_of_any_strides(case, dtype):
+    big = rand((300, 420), dtype, 3)
+    w = {"both_axes": lambda: big[::2, ::3], "rows_expanded": lambda: big[:1].expand(150, 420), "columns_expanded": lambda: big[:, :1].expand(300, 140),
+         "transposed_view": lambda: big.t()[5:, 3:], "one_column": lambda: big[:, 7:8], "one_row": lambda: big.t()[9:10], "offset": lambda: big[1:, 1:]}[case]()
+    q, ref = ops().q8_pack(w, tile=True), ops().q8_pack(w.clone(memory_format=torch.contiguous_format), tile=True)
+    assert torch.equal(q.codes, ref.codes) and torch.equal(q.scales[:, :w.shape[0]], ref.scales[:, :w.shape[0]])
+
+
+@pytest.mark.parametrize("wd", [BF, HF])
+def test_conv1x1_with_16_bit_parameters(wd):
+    """the parameters' values in another type: the same results, gradients in the parameters' type"""
+    o = ops()
+    x, wt, b, dy = conv_case(2, 72, 11, 13, 40, BF)
+    wt, b = (t.detach().to(wd).requires_grad_() for t in (wt, b))
+    w32, b32 = (t.detach().float().requires_grad_() for t in (wt, b))
+    y, ref = o.conv1x1_q8(x, wt, b), o.conv1x1_q8(x, w32, b32)
+    assert torch.equal(y, ref)
+    for p, q, t in zip(torch.autograd.grad(y, (x, wt, b), dy), torch.autograd.grad(ref, (x, w32, b32), dy), (x, wt, b)):
+        assert p.dtype == t.dtype and torch.equal(p, q.to(t.dtype))
+
+
+def test_conv1x1_with_a_transposed_weight():
+    o = ops()
+    x, wt, b, dy = conv_case(1, 64, 9, 10, 48, BF)
+    t = wt.detach().transpose(0, 1).contiguous().requires_grad_()
+    y, ref = o.conv1x1_q8(x, t.transpose(0, 1), b), o.conv1x1_q8(x, wt, b)
+    assert torch.equal(y, ref)
+    assert torch.equal(torch.autograd.grad(y, (t,), dy)[0].transpose(0, 1), torch.autograd.grad(ref, (wt,), dy)[0])
+
+
+def test_backward_twice_and_results_overwritten():
+    """a graph that is kept gives the same gradients again, also after inputs and results have been written over (neither is kept, but for the result that
+    a ReLU masks by)"""
+    o = ops()
+    x, wt, b, dy = conv_case(2, 64, 9, 10, 48, BF)
+    y = o.conv1x1_q8(x * 1, wt, b)
+    first = torch.autograd.grad(y, (x, wt, b), dy, retain_graph=True)
+    with torch.no_grad():
+        y.zero_(), wt.zero_(), b.zero_()
+    assert all(torch.equal(p, q) for p, q in zip(first, torch.autograd.grad(y, (x, wt, b), dy)))
+    y = o.conv1x1_q8(x, wt, b, relu=True)
+    with torch.no_grad():
+        y.add_(1)
+    with pytest.raises(RuntimeError):           # (autograd sees it)
+        torch.autograd.grad(y, (x,), dy)
+    x, norm, s, g = tail_case(2, 40, 7, 9, BF)
+    leaves = (x, s, norm.weight, norm.bias)
+    y = o.abn_add_relu_q8(x * 1, norm, s * 1)
+    first = torch.autograd.grad(y, leaves, g, retain_graph=True)
+    with torch.no_grad():
+        y.zero_(), x.zero_(), s.zero_()
+    assert all(torch.equal(p, q) for p, q in zip(first, torch.autograd.grad(y, leaves, g)))
+
+
+def test_block_tail_of_one_map_twice():
+    """the input as its own shortcut: the gradients of both places add up"""
+    o = ops()
+    x, norm, _, g = tail_case(2, 72, 9, 8, BF, 6)
+    import copy
+    other = copy.deepcopy(norm)
+    s = x.detach().clone(memory_format=torch.channels_last).requires_grad_()
+    y, ref = o.abn_add_relu_q8(x, norm, x), o.abn_add_relu_q8(x, other, s)
+    assert torch.equal(y, ref)
+    dx, ds = torch.autograd.grad(ref, (x, s), g)
+    assert torch.equal(torch.autograd.grad(y, (x,), g)[0], dx + ds)
+
+
+def test_one_map_into_two_convolutions():
+    """two consumers of a map on two streams at once, both backward passes: each call has buffers of its own"""
+    o = ops()
+    x, w1, b1, d1 = conv_case(4, 128, 40, 60, 64, BF, seed=1)
+    _, w2, b2, d2 = conv_case(4, 128, 40, 60, 200, BF, seed=2)
+    want = [torch.autograd.grad(o.conv1x1_q8(x, w, b), (x, w, b), d) for w, b, d in ((w1, b1, d1), (w2, b2, d2))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        torch.cuda.synchronize()
+        got = []
+        for st, w, b, d in zip(streams, (w1, w2), (b1, b2), (d1, d2)):
+            with torch.cuda.stream(st):
+                got.append(torch.autograd.grad(o.conv1x1_q8(x, w, b), (x, w, b), d))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for a, b in zip(got, want) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("c,cout", [(96, 40), (640, 48)])       # (packed on the way, and in a pass of its own whose codes go)
+def test_captured_with_frozen_weights(c, cout):
+    o = ops()
+    x, wt, b, dy = conv_case(2, c, 14, 10, cout, BF)
+    wt, b = wt.detach(), b.detach()
+    x = x.detach().requires_grad_()
+
+    def step():
+        y = o.conv1x1_q8(x, wt, b, relu=True)
+        return y.detach(), torch.autograd.grad(y, (x,), dy)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            out = step()
+    torch.cuda.current_stream().wait_stream(side)
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for rep in range(4):
+        with torch.no_grad():
+            x.copy_(rand_map(2, c, 14, 10, BF, 100 + rep))
+            wt.copy_(rand((cout, c), F32, 200 + rep, 0.2).view(cout, c, 1, 1) / math.sqrt(c))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(p, q) for p, q in zip(step(), got)), rep
+
+
+def test_saved_on_the_host_and_recomputed():
+    """what waits may wait elsewhere (saved-tensor hooks), or not at all (recomputation)"""
+    from torch.utils.checkpoint import checkpoint
+    o = ops()
+    x, wt, b, dy = conv_case(2, 64, 9, 10, 48, BF)
+    want = torch.autograd.grad(o.conv1x1_q8(x, wt, b, True), (x, wt, b), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = o.conv1x1_q8(x, wt, b, True)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, wt, b), dy), want))
+    y = checkpoint(lambda x: o.conv1x1_q8(x, wt, b, True), x, use_reentrant=False)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, wt, b), dy), want))
+    x, norm, s, g = tail_case(2, 40, 7, 9, HF)
+    leaves = (x, s, norm.weight, norm.bias)
+    want = torch.autograd.grad(o.abn_add_relu_q8(x, norm, s), leaves, g)
+    with torch.autograd.graph.save_on_cpu():
+        y = o.abn_add_relu_q8(x, norm, s)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, g), want))
+
+
+def test_product_of_operands_the_other_way_round():
+    """row scales and tile scales on either side, a bias that is a view, a result in another type than the source's"""
+    o = ops()
+    a, b = rand((200, 130), HF, 1), rand((72, 130), F32, 2)
+    bias = rand((72, 2), F32, 3, 0.0)[:, 1]
+    one = o.q8_matmul(o.q8_pack(a), o.q8_pack(b, tile=True), bias, out_dtype=F32)
+    other = o.q8_matmul(o.q8_pack(b, tile=True), o.q8_pack(a), out_dtype=F32).t() + bias
+    av, bv = q8_ref(a)[0], q8_ref(b, True)[0]
+    tol = (132 + 2) * 2.0 ** -23 * (av.abs() @ bv.abs().t() + bias.abs().double()) + group_tol(av, bv) + 2.0 ** -22 * bias.abs().double()
+    for y in (one, other):
+        assert bool(((y.double() - av @ bv.t() - bias.double()).abs() <= tol).all())
+    assert torch.equal(o.q8_matmul(o.q8_pack(a), o.q8_pack(b, tile=True), bias), one.half())
+
+
+def test_block_tail_masks_what_is_not_finite():
+    o = ops()
+    x, norm, s, g = tail_case(2, 72, 9, 8, HF, 9)
+    y = o.abn_add_relu_q8(x, norm, s)
+    off, leaves = y.detach() == 0, (x, s, norm.weight, norm.bias)
+    want = torch.autograd.grad(y, leaves, g.masked_fill(off, 0.0), retain_graph=True)
+    for v in (math.inf, math.nan):
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, g.masked_fill(off, v), retain_graph=True), want)), v
